@@ -124,6 +124,18 @@ _SIGS = {
     "dimq_soft_dequantize_forward": (_int, [_vp, _int, _i64, _vp, _i64, _dbl, _vp, _vp, _vp]),
     "dimq_soft_dequantize_backward": (_int, [_vp, _int, _i64, _vp, _i64, _dbl, _vp, _vp, _int, _vp, _int, _vp, _vp,
                                              _i64, _vp]),
+    "dimq_mx_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "dimq_mx_dequantize": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _int, _vp]),
+    "dimq_mxfp4_linear_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "dimq_mxfp4_linear": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _i64, _vp, _int, _vp, _int, _int, _vp,
+                                 _vp, _vp, _i64, _vp]),
+    "dimq_mx_grad_input_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64]),
+    "dimq_mxfp4_linear_grad_input": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _int, _vp, _i64, _vp]),
+    "dimq_mx_grad_weight_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64]),
+    "dimq_mx_linear_grad_weight": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _int, _vp, _int, _vp, _i64,
+                                          _vp]),
+    "dimq_mx_gelu_forward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "dimq_mx_gelu_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "dimq_separation_loss": (_int, [_vp, _int, _i64, _vp, _i64, _dbl, _dbl, _vp, _vp, _vp, _i64, _vp]),
 }
 

@@ -1,0 +1,328 @@
+// Microscaled formats (mx.h): quantization to 4 and 8 bits, the way back, and GELU with its input kept in 8 bits.
+#include "mx.h"
+
+namespace dimq {
+namespace {
+
+// n / d for n < 2^31 as (n * mul) >> shift: mul = ceil(2^(31 + s) / d), s = ceil(log2 d), is above the quotient by less
+// than 2^-(31 + s) of it, which times n stays below 1 / d.
+struct FastDiv {
+  uint32_t mul = 0, shift = 0, d = 1;
+  explicit FastDiv(uint32_t div) : d(div) {
+    uint32_t s = 0;
+    while ((1ull << s) < div) ++s;
+    shift = 31 + s;
+    mul = (uint32_t)(((1ull << shift) + div - 1) / div);
+  }
+  __device__ __forceinline__ uint32_t quot(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> shift); }
+};
+
+template <int DT>
+__device__ __forceinline__ float scalar_load(const void* p, int64_t i) {
+  return load_as_float(p, DT, i);
+}
+
+// Elements c .. c + 7 of a row of `cols` as fp32, zeros past its end.  VEC: the row is 16-byte aligned and cols % 8 == 0.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* x, int64_t at, int64_t c, int64_t cols, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (c >= cols) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    } else if constexpr (DT == DIMQ_F32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at + c);
+      const float4 a = p[0], b = p[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at + c);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = DT == DIMQ_F16 ? f16_bits_to_float(w[j] & 0xffffu) : bf16_bits_to_float(w[j] & 0xffffu);
+        v[2 * j + 1] = DT == DIMQ_F16 ? f16_bits_to_float(w[j] >> 16) : bf16_bits_to_float(w[j] >> 16);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? scalar_load<DT>(x, at + c + j) : 0.0f;
+  }
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(void* y, int64_t at, int64_t c, int64_t cols, const float (&v)[8]) {
+  if constexpr (VEC) {
+    if (c >= cols) return;
+    if constexpr (DT == DIMQ_F32) {
+      float4* p = reinterpret_cast<float4*>(static_cast<float*>(y) + at + c);
+      p[0] = make_float4(v[0], v[1], v[2], v[3]);
+      p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = DT == DIMQ_F16 ? f16x2_rne(v[2 * j], v[2 * j + 1]) : bf16x2_rne(v[2 * j], v[2 * j + 1]);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + at + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) store_from_float(y, DT, at + c + j, v[j]);
+  }
+}
+
+// Largest magnitude of a block's four lanes, as fp32 bits: integer order is the magnitudes' order, NaN above all.
+__device__ __forceinline__ uint32_t quad_max(uint32_t m) {
+  const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true);  // lanes 1 0 3 2
+  m = m > a ? m : a;
+  const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true);  // lanes 2 3 0 1
+  return m > b ? m : b;
+}
+
+// Eight fp32 values -> 8-bit codes in two dwords: v 2^(133 - byte) is exact or, below any rounding step, flushed;
+// clamped first (127.5 and more would round to 128), then rounded to nearest even by adding 1.5 * 2^23.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], uint32_t byte) {
+  uint32_t b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float t = __builtin_amdgcn_fmed3f(ldexpf(v[j], 133 - (int)byte), -127.0f, 127.0f);
+    b[j] = __float_as_uint(t + 12582912.0f);
+  }
+  uint2 w;
+  w.x = perm(perm(b[3], b[2], 0x00000400u), perm(b[1], b[0], 0x00000400u), 0x05040100u);
+  w.y = perm(perm(b[7], b[6], 0x00000400u), perm(b[5], b[4], 0x00000400u), 0x05040100u);
+  return w;
+}
+
+struct QuantArgs {
+  const void* x;
+  int64_t ldx, rows, cols;
+  uint8_t* codes4;   // rows of blocks * 16 bytes
+  uint8_t* scales4;
+  int8_t* codes8;    // rows of blocks8 * 32 bytes
+  uint8_t* scales8;
+  int64_t blocks, blocks8;  // blocks a row takes in the 4-bit output (the padded ones are zeros) and in the 8-bit one
+  void* y;           // GELU's output rows of cols
+};
+
+// A lane takes eight elements, four lanes a block: loads of 16 bytes and stores of 4, 8 and 16 next to one another
+// across the wave, the block's maximum by two lane exchanges.  Bound by the bytes: 4096 x 4096 fp32 to both formats
+// moves 67 MB in and 26 MB out.
+template <int XT, bool VEC, bool Q4, bool Q8, bool GELU>
+__global__ __launch_bounds__(256) void mx_quant_kernel(QuantArgs a, FastDiv div, uint32_t units) {
+  const uint32_t u = (blockIdx.x * 256u + threadIdx.x) >> 2;
+  if (u >= units) return;  // whole blocks: the four lanes leave together
+  const uint32_t q = threadIdx.x & 3u, row = div.quot(u), blk = u - row * div.d;
+  const int64_t c = (int64_t)blk * kMxBlock + q * 8;
+  float v[8];
+  load8<XT, VEC>(a.x, row * a.ldx, c, a.cols, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t m = __float_as_uint(v[j]) & 0x7fffffffu;
+    top = top > m ? top : m;
+  }
+  top = quad_max(top);
+  if constexpr (Q4) {
+    const uint32_t byte = mx_scale_byte<2>(top);
+    const int64_t b = (int64_t)row * a.blocks + blk;
+    reinterpret_cast<uint32_t*>(a.codes4)[b * 4 + q] = byte == kMxNan ? 0u : mx_codes4(v, mx_scale_operand(byte));
+    if (q == 0) a.scales4[b] = (uint8_t)byte;
+  }
+  if constexpr (Q8) {
+    if (blk < a.blocks8) {
+      const uint32_t byte = mx_scale_byte<0>(top);
+      const int64_t b = (int64_t)row * a.blocks8 + blk;
+      reinterpret_cast<uint2*>(a.codes8)[b * 4 + q] = byte == kMxNan ? make_uint2(0u, 0u) : codes8(v, byte);
+      if (q == 0) a.scales8[b] = (uint8_t)byte;
+    }
+  }
+  if constexpr (GELU) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = mx_gelu<XT == DIMQ_F32>(v[j]);
+    store8<XT, VEC>(a.y, row * a.cols, c, a.cols, y);
+  }
+}
+
+template <int BITS>
+__device__ __forceinline__ void decode8(const void* codes, uint32_t byte, int64_t unit, float (&v)[8]) {
+  if constexpr (BITS == 4) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const uint32_t w = static_cast<const uint32_t*>(codes)[unit];
+    const float s = mx_scale_operand(byte);
+    const f2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+    const f2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+    v[0] = p0.x; v[1] = p0.y; v[2] = p1.x; v[3] = p1.y;
+    v[4] = p2.x; v[5] = p2.y; v[6] = p3.x; v[7] = p3.y;
+  } else {
+    const uint2 w = static_cast<const uint2*>(codes)[unit];
+    const float s = mx_step8(byte);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * s;
+  }
+}
+
+struct BackArgs {
+  const void* codes;
+  const uint8_t* scales;
+  int64_t cols;
+  const void* g;  // GELU's upstream gradient (rows of ldg), null for the plain way back
+  int64_t ldg;
+  void* y;
+};
+
+// Codes to values (SLOPE 0), or the upstream gradient times GELU's slope at them.  Eight elements a lane, as above.
+template <int BITS, int YT, bool VEC, bool SLOPE>
+__global__ __launch_bounds__(256) void mx_back_kernel(BackArgs a, FastDiv div, uint32_t units) {
+  const uint32_t u = (blockIdx.x * 256u + threadIdx.x) >> 2;
+  if (u >= units) return;
+  const uint32_t q = threadIdx.x & 3u, row = div.quot(u), blk = u - row * div.d;
+  const int64_t c = (int64_t)blk * kMxBlock + q * 8, b = (int64_t)u;
+  float v[8];
+  decode8<BITS>(a.codes, a.scales[b], b * 4 + q, v);
+  if constexpr (SLOPE) {
+    float g[8];
+    load8<YT, VEC>(a.g, row * a.ldg, c, a.cols, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = g[j] * mx_gelu_slope<YT == DIMQ_F32>(v[j]);
+  }
+  store8<YT, VEC>(a.y, row * a.cols, c, a.cols, v);
+}
+
+bool vec_rows(const void* p, int dt, int64_t cols, int64_t ld) {
+  return aligned(p, 16) && cols % 8 == 0 && (ld * dtype_size(dt)) % 16 == 0;
+}
+
+// Units of a launch stay below 2^29 (FastDiv, grid of 2^31 threads): more rows go in several.
+template <typename F>
+int launch_rows(int64_t rows, int64_t blocks, const char* what, F&& f) {
+  DIMQ_CHECK(blocks < (1 << 29), "%s: rows of %lld blocks are not supported", what, (long long)blocks);
+  const int64_t step = (1 << 29) / blocks;
+  for (int64_t r = 0; r < rows; r += step) {
+    const int64_t n = rows - r < step ? rows - r : step;
+    const uint32_t units = (uint32_t)(n * blocks);
+    f(r, FastDiv((uint32_t)blocks), units, dim3((units + 63) / 64));
+    const int rc = check_launch(what);
+    if (rc != DIMQ_OK) return rc;
+  }
+  return DIMQ_OK;
+}
+
+template <int XT, bool VEC>
+int quant_launch(const QuantArgs& a, hipStream_t s) {
+  return launch_rows(a.rows, a.blocks, "mx_quantize", [&](int64_t r, FastDiv div, uint32_t units, dim3 grid) {
+    QuantArgs b = a;
+    const int64_t e = dtype_size(XT);
+    b.x = static_cast<const char*>(a.x) + r * a.ldx * e;
+    if (b.codes4) b.codes4 += r * a.blocks * 16, b.scales4 += r * a.blocks;
+    if (b.codes8) b.codes8 += r * a.blocks8 * 32, b.scales8 += r * a.blocks8;
+    if (b.y) b.y = static_cast<char*>(a.y) + r * a.cols * e;
+    if (b.y) mx_quant_kernel<XT, VEC, false, true, true><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.codes4 && b.codes8) mx_quant_kernel<XT, VEC, true, true, false><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.codes4) mx_quant_kernel<XT, VEC, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
+    else mx_quant_kernel<XT, VEC, false, true, false><<<grid, 256, 0, s>>>(b, div, units);
+  });
+}
+
+template <int XT>
+int quant_typed(const QuantArgs& a, hipStream_t s) {
+  const bool vec = vec_rows(a.x, XT, a.cols, a.ldx) && (!a.y || vec_rows(a.y, XT, a.cols, a.cols));
+  return vec ? quant_launch<XT, true>(a, s) : quant_launch<XT, false>(a, s);
+}
+
+int quant_any(int x_dtype, const QuantArgs& a, hipStream_t s) {
+  if (a.rows == 0 || a.cols == 0) return DIMQ_OK;
+  switch (x_dtype) {
+    case DIMQ_F32: return quant_typed<DIMQ_F32>(a, s);
+    case DIMQ_F16: return quant_typed<DIMQ_F16>(a, s);
+    default: return quant_typed<DIMQ_BF16>(a, s);
+  }
+}
+
+template <int BITS, int YT, bool VEC, bool SLOPE>
+int back_launch(int64_t rows, int64_t blocks, const BackArgs& a, hipStream_t s) {
+  return launch_rows(rows, blocks, "mx_dequantize", [&](int64_t r, FastDiv div, uint32_t units, dim3 grid) {
+    BackArgs b = a;
+    const int64_t e = dtype_size(YT);
+    b.codes = static_cast<const char*>(a.codes) + r * blocks * (BITS * 4);
+    b.scales = a.scales + r * blocks;
+    if (b.g) b.g = static_cast<const char*>(a.g) + r * a.ldg * e;
+    b.y = static_cast<char*>(a.y) + r * a.cols * e;
+    mx_back_kernel<BITS, YT, VEC, SLOPE><<<grid, 256, 0, s>>>(b, div, units);
+  });
+}
+
+template <int BITS, bool SLOPE>
+int back_any(int y_dtype, int64_t rows, const BackArgs& a, hipStream_t s) {
+  if (rows == 0 || a.cols == 0) return DIMQ_OK;
+  const int64_t blocks = mx_blocks(a.cols);
+  const bool vec = vec_rows(a.y, y_dtype, a.cols, a.cols) && (!SLOPE || vec_rows(a.g, y_dtype, a.cols, a.ldg));
+#define DIMQ_MX_BACK(T) \
+  return vec ? back_launch<BITS, T, true, SLOPE>(rows, blocks, a, s) : back_launch<BITS, T, false, SLOPE>(rows, blocks, a, s)
+  switch (y_dtype) {
+    case DIMQ_F32: DIMQ_MX_BACK(DIMQ_F32);
+    case DIMQ_F16: DIMQ_MX_BACK(DIMQ_F16);
+    default: DIMQ_MX_BACK(DIMQ_BF16);
+  }
+#undef DIMQ_MX_BACK
+}
+
+int check_codes(const char* what, const void* codes, const void* scales) {
+  DIMQ_CHECK(codes && scales, "%s: null pointer", what);
+  DIMQ_CHECK(aligned(codes, 16), "%s: codes must be 16-byte aligned", what);
+  return DIMQ_OK;
+}
+
+}  // namespace
+}  // namespace dimq
+
+using namespace dimq;
+
+extern "C" int dimq_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes4,
+                                uint8_t* scales4, int64_t blocks4, int8_t* codes8, uint8_t* scales8, void* stream) {
+  int rc = mx_check_rows("mx_quantize", x, x_dtype, rows, cols, ldx);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0 || cols == 0) return DIMQ_OK;
+  DIMQ_CHECK(codes4 || codes8, "mx_quantize: no output");
+  if (codes4 && (rc = check_codes("mx_quantize", codes4, scales4)) != DIMQ_OK) return rc;
+  if (codes8 && (rc = check_codes("mx_quantize", codes8, scales8)) != DIMQ_OK) return rc;
+  const int64_t nb = mx_blocks(cols);
+  DIMQ_CHECK(!codes4 || blocks4 >= nb, "mx_quantize: %lld blocks do not hold a row of %lld", (long long)blocks4,
+             (long long)cols);
+  return quant_any(x_dtype, {x, ldx, rows, cols, codes4, scales4, codes8, scales8, codes4 ? blocks4 : nb, nb, nullptr},
+                   as_stream(stream));
+}
+
+extern "C" int dimq_mx_dequantize(const void* codes, const uint8_t* scales, int bits, int64_t rows, int64_t cols, void* y,
+                                  int y_dtype, void* stream) {
+  int rc = mx_check_rows("mx_dequantize", y, y_dtype, rows, cols, cols);
+  if (rc != DIMQ_OK) return rc;
+  DIMQ_CHECK(bits == 4 || bits == 8, "mx_dequantize: bits must be 4 or 8");
+  if (rows == 0 || cols == 0) return DIMQ_OK;
+  if ((rc = check_codes("mx_dequantize", codes, scales)) != DIMQ_OK) return rc;
+  const BackArgs a{codes, scales, cols, nullptr, 0, y};
+  return bits == 4 ? back_any<4, false>(y_dtype, rows, a, as_stream(stream))
+                   : back_any<8, false>(y_dtype, rows, a, as_stream(stream));
+}
+
+extern "C" int dimq_mx_gelu_forward(const void* h, int dtype, int64_t rows, int64_t cols, int64_t ldh, void* y,
+                                    int8_t* codes8, uint8_t* scales8, void* stream) {
+  int rc = mx_check_rows("mx_gelu_forward", h, dtype, rows, cols, ldh);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0 || cols == 0) return DIMQ_OK;
+  if ((rc = check_codes("mx_gelu_forward", codes8, scales8)) != DIMQ_OK) return rc;
+  DIMQ_CHECK(y, "mx_gelu_forward: null pointer");
+  const int64_t nb = mx_blocks(cols);
+  return quant_any(dtype, {h, ldh, rows, cols, nullptr, nullptr, codes8, scales8, nb, nb, y}, as_stream(stream));
+}
+
+extern "C" int dimq_mx_gelu_backward(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ldg,
+                                     const int8_t* codes8, const uint8_t* scales8, void* gh, void* stream) {
+  int rc = mx_check_rows("mx_gelu_backward", g, dtype, rows, cols, ldg);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0 || cols == 0) return DIMQ_OK;
+  if ((rc = check_codes("mx_gelu_backward", codes8, scales8)) != DIMQ_OK) return rc;
+  DIMQ_CHECK(gh, "mx_gelu_backward: null pointer");
+  return back_any<8, true>(dtype, rows, {codes8, scales8, cols, g, ldg, gh}, as_stream(stream));
+}

@@ -347,6 +347,192 @@ Tensor max_pool2d_nhwc(const Tensor& x, int64_t kernel_h, int64_t kernel_w, int6
   return y;
 }
 
+// ---- microscaled formats -----------------------------------------------------------
+
+bool mx_float(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+int64_t mx_blocks(int64_t n) { return (n + 31) / 32; }
+
+// A tensor [..., cols] as rows of a common stride (copied only where it has none).
+struct Rows {
+  Tensor t;
+  int64_t n = 0, cols = 0, ld = 0;
+  Rows(const Tensor& x, const char* op, const char* what) {
+    TORCH_CHECK(x.is_cuda(), op, " expects a CUDA ", what);
+    TORCH_CHECK(mx_float(x.scalar_type()), op, ": ", what, " must be fp32, fp16 or bf16, not ", dtype_name(x.scalar_type()));
+    TORCH_CHECK(x.dim() > 0, op, ": ", what, " must have at least one dimension");
+    cols = x.size(-1);
+    n = cols ? x.numel() / cols : 0;
+    t = x.detach();
+    if (x.dim() != 2) t = t.reshape({n, cols});
+    if (cols > 1 && t.stride(1) != 1) t = t.contiguous();
+    if (n > 1 && t.stride(0) < cols) t = t.contiguous();
+    ld = n > 1 ? t.stride(0) : cols;
+  }
+};
+
+// Codes and scales of rows of `cols`, contiguous and aligned.
+struct Codes {
+  Tensor c, s;
+  int64_t rows = 0;
+  Codes(const Tensor& codes, const Tensor& scales, int64_t cols, int bits, const Tensor& like, const char* op) {
+    TORCH_CHECK(codes.device() == like.device() && scales.device() == like.device(), op,
+                ": codes and scales must be on ", like.device().str());
+    TORCH_CHECK(codes.scalar_type() == (bits == 4 ? at::kByte : at::kChar), op, ": codes must be ",
+                bits == 4 ? "uint8" : "int8");
+    TORCH_CHECK(scales.scalar_type() == at::kByte, op, ": scales must be uint8");
+    const int64_t nb = mx_blocks(cols);
+    TORCH_CHECK(codes.dim() > 0 && scales.dim() == codes.dim() && codes.size(-1) == nb * bits * 4 && scales.size(-1) == nb &&
+                    codes.sizes().slice(0, codes.dim() - 1) == scales.sizes().slice(0, codes.dim() - 1),
+                op, ": rows of ", cols, " have codes [..., ", nb * bits * 4, "] and scales [..., ", nb, "], not ",
+                tuple_of(codes.sizes()), " and ", tuple_of(scales.sizes()));
+    c = codes.contiguous();
+    if (reinterpret_cast<uintptr_t>(c.data_ptr()) % 16) c = c.clone();
+    s = scales.contiguous();
+    rows = nb ? s.numel() / nb : 0;
+  }
+};
+
+std::pair<Tensor, Tensor> new_codes(at::IntArrayRef shape, int bits, const Tensor& like) {
+  std::vector<int64_t> sh = shape.vec();
+  const int64_t nb = mx_blocks(sh.back());
+  sh.back() = nb * bits * 4;
+  const Tensor c = at::empty(sh, like.options().dtype(bits == 4 ? at::kByte : at::kChar));
+  sh.back() = nb;
+  return {c, at::empty(sh, like.options().dtype(at::kByte))};
+}
+
+uint8_t* pu8(const Tensor& t) { return static_cast<uint8_t*>(ptr(t)); }
+int8_t* pi8(const Tensor& t) { return static_cast<int8_t*>(ptr(t)); }
+
+std::vector<Tensor> mx_quantize(const Tensor& x, bool q4, bool q8, const char* op) {
+  const Rows r(x, op, "input");
+  std::pair<Tensor, Tensor> a, b;
+  if (q4) a = new_codes(x.sizes(), 4, x);
+  if (q8) b = new_codes(x.sizes(), 8, x);
+  const On on(x);
+  check_rc(dimq_mx_quantize(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, pu8(a.first), pu8(a.second), mx_blocks(r.cols),
+                            pi8(b.first), pu8(b.second), on.stream));
+  std::vector<Tensor> out;
+  if (q4) out.insert(out.end(), {a.first, a.second});
+  if (q8) out.insert(out.end(), {b.first, b.second});
+  return out;
+}
+
+std::tuple<Tensor, Tensor> quantize_mxfp4(const Tensor& x) {
+  const auto v = mx_quantize(x, true, false, "quantize_mxfp4");
+  return {v[0], v[1]};
+}
+std::tuple<Tensor, Tensor> compress_activation(const Tensor& x) {
+  const auto v = mx_quantize(x, false, true, "compress_activation");
+  return {v[0], v[1]};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> quantize_and_compress(const Tensor& x) {
+  const auto v = mx_quantize(x, true, true, "quantize_and_compress");
+  return {v[0], v[1], v[2], v[3]};
+}
+
+Tensor mx_dequantize(const Tensor& codes, const Tensor& scales, int64_t size, at::ScalarType dtype, int bits, const char* op) {
+  TORCH_CHECK(codes.is_cuda(), op, " expects CUDA codes");
+  TORCH_CHECK(mx_float(dtype), op, ": output dtype must be fp32, fp16 or bf16");
+  TORCH_CHECK(size >= 0, op, ": size must not be negative");
+  const Codes c(codes, scales, size, bits, codes, op);
+  std::vector<int64_t> shape = codes.sizes().vec();
+  shape.back() = size;
+  const Tensor y = at::empty(shape, codes.options().dtype(dtype));
+  const On on(codes);
+  check_rc(dimq_mx_dequantize(ptr(c.c), pu8(c.s), bits, c.rows, size, ptr(y), dt(y), on.stream));
+  return y;
+}
+Tensor dequantize_mxfp4(const Tensor& codes, const Tensor& scales, int64_t size, at::ScalarType dtype) {
+  return mx_dequantize(codes, scales, size, dtype, 4, "dequantize_mxfp4");
+}
+Tensor decompress_activation(const Tensor& codes, const Tensor& scales, int64_t size, at::ScalarType dtype) {
+  return mx_dequantize(codes, scales, size, dtype, 8, "decompress_activation");
+}
+
+// c8, s8: where x's 8-bit form goes (undefined: nowhere).
+Tensor mxfp4_linear_into(const Tensor& x, const Codes& w, const OptTensor& bias, const OptTensor& residual, int64_t activation,
+                         at::ScalarType out_dtype, const Tensor& c8, const Tensor& s8) {
+  const Rows r(x, "mxfp4_linear", "input");
+  TORCH_CHECK(mx_float(out_dtype), "mxfp4_linear: output dtype must be fp32, fp16 or bf16");
+  const Bias b(bias, w.rows, "out_features");
+  const std::vector<int64_t> shape = out_shape(x, w.rows);
+  const Residual res(residual, shape, at::MemoryFormat::Contiguous);
+  TORCH_CHECK((!b.t.defined() || b.t.device() == x.device()) && (!res.t.defined() || res.t.device() == x.device()),
+              "mxfp4_linear: bias and residual must be on ", x.device().str());
+  const Tensor y = at::empty(shape, x.options().dtype(out_dtype));
+  const On on(x);
+  const Tensor ws = workspace(dimq_mxfp4_linear_workspace_bytes(r.n, r.cols, w.rows), x);
+  check_rc(dimq_mxfp4_linear(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, pu8(w.c), pu8(w.s), b.p, b.dtype, w.rows, ptr(y), dt(y),
+                             res.p, res.dtype, static_cast<int>(activation), pi8(c8), pu8(s8), ptr(ws),
+                             ws.defined() ? ws.numel() : 0, on.stream));
+  return y;
+}
+
+Tensor mxfp4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias,
+                    const OptTensor& residual, int64_t activation, std::optional<at::ScalarType> out_dtype) {
+  TORCH_CHECK(x.is_cuda(), "mxfp4_linear expects a CUDA input");
+  TORCH_CHECK(x.dim() > 0 && codes.dim() == 2, "mxfp4_linear expects an input of at least one dimension and 2-D codes");
+  const Codes w(codes, scales, x.size(-1), 4, x, "mxfp4_linear");
+  return mxfp4_linear_into(x, w, bias, residual, activation, out_dtype.value_or(x.scalar_type()), Tensor(), Tensor());
+}
+
+Tensor mxfp4_linear_grad_input(const Tensor& grad, const Tensor& codes, const Tensor& scales, int64_t in_features,
+                               std::optional<at::ScalarType> out_dtype) {
+  const char* op = "mxfp4_linear_grad_input";
+  const Rows g(grad, op, "gradient");
+  TORCH_CHECK(codes.dim() == 2, op, " expects 2-D codes");
+  const Codes w(codes, scales, in_features, 4, grad, op);
+  TORCH_CHECK(w.rows == g.cols, op, ": the gradient's last dimension ", g.cols, " must equal the weights' rows ", w.rows);
+  const at::ScalarType odt = out_dtype.value_or(grad.scalar_type());
+  TORCH_CHECK(mx_float(odt), op, ": output dtype must be fp32, fp16 or bf16");
+  const Tensor gx = at::empty(out_shape(grad, in_features), grad.options().dtype(odt));
+  const On on(grad);
+  const Tensor ws = workspace(dimq_mx_grad_input_workspace_bytes(dt(g.t), g.n, g.cols, g.ld, in_features), grad);
+  check_rc(dimq_mxfp4_linear_grad_input(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, pu8(w.c), pu8(w.s), in_features, ptr(gx),
+                                        dt(gx), ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
+  return gx;
+}
+
+std::tuple<Tensor, Tensor> linear_grad_weight(const Tensor& grad, const Tensor& codes, const Tensor& scales,
+                                              int64_t in_features, bool bias, std::optional<at::ScalarType> out_dtype,
+                                              std::optional<at::ScalarType> bias_dtype) {
+  const char* op = "linear_grad_weight";
+  const Rows g(grad, op, "gradient");
+  const Codes x(codes, scales, in_features, 8, grad, op);
+  TORCH_CHECK(x.rows == g.n, op, ": the gradient has ", g.n, " rows, the checkpoint ", x.rows);
+  const at::ScalarType odt = out_dtype.value_or(at::kFloat), bdt = bias_dtype.value_or(odt);
+  TORCH_CHECK(mx_float(odt), op, ": output dtype must be fp32, fp16 or bf16");
+  TORCH_CHECK(g.cols > 0 && in_features > 0, "linear dimensions must be positive");
+  const Tensor gw = at::empty({g.cols, in_features}, grad.options().dtype(odt));
+  const Tensor gb = bias ? at::empty({g.cols}, grad.options().dtype(bdt)) : Tensor();
+  const On on(grad);
+  const Tensor ws = workspace(dimq_mx_grad_weight_workspace_bytes(dt(g.t), g.n, g.cols, g.ld, in_features), grad);
+  check_rc(dimq_mx_linear_grad_weight(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, pi8(x.c), pu8(x.s), in_features, ptr(gw), dt(gw),
+                                      ptr(gb), bias ? dt(gb) : static_cast<int>(DIMQ_F32), ptr(ws),
+                                      ws.defined() ? ws.numel() : 0, on.stream));
+  return {gw, bias ? gb : at::empty({0}, grad.options().dtype(bdt))};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gelu_forward(const Tensor& h) {
+  const Rows r(h, "gelu", "input");
+  const Tensor y = at::empty(h.sizes(), h.options());
+  const auto [c, s] = new_codes(h.sizes(), 8, h);
+  const On on(h);
+  check_rc(dimq_mx_gelu_forward(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, ptr(y), pi8(c), pu8(s), on.stream));
+  return {y, c, s};
+}
+
+Tensor gelu_backward(const Tensor& grad, const Tensor& codes, const Tensor& scales) {
+  const Rows g(grad, "gelu_backward", "gradient");
+  const Codes c(codes, scales, g.cols, 8, grad, "gelu_backward");
+  TORCH_CHECK(c.rows == g.n, "gelu_backward: the gradient has ", g.n, " rows, the checkpoint ", c.rows);
+  const Tensor gh = at::empty(grad.sizes(), grad.options());
+  const On on(grad);
+  check_rc(dimq_mx_gelu_backward(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, pi8(c.c), pu8(c.s), ptr(gh), on.stream));
+  return gh;
+}
+
 // ---- QAT functions ---------------------------------------------------------------
 
 struct QatInputs {
@@ -454,6 +640,70 @@ struct SeparationLoss : torch::autograd::Function<SeparationLoss> {
   }
 };
 
+// Gradients here are kernels without a graph of their own.
+void once(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": gradients of its gradients are not supported");
+}
+
+// y = Q4(x) Q4(w)^T + b, straight through backward: gx = g Q4(w), gw = g^T Q8(x), gb = sum g.  Kept for it: w's 4-bit
+// and x's 8-bit codes, each only where its gradient is asked for.
+struct MxLinear : torch::autograd::Function<MxLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias) {
+    TORCH_CHECK(x.is_cuda(), "mx.linear expects a CUDA input");
+    TORCH_CHECK(w.dim() == 2 && x.dim() > 0 && x.size(-1) == w.size(1),
+                "mx.linear: input's last dimension must equal the weight's, [out_features, in_features]");
+    TORCH_CHECK(w.device() == x.device(), "mx.linear: the weight must be on ", x.device().str());
+    TORCH_CHECK(mx_float(x.scalar_type()), "mx.linear: input must be fp32, fp16 or bf16, not ", dtype_name(x.scalar_type()));
+    TORCH_CHECK(!bias || mx_float(bias->scalar_type()), "mx.linear: bias must be fp32, fp16 or bf16");
+    const auto wq = mx_quantize(w, true, false, "mx.linear");
+    const Codes wc(wq[0], wq[1], w.size(1), 4, x, "mx.linear");
+    std::pair<Tensor, Tensor> x8;
+    if (w.requires_grad()) x8 = new_codes(x.sizes(), 8, x);
+    const Tensor y = mxfp4_linear_into(x.detach(), wc, bias ? OptTensor(bias->detach()) : bias, std::nullopt, 0,
+                                       x.scalar_type(), x8.first, x8.second);
+    const bool need_w = x.requires_grad();
+    ctx->save_for_backward({need_w ? wq[0] : Tensor(), need_w ? wq[1] : Tensor(), x8.first, x8.second});
+    ctx->saved_data["k"] = w.size(1);
+    ctx->saved_data["wdt"] = static_cast<int64_t>(w.scalar_type());
+    ctx->saved_data["b"] = static_cast<bool>(bias && bias->requires_grad());
+    ctx->saved_data["bdt"] = static_cast<int64_t>(bias ? bias->scalar_type() : at::kFloat);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("mx.linear");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& g = grads[0];
+    const int64_t K = ctx->saved_data["k"].toInt();
+    const bool b = ctx->saved_data["b"].toBool();
+    const auto bdt = static_cast<at::ScalarType>(ctx->saved_data["bdt"].toInt());
+    Tensor gx, gw, gb;
+    if (saved[0].defined()) gx = mxfp4_linear_grad_input(g, saved[0], saved[1], K, std::nullopt);
+    if (saved[2].defined()) {
+      const auto r = linear_grad_weight(g, saved[2], saved[3], K, b,
+                                        static_cast<at::ScalarType>(ctx->saved_data["wdt"].toInt()), bdt);
+      gw = std::get<0>(r);
+      if (b) gb = std::get<1>(r);
+    } else if (b) {
+      gb = g.reshape({-1, g.size(-1)}).sum(0, false, at::kFloat).to(bdt);
+    }
+    return {gx, gw, gb};
+  }
+};
+
+// gelu(h), h kept in 8 bits for the backward pass.
+struct MxGelu : torch::autograd::Function<MxGelu> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& h) {
+    const auto [y, c, s] = gelu_forward(h.detach());
+    ctx->save_for_backward({c, s});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("mx.gelu");
+    const auto saved = ctx->get_saved_variables();
+    return {gelu_backward(grads[0], saved[0], saved[1])};
+  }
+};
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(dimq, m) {
@@ -477,6 +727,19 @@ TORCH_LIBRARY_FRAGMENT(dimq, m) {
         "ScalarType? out_dtype=None) -> Tensor");
   m.def("max_pool2d_nhwc(Tensor x, int kernel_h, int kernel_w, int stride_h, int stride_w, int pad_h, int pad_w) "
         "-> Tensor");
+  m.def("quantize_mxfp4(Tensor x) -> (Tensor, Tensor)");
+  m.def("compress_activation(Tensor x) -> (Tensor, Tensor)");
+  m.def("quantize_and_compress(Tensor x) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("dequantize_mxfp4(Tensor codes, Tensor scales, int size, ScalarType dtype) -> Tensor");
+  m.def("decompress_activation(Tensor codes, Tensor scales, int size, ScalarType dtype) -> Tensor");
+  m.def("mxfp4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor? residual=None, int activation=0, "
+        "ScalarType? out_dtype=None) -> Tensor");
+  m.def("mxfp4_linear_grad_input(Tensor grad, Tensor codes, Tensor scales, int in_features, "
+        "ScalarType? out_dtype=None) -> Tensor");
+  m.def("linear_grad_weight(Tensor grad, Tensor codes, Tensor scales, int in_features, bool bias=True, "
+        "ScalarType? out_dtype=None, ScalarType? bias_dtype=None) -> (Tensor, Tensor)");
+  m.def("gelu_forward(Tensor h) -> (Tensor, Tensor, Tensor)");
+  m.def("gelu_backward(Tensor grad, Tensor codes, Tensor scales) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(dimq, CUDA, m) {
@@ -489,6 +752,16 @@ TORCH_LIBRARY_IMPL(dimq, CUDA, m) {
   m.impl("conv2d_codebook", conv2d_codebook);
   m.impl("layer_norm", layer_norm);
   m.impl("max_pool2d_nhwc", max_pool2d_nhwc);
+  m.impl("quantize_mxfp4", quantize_mxfp4);
+  m.impl("compress_activation", compress_activation);
+  m.impl("quantize_and_compress", quantize_and_compress);
+  m.impl("dequantize_mxfp4", dequantize_mxfp4);
+  m.impl("decompress_activation", decompress_activation);
+  m.impl("mxfp4_linear", mxfp4_linear);
+  m.impl("mxfp4_linear_grad_input", mxfp4_linear_grad_input);
+  m.impl("linear_grad_weight", linear_grad_weight);
+  m.impl("gelu_forward", gelu_forward);
+  m.impl("gelu_backward", gelu_backward);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -505,4 +778,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("separation_loss",
         [](const Tensor& w, const Tensor& c, double eta, double eps) { return SeparationLoss::apply(w, c, eta, eps); },
         Unlocked());
+  m.def("mx_linear", [](const Tensor& x, const Tensor& w, const OptTensor& b) { return MxLinear::apply(x, w, b); },
+        Unlocked());
+  m.def("mx_gelu", [](const Tensor& h) { return MxGelu::apply(h); }, Unlocked());
 }

@@ -529,6 +529,70 @@ int dimq_max_pool2d_nhwc(const void* x, int x_dtype, int64_t B, int64_t C, int64
                          int64_t kernel_w, int64_t stride_h, int64_t stride_w, int64_t pad_h, int64_t pad_w,
                          void* y, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * 4. Microscaled formats: 4-bit linear layers and 8-bit activation
+ *    checkpoints (no counterpart in the reference).  Along a row, blocks of 32
+ *    elements (the last one may be short) share a power of two 2^e, stored as
+ *    the byte e + 127:
+ *      4 bits  codes sign | 2 exponent bits | 1 mantissa bit ({0, .5, 1, 1.5,
+ *              2, 3, 4, 6}), two a byte, the earlier element in the low half,
+ *              16 bytes a block; e = max(floor(log2 max|v|) - 2, -127)
+ *      8 bits  integers -127..127 in units of 2^e / 64, 32 bytes a block;
+ *              e = max(floor(log2 max|v|), -127)
+ *    Codes are v / 2^e rounded to nearest (ties to the even code) and
+ *    saturated; a block that holds a NaN or an infinity has the scale byte 255
+ *    and stands for NaN throughout.  Rows are padded to whole blocks with zero
+ *    codes; codes are 16-byte aligned.  Q4 / Q8 below: the values that a
+ *    tensor's codes stand for.  Tensors are [rows, cols] with the given row
+ *    stride in elements; dtypes F32, F16, BF16.
+ * ------------------------------------------------------------------------- */
+
+/* x -> 4-bit codes [rows, blocks4, 16] and scales [rows, blocks4] (nullable
+ * pair; blocks4 >= ceil(cols / 32), blocks past the row zero) and 8-bit codes
+ * [rows, ceil(cols / 32), 32] and scales (nullable pair), from one read of x. */
+int dimq_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes4,
+                     uint8_t* scales4, int64_t blocks4, int8_t* codes8, uint8_t* scales8, void* stream);
+
+/* The values of codes of `bits` 4 or 8, [rows, ceil(cols / 32), ...], into y
+ * [rows, cols] contiguous, one rounding to y_dtype. */
+int dimq_mx_dequantize(const void* codes, const uint8_t* scales, int bits, int64_t rows, int64_t cols, void* y,
+                       int y_dtype, void* stream);
+
+/* y = act(Q4(x) W^T + bias + residual) for the 4-bit weights codes
+ * [N, ceil(K / 32), 16], scales [N, ceil(K / 32)]; fp32 accumulation of exact
+ * products, one rounding to y_dtype; bias [N] and residual [M, N] (contiguous)
+ * nullable, any float dtype.  codes8 / scales8 (nullable): x's 8-bit form,
+ * [M, ceil(K / 32), 32] and [M, ceil(K / 32)], written from the same read of x.
+ * The workspace (256-byte aligned, the size the query gives) is written on
+ * `stream`. */
+int64_t dimq_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int dimq_mxfp4_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* codes,
+                      const uint8_t* scales, const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype,
+                      const void* residual, int residual_dtype, int activation, int8_t* codes8, uint8_t* scales8,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Straight-through gradients of that layer for the upstream g [M, N]:
+ *   gx = g W             (W from its 4-bit codes)
+ *   gw = g^T Q8(x)       (x from its 8-bit checkpoint), gb = sum of g over m
+ * Every product is exact (g as a sum of bf16 parts, codes times scales in
+ * bf16), the sums are fp32 in a fixed order, outputs [M, K], [N, K], [N]
+ * (nullable) contiguous in their dtypes.  M = 0 gives zeros. */
+int64_t dimq_mx_grad_input_workspace_bytes(int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
+int dimq_mxfp4_linear_grad_input(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, const uint8_t* codes,
+                                 const uint8_t* scales, int64_t K, void* gx, int gx_dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+int64_t dimq_mx_grad_weight_workspace_bytes(int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
+int dimq_mx_linear_grad_weight(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, const int8_t* codes8,
+                               const uint8_t* scales8, int64_t K, void* gw, int gw_dtype, void* gb, int gb_dtype,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y = gelu(h) = h Phi(h) and h's 8-bit form from one read of h (y [rows, cols]
+ * contiguous in h's dtype), and the gradient gh = g gelu'(Q8(h)) in g's dtype. */
+int dimq_mx_gelu_forward(const void* h, int dtype, int64_t rows, int64_t cols, int64_t ldh, void* y, int8_t* codes8,
+                         uint8_t* scales8, void* stream);
+int dimq_mx_gelu_backward(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ldg, const int8_t* codes8,
+                          const uint8_t* scales8, void* gh, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
