@@ -1,5 +1,5 @@
 // Microscaled formats (mx.h): quantization to 4 and 8 bits, the way back, and GELU with its input kept in 8 bits.
-#include "mx.h"
+#include "mx_quant.h"
 
 namespace dimq {
 namespace {
@@ -16,60 +16,6 @@ struct FastDiv {
   }
   __device__ __forceinline__ uint32_t quot(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> shift); }
 };
-
-template <int DT>
-__device__ __forceinline__ float scalar_load(const void* p, int64_t i) {
-  return load_as_float(p, DT, i);
-}
-
-// Elements c .. c + 7 of a row of `cols` as fp32, zeros past its end.  VEC: the row is 16-byte aligned and cols % 8 == 0.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* x, int64_t at, int64_t c, int64_t cols, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c >= cols) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    } else if constexpr (DT == DIMQ_F32) {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at + c);
-      const float4 a = p[0], b = p[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at + c);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = DT == DIMQ_F16 ? f16_bits_to_float(w[j] & 0xffffu) : bf16_bits_to_float(w[j] & 0xffffu);
-        v[2 * j + 1] = DT == DIMQ_F16 ? f16_bits_to_float(w[j] >> 16) : bf16_bits_to_float(w[j] >> 16);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? scalar_load<DT>(x, at + c + j) : 0.0f;
-  }
-}
-
-template <int DT, bool VEC>
-__device__ __forceinline__ void store8(void* y, int64_t at, int64_t c, int64_t cols, const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c >= cols) return;
-    if constexpr (DT == DIMQ_F32) {
-      float4* p = reinterpret_cast<float4*>(static_cast<float*>(y) + at + c);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = DT == DIMQ_F16 ? f16x2_rne(v[2 * j], v[2 * j + 1]) : bf16x2_rne(v[2 * j], v[2 * j + 1]);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + at + c) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < cols) store_from_float(y, DT, at + c + j, v[j]);
-  }
-}
 
 // Largest magnitude of a block's four lanes, as fp32 bits: integer order is the magnitudes' order, NaN above all.
 __device__ __forceinline__ uint32_t quad_max(uint32_t m) {
@@ -103,19 +49,48 @@ struct QuantArgs {
   uint8_t* scales8;
   int64_t blocks, blocks8;  // blocks a row takes in the 4-bit output (the padded ones are zeros) and in the 8-bit one
   void* y;           // GELU's output rows of cols
+  int64_t scale_rows;  // not 0: scales4 is [stages of 8 blocks, scale_rows, 8] (mx_mm.h), this launch's rows from row0
+  int64_t row0;
+  MxScaleTurn turn;    // with it: another tensor's scales that the launch's first work-groups bring into that order
 };
+
+// Eight scales of a row a thread, zeros past the row's end.
+__device__ __forceinline__ void turn_scales(const MxScaleTurn& t, uint32_t group) {
+  const int64_t i = (int64_t)group * 256 + threadIdx.x;
+  if (i >= t.stages * t.n) return;
+  const int64_t stage = i / t.n, row = i - stage * t.n;
+  const uint8_t* src = t.in + row * t.blocks + stage * 8;
+  uint2 w = make_uint2(0, 0);
+  if (t.blocks % 8 == 0 && aligned(t.in, 8)) {
+    w = *reinterpret_cast<const uint2*>(src);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (stage * 8 + j < t.blocks) (j < 4 ? w.x : w.y) |= (uint32_t)src[j] << (8 * (j & 3));
+  }
+  *reinterpret_cast<uint2*>(t.out + (stage * t.rows + row) * 8) = w;
+}
 
 // A lane takes eight elements, four lanes a block: loads of 16 bytes and stores of 4, 8 and 16 next to one another
 // across the wave, the block's maximum by two lane exchanges.  Bound by the bytes: 4096 x 4096 fp32 to both formats
 // moves 67 MB in and 26 MB out.
-template <int XT, bool VEC, bool Q4, bool Q8, bool GELU>
+// TILED: the 4-bit output is a tiled product's operand, with its scales in that order.
+template <int XT, bool VEC, bool Q4, bool Q8, bool GELU, bool TILED>
 __global__ __launch_bounds__(256) void mx_quant_kernel(QuantArgs a, FastDiv div, uint32_t units) {
-  const uint32_t u = (blockIdx.x * 256u + threadIdx.x) >> 2;
+  uint32_t group = blockIdx.x;
+  if constexpr (TILED) {
+    if (group < a.turn.groups) {
+      turn_scales(a.turn, group);
+      return;
+    }
+    group -= a.turn.groups;
+  }
+  const uint32_t u = (group * 256u + threadIdx.x) >> 2;
   if (u >= units) return;  // whole blocks: the four lanes leave together
   const uint32_t q = threadIdx.x & 3u, row = div.quot(u), blk = u - row * div.d;
   const int64_t c = (int64_t)blk * kMxBlock + q * 8;
   float v[8];
-  load8<XT, VEC>(a.x, row * a.ldx, c, a.cols, v);
+  mx_load_row8<XT, VEC>(a.x, row * a.ldx, c, a.cols, v);
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -127,7 +102,10 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(QuantArgs a, FastDiv div,
     const uint32_t byte = mx_scale_byte<2>(top);
     const int64_t b = (int64_t)row * a.blocks + blk;
     reinterpret_cast<uint32_t*>(a.codes4)[b * 4 + q] = byte == kMxNan ? 0u : mx_codes4(v, mx_scale_operand(byte));
-    if (q == 0) a.scales4[b] = (uint8_t)byte;
+    if (q == 0) {
+      if constexpr (TILED) a.scales4[((int64_t)(blk >> 3) * a.scale_rows + a.row0 + row) * 8 + (blk & 7)] = (uint8_t)byte;
+      else a.scales4[b] = (uint8_t)byte;
+    }
   }
   if constexpr (Q8) {
     if (blk < a.blocks8) {
@@ -141,7 +119,7 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(QuantArgs a, FastDiv div,
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = mx_gelu<XT == DIMQ_F32>(v[j]);
-    store8<XT, VEC>(a.y, row * a.cols, c, a.cols, y);
+    mx_store_row8<XT, VEC>(a.y, row * a.cols, c, a.cols, y);
   }
 }
 
@@ -183,15 +161,11 @@ __global__ __launch_bounds__(256) void mx_back_kernel(BackArgs a, FastDiv div, u
   decode8<BITS>(a.codes, a.scales[b], b * 4 + q, v);
   if constexpr (SLOPE) {
     float g[8];
-    load8<YT, VEC>(a.g, row * a.ldg, c, a.cols, g);
+    mx_load_row8<YT, VEC>(a.g, row * a.ldg, c, a.cols, g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = g[j] * mx_gelu_slope<YT == DIMQ_F32>(v[j]);
   }
-  store8<YT, VEC>(a.y, row * a.cols, c, a.cols, v);
-}
-
-bool vec_rows(const void* p, int dt, int64_t cols, int64_t ld) {
-  return aligned(p, 16) && cols % 8 == 0 && (ld * dtype_size(dt)) % 16 == 0;
+  mx_store_row8<YT, VEC>(a.y, row * a.cols, c, a.cols, v);
 }
 
 // Units of a launch stay below 2^29 (FastDiv, grid of 2^31 threads): more rows go in several.
@@ -215,19 +189,25 @@ int quant_launch(const QuantArgs& a, hipStream_t s) {
     QuantArgs b = a;
     const int64_t e = dtype_size(XT);
     b.x = static_cast<const char*>(a.x) + r * a.ldx * e;
-    if (b.codes4) b.codes4 += r * a.blocks * 16, b.scales4 += r * a.blocks;
+    if (b.codes4) b.codes4 += r * a.blocks * 16;
+    if (b.codes4 && !a.scale_rows) b.scales4 += r * a.blocks;
+    b.row0 = r;
+    if (r > 0) b.turn.groups = 0;
+    grid.x += b.turn.groups;
     if (b.codes8) b.codes8 += r * a.blocks8 * 32, b.scales8 += r * a.blocks8;
     if (b.y) b.y = static_cast<char*>(a.y) + r * a.cols * e;
-    if (b.y) mx_quant_kernel<XT, VEC, false, true, true><<<grid, 256, 0, s>>>(b, div, units);
-    else if (b.codes4 && b.codes8) mx_quant_kernel<XT, VEC, true, true, false><<<grid, 256, 0, s>>>(b, div, units);
-    else if (b.codes4) mx_quant_kernel<XT, VEC, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
-    else mx_quant_kernel<XT, VEC, false, true, false><<<grid, 256, 0, s>>>(b, div, units);
+    if (b.y) mx_quant_kernel<XT, VEC, false, true, true, false><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.scale_rows && b.codes8) mx_quant_kernel<XT, VEC, true, true, false, true><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.scale_rows) mx_quant_kernel<XT, VEC, true, false, false, true><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.codes4 && b.codes8) mx_quant_kernel<XT, VEC, true, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.codes4) mx_quant_kernel<XT, VEC, true, false, false, false><<<grid, 256, 0, s>>>(b, div, units);
+    else mx_quant_kernel<XT, VEC, false, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
   });
 }
 
 template <int XT>
 int quant_typed(const QuantArgs& a, hipStream_t s) {
-  const bool vec = vec_rows(a.x, XT, a.cols, a.ldx) && (!a.y || vec_rows(a.y, XT, a.cols, a.cols));
+  const bool vec = mx_vec_rows(a.x, XT, a.cols, a.ldx) && (!a.y || mx_vec_rows(a.y, XT, a.cols, a.cols));
   return vec ? quant_launch<XT, true>(a, s) : quant_launch<XT, false>(a, s);
 }
 
@@ -257,7 +237,7 @@ template <int BITS, bool SLOPE>
 int back_any(int y_dtype, int64_t rows, const BackArgs& a, hipStream_t s) {
   if (rows == 0 || a.cols == 0) return DIMQ_OK;
   const int64_t blocks = mx_blocks(a.cols);
-  const bool vec = vec_rows(a.y, y_dtype, a.cols, a.cols) && (!SLOPE || vec_rows(a.g, y_dtype, a.cols, a.ldg));
+  const bool vec = mx_vec_rows(a.y, y_dtype, a.cols, a.cols) && (!SLOPE || mx_vec_rows(a.g, y_dtype, a.cols, a.ldg));
 #define DIMQ_MX_BACK(T) \
   return vec ? back_launch<BITS, T, true, SLOPE>(rows, blocks, a, s) : back_launch<BITS, T, false, SLOPE>(rows, blocks, a, s)
   switch (y_dtype) {
@@ -277,6 +257,21 @@ int check_codes(const char* what, const void* codes, const void* scales) {
 }  // namespace
 }  // namespace dimq
 
+namespace dimq {
+
+int mx_quantize_tiled(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                      int64_t blocks, int64_t scale_rows, int8_t* codes8, uint8_t* scales8, MxScaleTurn turn,
+                      hipStream_t s) {
+  turn.stages = (turn.blocks + 7) / 8;
+  const int64_t groups = (turn.stages * turn.n + 255) / 256;
+  DIMQ_CHECK(groups < (1 << 28), "mxfp4_linear: too many outputs");
+  turn.groups = (uint32_t)groups;
+  return quant_any(x_dtype, {x, ldx, rows, cols, codes, scales, codes8, scales8, blocks, mx_blocks(cols), nullptr, scale_rows,
+                             0, turn}, s);
+}
+
+}  // namespace dimq
+
 using namespace dimq;
 
 extern "C" int dimq_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes4,
@@ -290,7 +285,7 @@ extern "C" int dimq_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_
   const int64_t nb = mx_blocks(cols);
   DIMQ_CHECK(!codes4 || blocks4 >= nb, "mx_quantize: %lld blocks do not hold a row of %lld", (long long)blocks4,
              (long long)cols);
-  return quant_any(x_dtype, {x, ldx, rows, cols, codes4, scales4, codes8, scales8, codes4 ? blocks4 : nb, nb, nullptr},
+  return quant_any(x_dtype, {x, ldx, rows, cols, codes4, scales4, codes8, scales8, codes4 ? blocks4 : nb, nb, nullptr, 0, 0, {}},
                    as_stream(stream));
 }
 
@@ -314,7 +309,7 @@ extern "C" int dimq_mx_gelu_forward(const void* h, int dtype, int64_t rows, int6
   if ((rc = check_codes("mx_gelu_forward", codes8, scales8)) != DIMQ_OK) return rc;
   DIMQ_CHECK(y, "mx_gelu_forward: null pointer");
   const int64_t nb = mx_blocks(cols);
-  return quant_any(dtype, {h, ldh, rows, cols, nullptr, nullptr, codes8, scales8, nb, nb, y}, as_stream(stream));
+  return quant_any(dtype, {h, ldh, rows, cols, nullptr, nullptr, codes8, scales8, nb, nb, y, 0, 0, {}}, as_stream(stream));
 }
 
 extern "C" int dimq_mx_gelu_backward(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ldg,

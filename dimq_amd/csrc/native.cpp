@@ -488,7 +488,7 @@ Tensor mxfp4_linear_grad_input(const Tensor& grad, const Tensor& codes, const Te
   TORCH_CHECK(mx_float(odt), op, ": output dtype must be fp32, fp16 or bf16");
   const Tensor gx = at::empty(out_shape(grad, in_features), grad.options().dtype(odt));
   const On on(grad);
-  const Tensor ws = workspace(dimq_mx_grad_input_workspace_bytes(dt(g.t), g.n, g.cols, g.ld, in_features), grad);
+  const Tensor ws = workspace(dimq_mx_grad_input_workspace_bytes(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, in_features), grad);
   check_rc(dimq_mxfp4_linear_grad_input(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, pu8(w.c), pu8(w.s), in_features, ptr(gx),
                                         dt(gx), ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
   return gx;
@@ -507,7 +507,7 @@ std::tuple<Tensor, Tensor> linear_grad_weight(const Tensor& grad, const Tensor& 
   const Tensor gw = at::empty({g.cols, in_features}, grad.options().dtype(odt));
   const Tensor gb = bias ? at::empty({g.cols}, grad.options().dtype(bdt)) : Tensor();
   const On on(grad);
-  const Tensor ws = workspace(dimq_mx_grad_weight_workspace_bytes(dt(g.t), g.n, g.cols, g.ld, in_features), grad);
+  const Tensor ws = workspace(dimq_mx_grad_weight_workspace_bytes(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, in_features), grad);
   check_rc(dimq_mx_linear_grad_weight(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, pi8(x.c), pu8(x.s), in_features, ptr(gw), dt(gw),
                                       ptr(gb), bias ? dt(gb) : static_cast<int>(DIMQ_F32), ptr(ws),
                                       ws.defined() ? ws.numel() : 0, on.stream));

@@ -577,11 +577,11 @@ int dimq_mxfp4_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t 
  * Every product is exact (g as a sum of bf16 parts, codes times scales in
  * bf16), the sums are fp32 in a fixed order, outputs [M, K], [N, K], [N]
  * (nullable) contiguous in their dtypes.  M = 0 gives zeros. */
-int64_t dimq_mx_grad_input_workspace_bytes(int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
+int64_t dimq_mx_grad_input_workspace_bytes(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
 int dimq_mxfp4_linear_grad_input(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, const uint8_t* codes,
                                  const uint8_t* scales, int64_t K, void* gx, int gx_dtype, void* workspace,
                                  int64_t workspace_bytes, void* stream);
-int64_t dimq_mx_grad_weight_workspace_bytes(int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
+int64_t dimq_mx_grad_weight_workspace_bytes(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
 int dimq_mx_linear_grad_weight(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, const int8_t* codes8,
                                const uint8_t* scales8, int64_t K, void* gw, int gw_dtype, void* gb, int gb_dtype,
                                void* workspace, int64_t workspace_bytes, void* stream);
