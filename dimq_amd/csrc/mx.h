@@ -58,51 +58,62 @@ __device__ __forceinline__ uint32_t mx_codes4(const float (&v)[8], float scale) 
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], scale, 3);
 }
 
-// erfc(a) exp(a^2), a >= 0, as t P(t) with t = 1 / (1 + 0.33 a): P by weighted least squares on Chebyshev nodes of t
-// over a <= 10 with P(1) = 1, the weights moved towards equal relative errors: 1e-7, 5e-7 as evaluated in fp32 and none
-// at a = 0, the value of most zeros of a quantized block.
-__device__ __forceinline__ float mx_erfcx(float a) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.33f, a, 1.0f));
-  float r = -0.13529980182647705f;
-  r = fmaf(r, t, 0.4600503742694855f);
-  r = fmaf(r, t, -0.3508346676826477f);
-  r = fmaf(r, t, 0.408215194940567f);
-  r = fmaf(r, t, 0.04736927151679993f);
-  r = fmaf(r, t, 0.20117920637130737f);
-  r = fmaf(r, t, 0.18296308815479279f);
-  r = fmaf(r, t, 0.18635733425617218f);
+// Phi(-a) exp(a^2 / 2), 0 <= a, as t P(t) with t = 1 / (1 + k a): P by weighted least squares on Chebyshev nodes of t
+// over a <= 14 with P(1) = 1/2, the weights moved towards equal relative errors, and so exact at a = 0, the value of most
+// zeros of a quantized block.  FINE (fp32 outputs): 8 coefficients, 5e-7 as evaluated in fp32; otherwise 7, 1.2e-6.
+template <bool FINE>
+__device__ __forceinline__ float mx_tail_factor(float a) {
+  if constexpr (FINE) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.2333452377915607f, a, 1.0f));
+    float r = -0.067649900913238525f;
+    r = fmaf(r, t, 0.23002518713474274f);
+    r = fmaf(r, t, -0.17541733384132385f);
+    r = fmaf(r, t, 0.2041075974702835f);
+    r = fmaf(r, t, 0.023684635758399963f);
+    r = fmaf(r, t, 0.10058960318565369f);
+    r = fmaf(r, t, 0.091481544077396393f);
+    r = fmaf(r, t, 0.09317866712808609f);
+    return r * t;
+  }
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.36f, a, 1.0f));
+  float r = 0.04709881659085434f;
+  r = fmaf(r, t, -0.17988737532749394f);
+  r = fmaf(r, t, 0.18109358442700213f);
+  r = fmaf(r, t, 0.02646958676291894f);
+  r = fmaf(r, t, 0.13974328500731586f);
+  r = fmaf(r, t, 0.14176884610587542f);
+  r = fmaf(r, t, 0.14371325643352723f);
   return r * t;
 }
 
-// exp(-h^2 / 4).  Products take it twice, so that they reach the subnormal numbers, which the exponential itself
-// flushes.  FINE (fp32 outputs): the argument's roundings, 2^-24 of up to 150, are carried along and applied to first
-// order; without it the tail is 6e-6 off where it is not yet 0, far below a rounding to 16 bits.
+// exp(-a^2 / 4).  Products take it twice, so that they reach the subnormal numbers, which the exponential itself flushes.
+// FINE: the argument's roundings, 2^-24 of up to 150, are carried along and applied to first order.
 template <bool FINE>
-__device__ __forceinline__ float mx_exp_quarter(float h) {
+__device__ __forceinline__ float mx_exp_quarter(float a) {
   constexpr float kC = -0.36067376022224085f;  // -log2(e) / 4
-  if constexpr (!FINE) return __builtin_amdgcn_exp2f(h * h * kC);
+  if constexpr (!FINE) return __builtin_amdgcn_exp2f(a * a * kC);
   constexpr float kLow = (float)(-0.36067376022224085187998 - (double)kC);
-  h = fminf(fabsf(h), 40.0f);  // exp(-400) is 0: keeps infinities out of the differences
-  const float q = h * h, t = q * kC;
-  const float low = fmaf(q, kLow, fmaf(fmaf(h, h, -q), kC, fmaf(q, kC, -t)));
+  const float q = a * a, t = q * kC;
+  const float low = fmaf(q, kLow, fmaf(fmaf(a, a, -q), kC, fmaf(q, kC, -t)));
   const float e = __builtin_amdgcn_exp2f(t);
   return fmaf(e, low * 0.69314718055994531f, e);
 }
 
-// h Phi(h): relative error about 1e-6 down the negative tail too, where 1 + erf would cancel.
+// h Phi(h) = max(h, 0) - a Phi(-a), a = |h|, which keeps the negative tail's relative error (1e-6; not FINE, for outputs of
+// 16 bits: 1.5e-5 where the tail is 1e-37) where 1 + erf would cancel.  a stops at 40, where the tail is 0: infinity times 0.
 template <bool FINE>
 __device__ __forceinline__ float mx_gelu(float h) {
-  const float root = mx_exp_quarter<FINE>(h);
-  const float tail = 0.5f * h * mx_erfcx(fabsf(h) * 0.70710678118654752f) * root * root;  // h Phi(-|h|)
-  return h < 0.0f ? tail : h > 40.0f ? h : h - tail;  // the select: infinity times a tail of 0
+  const float a = fminf(fabsf(h), 40.0f), m = mx_tail_factor<FINE>(a);
+  const float root = mx_exp_quarter<FINE>(a);
+  return fmaf(-(a * m * root), root, 0.5f * (h + fabsf(h)));  // the last sum keeps NaN
 }
 
 // d gelu / dh = Phi(h) + h phi(h)
 template <bool FINE>
 __device__ __forceinline__ float mx_gelu_slope(float h) {
-  const float root = mx_exp_quarter<FINE>(h);
-  const float tail = 0.5f * mx_erfcx(fabsf(h) * 0.70710678118654752f) * root * root;
-  return fmaf(h * 0.39894228040143268f * root, root, h < 0.0f ? tail : 1.0f - tail);
+  const float a = fminf(fabsf(h), 40.0f), m = mx_tail_factor<FINE>(a), c = h * 0.39894228040143268f;
+  const float root = mx_exp_quarter<FINE>(a), tail = m * root * root;
+  return fmaf(c * root, root, h < 0.0f ? tail : 1.0f - tail);
 }
 
 }  // namespace dimq

@@ -23,16 +23,23 @@ struct FewArgs {
 // The lane's block of x in 4 bits: 32 elements from column c of a row.  16-bit elements stay in pairs: integer maxima of
 // their magnitudes and the conversions that take pairs, 50 instructions a block where fp32 copies take 150, which is what
 // the kernel spends its time on from 8 rows on (16 x 4096 -> 4096: 13.3 us with copies).
-template <int XT, bool VEC>
+template <int XT>
 __device__ __forceinline__ void quantize_block(const void* x, int64_t at, int64_t c, int64_t cols, uint4& codes, uint32_t& byte) {
-  if constexpr (VEC && XT != DIMQ_F32) {
+  if constexpr (XT != DIMQ_F32) {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 t = c + 8 * i < cols ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at + c + 8 * i)
-                                       : make_uint4(0, 0, 0, 0);
+      const uint16_t* p = static_cast<const uint16_t*>(x) + at + c + 8 * i;
+      uint4 t = make_uint4(0, 0, 0, 0);
+      if (c + 8 * i + 8 <= cols) {
+        t = mx_read16(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + 8 * i + j < cols) (&t.x)[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+      }
       w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
     }
     u16x2 top = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
@@ -59,7 +66,7 @@ __device__ __forceinline__ void quantize_block(const void* x, int64_t at, int64_
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    mx_load_row8<XT, VEC>(x, at, c + 8 * i, cols, v[i]);
+    mx_load_row8<XT>(x, at, c + 8 * i, cols, v[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t m = __float_as_uint(v[i][j]) & 0x7fffffffu;
@@ -76,7 +83,7 @@ __device__ __forceinline__ void quantize_block(const void* x, int64_t at, int64_
 // 4 (l / 16) .. + 3 of a turn for row l % 16 of either operand: 64 contiguous bytes of codes and one dword of scales,
 // whose bytes the four instructions select.  Bound by latency: all of a turn's loads are in flight at once, and with 16
 // outputs and 8 waves a work-group the 8.4 MB of a 4096 x 4096 layer are requested by the first turn of 256 work-groups.
-template <int XT, bool VEC, int MT>
+template <int XT, int MT>
 __global__ __launch_bounds__(512) void mx4_few_rows(const FewArgs p) {
   __shared__ f32x4 red[8 * MT * 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r = lane & 15, g = lane >> 4;
@@ -107,7 +114,7 @@ __global__ __launch_bounds__(512) void mx4_few_rows(const FewArgs p) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         uint32_t byte;
-        quantize_block<XT, VEC>(p.x, m * p.ldx, (b + s) * 32, p.K, x[s], byte);
+        quantize_block<XT>(p.x, m * p.ldx, (b + s) * 32, p.K, x[s], byte);
         xs |= byte << (8 * s);
       }
       mx_each<4>([&](auto sc) {
@@ -129,23 +136,22 @@ __global__ __launch_bounds__(512) void mx4_few_rows(const FewArgs p) {
   }
 }
 
-template <int XT, bool VEC>
+template <int XT>
 void few_rows(const FewArgs& p, hipStream_t s) {
   const int64_t turns = (p.blocks + 15) / 16;
   int waves = 1;
   while (waves < 8 && waves < turns) waves *= 2;
   const dim3 grid((unsigned)((p.N + 15) / 16));
-  if (p.M <= 16) mx4_few_rows<XT, VEC, 1><<<grid, 64 * waves, 0, s>>>(p);
-  else if (p.M <= 32) mx4_few_rows<XT, VEC, 2><<<grid, 64 * waves, 0, s>>>(p);
-  else mx4_few_rows<XT, VEC, 4><<<grid, 64 * waves, 0, s>>>(p);
+  if (p.M <= 16) mx4_few_rows<XT, 1><<<grid, 64 * waves, 0, s>>>(p);
+  else if (p.M <= 32) mx4_few_rows<XT, 2><<<grid, 64 * waves, 0, s>>>(p);
+  else mx4_few_rows<XT, 4><<<grid, 64 * waves, 0, s>>>(p);
 }
 
 int few_rows_any(int x_dtype, const FewArgs& p, hipStream_t s) {
-  const bool vec = mx_vec_rows(p.x, x_dtype, p.K, p.ldx);
   switch (x_dtype) {
-    case DIMQ_F32: vec ? few_rows<DIMQ_F32, true>(p, s) : few_rows<DIMQ_F32, false>(p, s); break;
-    case DIMQ_F16: vec ? few_rows<DIMQ_F16, true>(p, s) : few_rows<DIMQ_F16, false>(p, s); break;
-    default: vec ? few_rows<DIMQ_BF16, true>(p, s) : few_rows<DIMQ_BF16, false>(p, s);
+    case DIMQ_F32: few_rows<DIMQ_F32>(p, s); break;
+    case DIMQ_F16: few_rows<DIMQ_F16>(p, s); break;
+    default: few_rows<DIMQ_BF16>(p, s);
   }
   return check_launch("mxfp4_linear");
 }

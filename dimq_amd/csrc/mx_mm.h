@@ -17,7 +17,7 @@
 #include <type_traits>
 #include <utility>
 
-#include "mx.h"
+#include "mx_quant.h"
 
 namespace dimq {
 
@@ -86,48 +86,36 @@ __device__ __forceinline__ void mx_each(F&& f) {
 }
 
 // Columns n .. n + 7 of a bias or residual; those from `left` on are 0.
-__device__ __forceinline__ void mx_load8(const void* p, int dt, int64_t at, int left, bool vec, float (&v)[8]) {
-  if (vec && left >= 8 && dt != DIMQ_F64) {
-    if (dt == DIMQ_F32) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-      const float4 a = q[0], b = q[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t h = (w[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-        v[j] = dt == DIMQ_F16 ? f16_bits_to_float(h) : bf16_bits_to_float(h);
-      }
-    }
+__device__ __forceinline__ void mx_load8(const void* p, int dt, int64_t at, int left, float (&v)[8]) {
+  if (left >= 8 && dt != DIMQ_F64) {
+    if (dt == DIMQ_F32) mx_load_row8<DIMQ_F32>(p, at, 0, 8, v);
+    else if (dt == DIMQ_F16) mx_load_row8<DIMQ_F16>(p, at, 0, 8, v);
+    else mx_load_row8<DIMQ_BF16>(p, at, 0, 8, v);
     return;
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = j < left ? load_as_float(p, dt, at + j) : 0.0f;
 }
 
-typedef float mx_f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
-template <bool STREAM, class V>
-__device__ __forceinline__ void mx_put(void* p, const V& v) {
-  if constexpr (STREAM) __builtin_nontemporal_store(v, static_cast<V*>(p));
-  else *static_cast<V*>(p) = v;
+// 16 bytes to a multiple of the element's size.
+template <bool STREAM>
+__device__ __forceinline__ void mx_put(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+  const u4 v = {a, b, c, d};
+  if constexpr (STREAM) __builtin_nontemporal_store(v, static_cast<u4*>(p));
+  else *static_cast<u4*>(p) = v;
 }
 
-// Outputs n .. n + 7 (n % 8 == 0) of row m; bias: the column's (zeros without one); vec: rows and the residual's are
-// 16-byte aligned; STREAM: past the L2.
+// Outputs n .. n + 7 (n % 8 == 0) of row m; bias: the column's (zeros without one); STREAM: past the L2.
 template <bool STREAM>
-__device__ __forceinline__ void mx_store8(const MxOut& o, int64_t m, int64_t n, float (&v)[8], const float (&bias)[8],
-                                          bool vec) {
+__device__ __forceinline__ void mx_store8(const MxOut& o, int64_t m, int64_t n, float (&v)[8], const float (&bias)[8]) {
   const int64_t at = m * o.ld + n;
   const int left = o.cols - n < 8 ? (int)(o.cols - n) : 8;
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] += bias[j];
   if (o.res) {
     float r[8];
-    mx_load8(o.res, o.res_dtype, at, left, vec, r);
+    mx_load8(o.res, o.res_dtype, at, left, r);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += r[j];
   }
@@ -138,17 +126,17 @@ __device__ __forceinline__ void mx_store8(const MxOut& o, int64_t m, int64_t n, 
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = mx_gelu<true>(v[j]);
   }
-  if (vec && left == 8) {
+  if (left == 8) {
     if (o.dtype == DIMQ_F32) {
       float* y = static_cast<float*>(o.y) + at;
-      mx_put<STREAM>(y, mx_f4{v[0], v[1], v[2], v[3]});
-      mx_put<STREAM>(y + 4, mx_f4{v[4], v[5], v[6], v[7]});
+      mx_put<STREAM>(y, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      mx_put<STREAM>(y + 4, __float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
     } else {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         w[j] = o.dtype == DIMQ_F16 ? f16x2_rne(v[2 * j], v[2 * j + 1]) : bf16x2_rne(v[2 * j], v[2 * j + 1]);
-      mx_put<STREAM>(static_cast<uint16_t*>(o.y) + at, mx_u4{w[0], w[1], w[2], w[3]});
+      mx_put<STREAM>(static_cast<uint16_t*>(o.y) + at, w[0], w[1], w[2], w[3]);
     }
     return;
   }
@@ -169,10 +157,6 @@ __device__ __forceinline__ void mx_store4(const MxOut& o, int64_t m, int64_t n, 
     if (o.act == DIMQ_ACT_GELU) t = mx_gelu<true>(t);
     store_from_float(o.y, o.dtype, m * o.ld + n + j, t);
   }
-}
-
-__device__ __forceinline__ bool mx_vec_out(const MxOut& o) {
-  return o.ld % 8 == 0 && aligned(o.y, 16) && (!o.res || aligned(o.res, 16));
 }
 
 // Tiles in the order of their work-groups: those of one XCD (work-groups i, i + 8, ...) are a contiguous run, in columns
@@ -470,14 +454,13 @@ __global__ __launch_bounds__(T::NT) void mx_mm_kernel(const MxMm p) {
   // of the largest tile pass by the L2, which the operands need (16384 x 8192 -> 8192: 539 us with plain stores, 504 so)
   MxOut o = p.out;
   if (gridDim.y > 1) o.y = static_cast<float*>(o.y) + blockIdx.y * p.partial;
-  const bool vec = mx_vec_out(o);
   float* park = reinterpret_cast<float*>(sm) + wave * 32 * CB * 32;
   constexpr int LPR = CB * 4, RPI = 64 / LPR;  // lanes a row, rows a pass
   auto place = [&](int row, int chunk) MX_INLINE { return row * CB * 32 + ((chunk ^ (CB >= 2 ? row & 15 : (row >> 1) & 7)) << 2); };
   const int qc = lane % LPR;
   const int64_t n = c0 + wc * CB * 32 + qc * 8;
   float bias[8] = {};
-  if (o.bias && n < o.cols) mx_load8(o.bias, o.bias_dtype, n, o.cols - n < 8 ? (int)(o.cols - n) : 8, aligned(o.bias, 16), bias);
+  if (o.bias && n < o.cols) mx_load8(o.bias, o.bias_dtype, n, o.cols - n < 8 ? (int)(o.cols - n) : 8, bias);
   mx_each<RB>([&](auto ic) MX_INLINE {
     constexpr int i = decltype(ic)::value;
 #pragma unroll
@@ -494,7 +477,7 @@ __global__ __launch_bounds__(T::NT) void mx_mm_kernel(const MxMm p) {
       const float4 b = *reinterpret_cast<const float4*>(park + place(row, 2 * qc + 1));
       float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
       const int64_t m = r0 + (wr * RB + i) * 32 + row;
-      if (m < p.rows && n < o.cols) mx_store8<T::BR == 256>(o, m, n, v, bias, vec);
+      if (m < p.rows && n < o.cols) mx_store8<T::BR == 256>(o, m, n, v, bias);
     }
     __builtin_amdgcn_wave_barrier();
   });
@@ -515,8 +498,8 @@ static __global__ __launch_bounds__(256) void mx_reduce_kernel(const float* part
   }
   float bias[8] = {};
   if (n >= o.cols) return;
-  if (o.bias) mx_load8(o.bias, o.bias_dtype, n, o.cols - n < 8 ? (int)(o.cols - n) : 8, aligned(o.bias, 16), bias);
-  mx_store8<false>(o, m, n, v, bias, mx_vec_out(o));
+  if (o.bias) mx_load8(o.bias, o.bias_dtype, n, o.cols - n < 8 ? (int)(o.cols - n) : 8, bias);
+  mx_store8<false>(o, m, n, v, bias);
 }
 
 // How a product is cut: the tile (0: 256 x 256, 1: 128 x 128, 2: 64 x 64) and the slices of its reduction.

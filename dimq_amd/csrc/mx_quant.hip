@@ -75,7 +75,7 @@ __device__ __forceinline__ void turn_scales(const MxScaleTurn& t, uint32_t group
 // across the wave, the block's maximum by two lane exchanges.  Bound by the bytes: 4096 x 4096 fp32 to both formats
 // moves 67 MB in and 26 MB out.
 // TILED: the 4-bit output is a tiled product's operand, with its scales in that order.
-template <int XT, bool VEC, bool Q4, bool Q8, bool GELU, bool TILED>
+template <int XT, bool Q4, bool Q8, bool GELU, bool TILED>
 __global__ __launch_bounds__(256) void mx_quant_kernel(QuantArgs a, FastDiv div, uint32_t units) {
   uint32_t group = blockIdx.x;
   if constexpr (TILED) {
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(QuantArgs a, FastDiv div,
   const uint32_t q = threadIdx.x & 3u, row = div.quot(u), blk = u - row * div.d;
   const int64_t c = (int64_t)blk * kMxBlock + q * 8;
   float v[8];
-  mx_load_row8<XT, VEC>(a.x, row * a.ldx, c, a.cols, v);
+  mx_load_row8<XT>(a.x, row * a.ldx, c, a.cols, v);
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -119,25 +119,7 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(QuantArgs a, FastDiv div,
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = mx_gelu<XT == DIMQ_F32>(v[j]);
-    mx_store_row8<XT, VEC>(a.y, row * a.cols, c, a.cols, y);
-  }
-}
-
-template <int BITS>
-__device__ __forceinline__ void decode8(const void* codes, uint32_t byte, int64_t unit, float (&v)[8]) {
-  if constexpr (BITS == 4) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    const uint32_t w = static_cast<const uint32_t*>(codes)[unit];
-    const float s = mx_scale_operand(byte);
-    const f2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
-    const f2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
-    v[0] = p0.x; v[1] = p0.y; v[2] = p1.x; v[3] = p1.y;
-    v[4] = p2.x; v[5] = p2.y; v[6] = p3.x; v[7] = p3.y;
-  } else {
-    const uint2 w = static_cast<const uint2*>(codes)[unit];
-    const float s = mx_step8(byte);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * s;
+    mx_store_row8<XT>(a.y, row * a.cols, c, a.cols, y);
   }
 }
 
@@ -151,21 +133,21 @@ struct BackArgs {
 };
 
 // Codes to values (SLOPE 0), or the upstream gradient times GELU's slope at them.  Eight elements a lane, as above.
-template <int BITS, int YT, bool VEC, bool SLOPE>
+template <int BITS, int YT, bool SLOPE>
 __global__ __launch_bounds__(256) void mx_back_kernel(BackArgs a, FastDiv div, uint32_t units) {
   const uint32_t u = (blockIdx.x * 256u + threadIdx.x) >> 2;
   if (u >= units) return;
   const uint32_t q = threadIdx.x & 3u, row = div.quot(u), blk = u - row * div.d;
   const int64_t c = (int64_t)blk * kMxBlock + q * 8, b = (int64_t)u;
   float v[8];
-  decode8<BITS>(a.codes, a.scales[b], b * 4 + q, v);
+  mx_decode8<BITS>(a.codes, a.scales[b], b * 4 + q, v);
   if constexpr (SLOPE) {
     float g[8];
-    mx_load_row8<YT, VEC>(a.g, row * a.ldg, c, a.cols, g);
+    mx_load_row8<YT>(a.g, row * a.ldg, c, a.cols, g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = g[j] * mx_gelu_slope<YT == DIMQ_F32>(v[j]);
   }
-  mx_store_row8<YT, VEC>(a.y, row * a.cols, c, a.cols, v);
+  mx_store_row8<YT>(a.y, row * a.cols, c, a.cols, v);
 }
 
 // Units of a launch stay below 2^29 (FastDiv, grid of 2^31 threads): more rows go in several.
@@ -183,7 +165,7 @@ int launch_rows(int64_t rows, int64_t blocks, const char* what, F&& f) {
   return DIMQ_OK;
 }
 
-template <int XT, bool VEC>
+template <int XT>
 int quant_launch(const QuantArgs& a, hipStream_t s) {
   return launch_rows(a.rows, a.blocks, "mx_quantize", [&](int64_t r, FastDiv div, uint32_t units, dim3 grid) {
     QuantArgs b = a;
@@ -196,31 +178,25 @@ int quant_launch(const QuantArgs& a, hipStream_t s) {
     grid.x += b.turn.groups;
     if (b.codes8) b.codes8 += r * a.blocks8 * 32, b.scales8 += r * a.blocks8;
     if (b.y) b.y = static_cast<char*>(a.y) + r * a.cols * e;
-    if (b.y) mx_quant_kernel<XT, VEC, false, true, true, false><<<grid, 256, 0, s>>>(b, div, units);
-    else if (b.scale_rows && b.codes8) mx_quant_kernel<XT, VEC, true, true, false, true><<<grid, 256, 0, s>>>(b, div, units);
-    else if (b.scale_rows) mx_quant_kernel<XT, VEC, true, false, false, true><<<grid, 256, 0, s>>>(b, div, units);
-    else if (b.codes4 && b.codes8) mx_quant_kernel<XT, VEC, true, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
-    else if (b.codes4) mx_quant_kernel<XT, VEC, true, false, false, false><<<grid, 256, 0, s>>>(b, div, units);
-    else mx_quant_kernel<XT, VEC, false, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
+    if (b.y) mx_quant_kernel<XT, false, true, true, false><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.scale_rows && b.codes8) mx_quant_kernel<XT, true, true, false, true><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.scale_rows) mx_quant_kernel<XT, true, false, false, true><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.codes4 && b.codes8) mx_quant_kernel<XT, true, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.codes4) mx_quant_kernel<XT, true, false, false, false><<<grid, 256, 0, s>>>(b, div, units);
+    else mx_quant_kernel<XT, false, true, false, false><<<grid, 256, 0, s>>>(b, div, units);
   });
-}
-
-template <int XT>
-int quant_typed(const QuantArgs& a, hipStream_t s) {
-  const bool vec = mx_vec_rows(a.x, XT, a.cols, a.ldx) && (!a.y || mx_vec_rows(a.y, XT, a.cols, a.cols));
-  return vec ? quant_launch<XT, true>(a, s) : quant_launch<XT, false>(a, s);
 }
 
 int quant_any(int x_dtype, const QuantArgs& a, hipStream_t s) {
   if (a.rows == 0 || a.cols == 0) return DIMQ_OK;
   switch (x_dtype) {
-    case DIMQ_F32: return quant_typed<DIMQ_F32>(a, s);
-    case DIMQ_F16: return quant_typed<DIMQ_F16>(a, s);
-    default: return quant_typed<DIMQ_BF16>(a, s);
+    case DIMQ_F32: return quant_launch<DIMQ_F32>(a, s);
+    case DIMQ_F16: return quant_launch<DIMQ_F16>(a, s);
+    default: return quant_launch<DIMQ_BF16>(a, s);
   }
 }
 
-template <int BITS, int YT, bool VEC, bool SLOPE>
+template <int BITS, int YT, bool SLOPE>
 int back_launch(int64_t rows, int64_t blocks, const BackArgs& a, hipStream_t s) {
   return launch_rows(rows, blocks, "mx_dequantize", [&](int64_t r, FastDiv div, uint32_t units, dim3 grid) {
     BackArgs b = a;
@@ -229,7 +205,7 @@ int back_launch(int64_t rows, int64_t blocks, const BackArgs& a, hipStream_t s) 
     b.scales = a.scales + r * blocks;
     if (b.g) b.g = static_cast<const char*>(a.g) + r * a.ldg * e;
     b.y = static_cast<char*>(a.y) + r * a.cols * e;
-    mx_back_kernel<BITS, YT, VEC, SLOPE><<<grid, 256, 0, s>>>(b, div, units);
+    mx_back_kernel<BITS, YT, SLOPE><<<grid, 256, 0, s>>>(b, div, units);
   });
 }
 
@@ -237,15 +213,11 @@ template <int BITS, bool SLOPE>
 int back_any(int y_dtype, int64_t rows, const BackArgs& a, hipStream_t s) {
   if (rows == 0 || a.cols == 0) return DIMQ_OK;
   const int64_t blocks = mx_blocks(a.cols);
-  const bool vec = mx_vec_rows(a.y, y_dtype, a.cols, a.cols) && (!SLOPE || mx_vec_rows(a.g, y_dtype, a.cols, a.ldg));
-#define DIMQ_MX_BACK(T) \
-  return vec ? back_launch<BITS, T, true, SLOPE>(rows, blocks, a, s) : back_launch<BITS, T, false, SLOPE>(rows, blocks, a, s)
   switch (y_dtype) {
-    case DIMQ_F32: DIMQ_MX_BACK(DIMQ_F32);
-    case DIMQ_F16: DIMQ_MX_BACK(DIMQ_F16);
-    default: DIMQ_MX_BACK(DIMQ_BF16);
+    case DIMQ_F32: return back_launch<BITS, DIMQ_F32, SLOPE>(rows, blocks, a, s);
+    case DIMQ_F16: return back_launch<BITS, DIMQ_F16, SLOPE>(rows, blocks, a, s);
+    default: return back_launch<BITS, DIMQ_BF16, SLOPE>(rows, blocks, a, s);
   }
-#undef DIMQ_MX_BACK
 }
 
 int check_codes(const char* what, const void* codes, const void* scales) {

@@ -676,16 +676,19 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     const int64_t K = ctx->saved_data["k"].toInt();
     const bool b = ctx->saved_data["b"].toBool();
     const auto bdt = static_cast<at::ScalarType>(ctx->saved_data["bdt"].toInt());
+    const char* op = "mx.linear";
+    const Rows r(g, op, "gradient");
     Tensor gx, gw, gb;
-    if (saved[0].defined()) gx = mxfp4_linear_grad_input(g, saved[0], saved[1], K, std::nullopt);
-    if (saved[2].defined()) {
-      const auto r = linear_grad_weight(g, saved[2], saved[3], K, b,
-                                        static_cast<at::ScalarType>(ctx->saved_data["wdt"].toInt()), bdt);
-      gw = std::get<0>(r);
-      if (b) gb = std::get<1>(r);
-    } else if (b) {
-      gb = g.reshape({-1, g.size(-1)}).sum(0, false, at::kFloat).to(bdt);
-    }
+    if (saved[0].defined()) gx = at::empty(out_shape(g, K), g.options());
+    if (saved[2].defined())
+      gw = at::empty({r.cols, K}, g.options().dtype(static_cast<at::ScalarType>(ctx->saved_data["wdt"].toInt())));
+    if (b) gb = at::empty({r.cols}, g.options().dtype(bdt));
+    const On on(g);
+    const Tensor ws = workspace(dimq_mx_linear_backward_workspace_bytes(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, K,
+                                                                        gx.defined() + 2 * gw.defined() + 4 * b), g);
+    check_rc(dimq_mx_linear_backward(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, pu8(saved[0]), pu8(saved[1]), pi8(saved[2]),
+                                     pu8(saved[3]), K, ptr(gx), gx.defined() ? dt(gx) : 0, ptr(gw), gw.defined() ? dt(gw) : 0,
+                                     ptr(gb), b ? dt(gb) : 0, ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
     return {gx, gw, gb};
   }
 };

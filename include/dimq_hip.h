@@ -576,7 +576,8 @@ int dimq_mxfp4_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t 
  *   gw = g^T Q8(x)       (x from its 8-bit checkpoint), gb = sum of g over m
  * Every product is exact (g as a sum of bf16 parts, codes times scales in
  * bf16), the sums are fp32 in a fixed order, outputs [M, K], [N, K], [N]
- * (nullable) contiguous in their dtypes.  M = 0 gives zeros. */
+ * (nullable) contiguous in their dtypes.  M = 0 gives zeros.  The queries
+ * take g because a copy is made of one that is not 16-byte aligned. */
 int64_t dimq_mx_grad_input_workspace_bytes(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
 int dimq_mxfp4_linear_grad_input(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, const uint8_t* codes,
                                  const uint8_t* scales, int64_t K, void* gx, int gx_dtype, void* workspace,
@@ -585,6 +586,16 @@ int64_t dimq_mx_grad_weight_workspace_bytes(const void* g, int g_dtype, int64_t 
 int dimq_mx_linear_grad_weight(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, const int8_t* codes8,
                                const uint8_t* scales8, int64_t K, void* gw, int gw_dtype, void* gb, int gb_dtype,
                                void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Those gradients in one call, each where its output is given (gx, gw, gb
+ * nullable; `outputs` of the query: 1 gx, 2 gw, 4 gb).  The two calls above
+ * are parts of it; together they share the split of g. */
+int64_t dimq_mx_linear_backward_workspace_bytes(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K,
+                                                int outputs);
+int dimq_mx_linear_backward(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, const uint8_t* codes,
+                            const uint8_t* scales, const int8_t* codes8, const uint8_t* scales8, int64_t K, void* gx,
+                            int gx_dtype, void* gw, int gw_dtype, void* gb, int gb_dtype, void* workspace,
+                            int64_t workspace_bytes, void* stream);
 
 /* y = gelu(h) = h Phi(h) and h's 8-bit form from one read of h (y [rows, cols]
  * contiguous in h's dtype), and the gradient gh = g gelu'(Q8(h)) in g's dtype. */
