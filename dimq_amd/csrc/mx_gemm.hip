@@ -20,35 +20,83 @@ struct FewArgs {
   MxOut out;
 };
 
-// The lane's block of x in 4 bits: 32 elements from column c of a row.  16-bit elements stay in pairs: integer maxima of
-// their magnitudes and the conversions that take pairs, 50 instructions a block where fp32 copies take 150, which is what
-// the kernel spends its time on from 8 rows on (16 x 4096 -> 4096: 13.3 us with copies).
+// A block of x as it lies in memory, and how its loads are bounded: kWhole no bound, kGroups whole groups of 8 elements
+// only (addresses past the row go to its start, their values to zero: loads stay free of branches, so that all of a turn's
+// are in flight together), kAny element by element.
+enum { kWhole, kGroups, kAny };
 template <int XT>
-__device__ __forceinline__ void quantize_block(const void* x, int64_t at, int64_t c, int64_t cols, uint4& codes, uint32_t& byte) {
-  if constexpr (XT != DIMQ_F32) {
+struct RawBlock {
+  static constexpr int N = XT == DIMQ_F32 ? 8 : 4;  // 16-byte pieces
+  uint4 v[N];
+};
+
+template <int XT, int BOUND>
+__device__ __forceinline__ void load_block(const void* x, int64_t at, int64_t c, int64_t cols, RawBlock<XT>& o) {
+  constexpr int E = XT == DIMQ_F32 ? 4 : 8;  // elements a piece
+  constexpr int SIZE = XT == DIMQ_F32 ? 4 : 2;
+#pragma unroll
+  for (int i = 0; i < RawBlock<XT>::N; ++i) {
+    const int64_t e = c + E * i;
+    const char* p = static_cast<const char*>(x) + at * SIZE;
+    if constexpr (BOUND != kAny) {
+      o.v[i] = mx_read16(p + (BOUND == kWhole || e < cols ? e : 0) * SIZE);
+    } else {
+      o.v[i] = make_uint4(0, 0, 0, 0);
+      if (e + E <= cols) {
+        o.v[i] = mx_read16(p + e * SIZE);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          if (e + j >= cols) break;
+          if constexpr (SIZE == 4) (&o.v[i].x)[j] = reinterpret_cast<const uint32_t*>(p)[e + j];
+          else (&o.v[i].x)[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e + j] << (16 * (j & 1));
+        }
+      }
+    }
+  }
+}
+
+template <int XT>
+__device__ __forceinline__ void clear_past_end(int64_t c, int64_t cols, RawBlock<XT>& o) {
+  constexpr int E = XT == DIMQ_F32 ? 4 : 8;
+#pragma unroll
+  for (int i = 0; i < RawBlock<XT>::N; ++i)
+    if (c + E * i >= cols) o.v[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Its 4-bit codes and scale.  16-bit elements stay in pairs: integer maxima of their magnitudes and the conversions that
+// take pairs, 50 instructions a block where fp32 copies take 150.
+template <int XT>
+__device__ __forceinline__ void quantize_block(const RawBlock<XT>& x, uint4& codes, uint32_t& byte) {
+  uint32_t o[4];
+  if constexpr (XT == DIMQ_F32) {
+    float v[4][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w[4] = {x.v[i].x, x.v[i].y, x.v[i].z, x.v[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[i / 2][4 * (i & 1) + j] = __uint_as_float(w[j]);
+        const uint32_t m = w[j] & 0x7fffffffu;
+        top = top > m ? top : m;
+      }
+    }
+    byte = mx_scale_byte<2>(top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = mx_codes4(v[i], mx_scale_operand(byte));
+  } else {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint16_t* p = static_cast<const uint16_t*>(x) + at + c + 8 * i;
-      uint4 t = make_uint4(0, 0, 0, 0);
-      if (c + 8 * i + 8 <= cols) {
-        t = mx_read16(p);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + 8 * i + j < cols) (&t.x)[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
-      }
-      w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
-    }
+    for (int i = 0; i < 4; ++i) w[4 * i] = x.v[i].x, w[4 * i + 1] = x.v[i].y, w[4 * i + 2] = x.v[i].z, w[4 * i + 3] = x.v[i].w;
     u16x2 top = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
     const uint32_t m = top.x > top.y ? top.x : top.y;
     byte = mx_scale_byte<2>(XT == DIMQ_BF16 ? m << 16 : __float_as_uint(f16_bits_to_float(m)));
     const float s = mx_scale_operand(byte);
-    uint32_t o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t q = 0;
@@ -57,82 +105,96 @@ __device__ __forceinline__ void quantize_block(const void* x, int64_t at, int64_
         if constexpr (XT == DIMQ_BF16) q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, w[4 * i + j]), s, j);
         else q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(f16x2, w[4 * i + j]), s, j);
       });
-      o[i] = byte == kMxNan ? 0u : q;
-    }
-    codes = make_uint4(o[0], o[1], o[2], o[3]);
-    return;
-  }
-  float v[4][8];
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    mx_load_row8<XT>(x, at, c + 8 * i, cols, v[i]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t m = __float_as_uint(v[i][j]) & 0x7fffffffu;
-      top = top > m ? top : m;
+      o[i] = q;
     }
   }
-  byte = mx_scale_byte<2>(top);
-  const float s = mx_scale_operand(byte);
-  codes = make_uint4(mx_codes4(v[0], s), mx_codes4(v[1], s), mx_codes4(v[2], s), mx_codes4(v[3], s));
-  if (byte == kMxNan) codes = make_uint4(0, 0, 0, 0);
+  codes = byte == kMxNan ? make_uint4(0, 0, 0, 0) : make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Up to 16 MT rows.  A work-group owns 16 outputs; its waves take the reduction in turns of 16 blocks, lane l the blocks
-// 4 (l / 16) .. + 3 of a turn for row l % 16 of either operand: 64 contiguous bytes of codes and one dword of scales,
-// whose bytes the four instructions select.  Bound by latency: all of a turn's loads are in flight at once, and with 16
-// outputs and 8 waves a work-group the 8.4 MB of a 4096 x 4096 layer are requested by the first turn of 256 work-groups.
-template <int XT, int MT>
+// A turn of a wave: 16 blocks from b0, lane l the blocks b0 + 4 (l / 16) .. + 3 for row l % 16 of either operand.
+template <int XT, int BOUND>
+__device__ __forceinline__ void few_rows_turn(const FewArgs& p, const uint8_t* wrow, const uint8_t* srow, int64_t xat, int r,
+                                              int64_t b, f32x4& acc) {
+  constexpr bool whole = BOUND == kWhole;
+  uint4 w[4];
+  uint32_t ws = 0;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) w[s] = *reinterpret_cast<const uint4*>(wrow + (whole || b + s < p.blocks ? b + s : 0) * 16);
+  if (p.wide_scales) {  // blocks % 4 == 0
+    ws = *reinterpret_cast<const uint32_t*>(srow + (whole || b < p.blocks ? b : 0));
+  } else {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) ws |= (uint32_t)srow[whole || b + s < p.blocks ? b + s : 0] << (8 * s);
+  }
+  RawBlock<XT> raw[4] = {};
+  if (r < p.M) {  // rows that are not there cost no loads
+#pragma unroll
+    for (int s = 0; s < 4; ++s) load_block<XT, BOUND>(p.x, xat, (b + s) * 32, p.K, raw[s]);
+  }
+  uint32_t xs = 0;
+  uint4 x[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    if constexpr (BOUND == kGroups) clear_past_end<XT>((b + s) * 32, p.K, raw[s]);
+    uint32_t byte;
+    quantize_block<XT>(raw[s], x[s], byte);
+    xs |= byte << (8 * s);
+  }
+  // past the weights' last block: codes of x are zero there, and so has to be the scale (another block's may be NaN)
+  if constexpr (!whole) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (b + s >= p.blocks) ws &= ~(255u << (8 * s));
+  }
+  mx_each<4>([&](auto sc) {
+    constexpr int s = decltype(sc)::value;
+    const i32x8 u = {(int)w[s].x, (int)w[s].y, (int)w[s].z, (int)w[s].w, 0, 0, 0, 0};
+    const i32x8 v = {(int)x[s].x, (int)x[s].y, (int)x[s].z, (int)x[s].w, 0, 0, 0, 0};
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(u, v, acc, 4, 4, s, (int)ws, s, (int)xs);
+  });
+}
+
+// Up to 16 rows.  A work-group owns 16 outputs; its waves take the reduction in turns of 16 blocks: 64 contiguous bytes of
+// codes and one dword of scales a lane, whose bytes the four instructions select.  Bound by latency: with 8 waves a
+// work-group the 8.4 MB of a 4096 x 4096 layer are requested by the first turn of 256 work-groups.
+template <int XT>
 __global__ __launch_bounds__(512) void mx4_few_rows(const FewArgs p) {
-  __shared__ f32x4 red[8 * MT * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r = lane & 15, g = lane >> 4;
+  __shared__ f32x4 red[8 * 64];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t n = n0 + r < p.N ? n0 + r : p.N - 1;
   const uint8_t* wrow = p.codes + n * p.blocks * 16;
   const uint8_t* srow = p.scales + n * p.blocks;
-  f32x4 acc[MT] = {};
+  const int64_t xat = (r < p.M ? r : 0) * p.ldx;
+  f32x4 acc = {};
   for (int64_t b0 = wave * 16; b0 < p.blocks; b0 += waves * 16) {
     const int64_t b = b0 + 4 * g;
-    uint4 w[4];
-    uint32_t ws = 0;
+    if ((b0 + 16) * 32 <= p.K) few_rows_turn<XT, kWhole>(p, wrow, srow, xat, r, b, acc);
+    else if (p.K % 8 == 0) few_rows_turn<XT, kGroups>(p, wrow, srow, xat, r, b, acc);
+    else few_rows_turn<XT, kAny>(p, wrow, srow, xat, r, b, acc);
+  }
+  // the first wave adds up and stores: lane l the outputs n0 + 4 (l / 16) .. + 3 of row l % 16
+  const int64_t n4 = n0 + g * 4;
+  const int left = p.N - n4 < 4 ? (int)(p.N - n4) : 4;
+  float bias[4] = {}, res[4] = {};
+  if (wave == 0 && r < p.M) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-      w[s] = b + s < p.blocks ? *reinterpret_cast<const uint4*>(wrow + (b + s) * 16) : make_uint4(0, 0, 0, 0);
-    if (p.wide_scales) {
-      if (b < p.blocks) ws = *reinterpret_cast<const uint32_t*>(srow + b);
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (b + s < p.blocks) ws |= (uint32_t)srow[b + s] << (8 * s);
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int64_t m = 16 * t + r < p.M ? 16 * t + r : p.M - 1;
-      uint4 x[4];
-      uint32_t xs = 0;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        uint32_t byte;
-        quantize_block<XT>(p.x, m * p.ldx, (b + s) * 32, p.K, x[s], byte);
-        xs |= byte << (8 * s);
-      }
-      mx_each<4>([&](auto sc) {
-        constexpr int s = decltype(sc)::value;
-        const i32x8 a = {(int)w[s].x, (int)w[s].y, (int)w[s].z, (int)w[s].w, 0, 0, 0, 0};
-        const i32x8 c = {(int)x[s].x, (int)x[s].y, (int)x[s].z, (int)x[s].w, 0, 0, 0, 0};
-        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, c, acc[t], 4, 4, s, (int)ws, s, (int)xs);
-      });
+    for (int j = 0; j < 4; ++j) {
+      if (p.out.bias && j < left) bias[j] = load_as_float(p.out.bias, p.out.bias_dtype, n4 + j);
+      if (p.out.res && j < left) res[j] = load_as_float(p.out.res, p.out.res_dtype, r * p.out.ld + n4 + j);
     }
   }
-#pragma unroll
-  for (int t = 0; t < MT; ++t) red[(wave * MT + t) * 64 + lane] = acc[t];
+  red[wave * 64 + lane] = acc;
   __syncthreads();
-  for (int i = threadIdx.x; i < MT * 64; i += blockDim.x) {
-    f32x4 sum = red[i];
-    for (int w = 1; w < waves; ++w) sum += red[w * MT * 64 + i];
-    const int64_t m = i / 64 * 16 + (i & 15), n4 = n0 + ((i >> 4) & 3) * 4;
-    if (m < p.M) mx_store4(p.out, m, n4, sum);
+  if (wave != 0 || r >= p.M) return;
+  for (int w = 1; w < waves; ++w) acc += red[w * 64 + lane];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float t = acc[j] + bias[j] + res[j];
+    if (p.out.act == DIMQ_ACT_RELU) t = t < 0.0f ? 0.0f : t;
+    if (p.out.act == DIMQ_ACT_GELU) t = mx_gelu<true>(t);
+    if (j < left) store_from_float(p.out.y, p.out.dtype, r * p.out.ld + n4 + j, t);
   }
 }
 
@@ -141,10 +203,7 @@ void few_rows(const FewArgs& p, hipStream_t s) {
   const int64_t turns = (p.blocks + 15) / 16;
   int waves = 1;
   while (waves < 8 && waves < turns) waves *= 2;
-  const dim3 grid((unsigned)((p.N + 15) / 16));
-  if (p.M <= 16) mx4_few_rows<XT, 1><<<grid, 64 * waves, 0, s>>>(p);
-  else if (p.M <= 32) mx4_few_rows<XT, 2><<<grid, 64 * waves, 0, s>>>(p);
-  else mx4_few_rows<XT, 4><<<grid, 64 * waves, 0, s>>>(p);
+  mx4_few_rows<XT><<<dim3((unsigned)((p.N + 15) / 16)), 64 * waves, 0, s>>>(p);
 }
 
 int few_rows_any(int x_dtype, const FewArgs& p, hipStream_t s) {
@@ -156,8 +215,16 @@ int few_rows_any(int x_dtype, const FewArgs& p, hipStream_t s) {
   return check_launch("mxfp4_linear");
 }
 
-// Rows up to which the one launch is taken.
-constexpr int64_t kFewRows = 16;
+// Whether the one launch is the faster route.  It takes 3.6 us and, for each 4,096 of K and each work-group of a CU, 2.3 us
+// and 0.17 a row (fp32 x: 4.0, 2.8 and 0.31); the other route 5 us for its launches and the tiled product.  Measured with
+// 16-bit x, one launch / other route: 768 -> 768 with 16 rows 4.9 us / 6.8; 4096 -> 4096 with 1 row 5.9, with 16 8.4 / 11.3;
+// 8192 -> 8192 with 1 row 14.3 / 16.3, with 16 24.4 / 16.7.
+bool few_rows_pay(bool f32, int64_t M, int64_t K, int64_t N) {
+  if (M > 16) return false;
+  const double units = K / 4096.0 * (double)((N + 4095) / 4096);
+  const double us = f32 ? 4.0 + units * (2.8 + 0.31 * M) : 3.6 + units * (2.3 + 0.17 * M);
+  return us <= 5.0 + mx_plan(true, M, N, (mx_blocks(K) + 7) / 8).us;
+}
 
 // Workspace: x's codes and scales, the weights' scales, the slices of a split reduction.
 struct Layout {
@@ -180,7 +247,7 @@ struct Layout {
 using namespace dimq;
 
 extern "C" int64_t dimq_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N) {
-  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  if (M <= 0 || K <= 0 || N <= 0 || (few_rows_pay(false, M, K, N) && few_rows_pay(true, M, K, N))) return 0;
   return Layout(M, K, N).bytes;
 }
 
@@ -204,7 +271,8 @@ extern "C" int dimq_mxfp4_linear(const void* x, int x_dtype, int64_t M, int64_t 
   const int64_t blocks = mx_blocks(K), pitch = mx_pad8(blocks);
   hipStream_t s = as_stream(stream);
   const MxOut out{y, y_dtype, N, N, bias, bias_dtype, residual, residual_dtype, activation};
-  if (M <= kFewRows && !codes8) {
+  if (few_rows_pay(x_dtype == DIMQ_F32, M, K, N)) {
+    if (codes8 && (rc = dimq_mx_quantize(x, x_dtype, M, K, ldx, nullptr, nullptr, 0, codes8, scales8, stream)) != DIMQ_OK) return rc;
     DIMQ_CHECK((N + 15) / 16 < (1ll << 31), "mxfp4_linear: too many outputs");
     return few_rows_any(x_dtype, {x, ldx, M, K, codes, scales, N, blocks, blocks % 4 == 0 && aligned(scales, 4), out}, s);
   }

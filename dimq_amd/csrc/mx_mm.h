@@ -145,20 +145,6 @@ __device__ __forceinline__ void mx_store8(const MxOut& o, int64_t m, int64_t n, 
     if (j < left) store_from_float(o.y, o.dtype, at + j, v[j]);
 }
 
-// Outputs n .. n + 3 of row m, one by one.
-__device__ __forceinline__ void mx_store4(const MxOut& o, int64_t m, int64_t n, f32x4 v) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (n + j >= o.cols) return;
-    float t = v[j];
-    if (o.bias) t += load_as_float(o.bias, o.bias_dtype, n + j);
-    if (o.res) t += load_as_float(o.res, o.res_dtype, m * o.ld + n + j);
-    if (o.act == DIMQ_ACT_RELU) t = t < 0.0f ? 0.0f : t;
-    if (o.act == DIMQ_ACT_GELU) t = mx_gelu<true>(t);
-    store_from_float(o.y, o.dtype, m * o.ld + n + j, t);
-  }
-}
-
 // Tiles in the order of their work-groups: those of one XCD (work-groups i, i + 8, ...) are a contiguous run, in columns
 // of 8 row tiles, so that the 32 tiles an XCD works on share few operand rows in its L2: 8 x 4 tiles read 12 tile edges,
 // 1 x 32 would read 33.
@@ -505,6 +491,7 @@ static __global__ __launch_bounds__(256) void mx_reduce_kernel(const float* part
 // How a product is cut: the tile (0: 256 x 256, 1: 128 x 128, 2: 64 x 64) and the slices of its reduction.
 struct MxPlan {
   int tile, splits;
+  double us;  // estimated
 };
 
 inline int64_t mx_pad8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -524,8 +511,7 @@ inline int64_t mx_partial_bytes(const MxPlan& pl, int64_t rows, int64_t cols) {
 // 0.60 n), of the 64 tile 0.24 / 0.20 n (FP4: 0.41 / 0.25 n).  On
 // 171 products, each with 5 to 20 plans measured, the estimate's choice is 1.6 % slower than the best one in the mean.
 inline MxPlan mx_plan(bool fp4, int64_t rows, int64_t cols, int64_t stages) {
-  MxPlan best{2, 1};
-  double least = 1e300;
+  MxPlan best{2, 1, 1e300};
   for (int tile = 0; tile < 3; ++tile) {
     for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (splits > 1 && stages < 4 * splits) break;
@@ -540,7 +526,7 @@ inline MxPlan mx_plan(bool fp4, int64_t rows, int64_t cols, int64_t stages) {
         us = each * (alone > share ? alone : share) + n * (tile == 1 ? 2.8 : 0.8);
       }
       if (splits > 1) us += 4.0 + (double)splits * rows * cols * 8 / 5e6;
-      if (us < least) least = us, best = MxPlan{tile, splits};
+      if (us < best.us) best = MxPlan{tile, splits, us};
     }
   }
   return best;

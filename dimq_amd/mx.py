@@ -10,7 +10,8 @@ infinity stands for NaN throughout.  ``Q4(x)`` and ``Q8(x)`` are the values that
 * Training: ``linear`` (``MXFP4TrainLinear``) runs that layer on the master weights with straight-through gradients and
   keeps its input in 8 bits for the weight gradient; ``gelu`` keeps its input in 8 bits too.
 
-All of it is for CUDA (HIP) tensors in fp32, fp16 and bf16; the gradients are those of the formulas in each function's
+The functions without gradients are torch ops too (``torch.ops.dimq.quantize_mxfp4`` and so on).  All of it is for CUDA
+(HIP) tensors in fp32, fp16 and bf16; the gradients are those of the formulas in each function's
 description and have no gradients of their own.
 """
 
@@ -23,32 +24,30 @@ from torch import Tensor
 from ._C import _native
 from .ops import ACTIVATIONS
 
-_ops = torch.ops.dimq
-
 
 def quantize_mxfp4(x: Tensor) -> tuple[Tensor, Tensor]:
     """(codes, scales) of x's last dimension in 4 bits: uint8 ``[..., 16 * blocks]`` and ``[..., blocks]``."""
-    return _ops.quantize_mxfp4(x)
+    return _native.quantize_mxfp4(x)
 
 
 def compress_activation(x: Tensor) -> tuple[Tensor, Tensor]:
     """(codes, scales) of x's last dimension in 8 bits: int8 ``[..., 32 * blocks]`` and uint8 ``[..., blocks]``."""
-    return _ops.compress_activation(x)
+    return _native.compress_activation(x)
 
 
 def quantize_and_compress(x: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """``quantize_mxfp4(x) + compress_activation(x)`` from one read of x."""
-    return _ops.quantize_and_compress(x)
+    return _native.quantize_and_compress(x)
 
 
 def dequantize_mxfp4(codes: Tensor, scales: Tensor, size: int, dtype: torch.dtype = torch.float32) -> Tensor:
     """The values of 4-bit codes, ``[..., size]``, rounded to ``dtype`` (exact in fp32 and bf16)."""
-    return _ops.dequantize_mxfp4(codes, scales, size, dtype)
+    return _native.dequantize_mxfp4(codes, scales, size, dtype)
 
 
 def decompress_activation(codes: Tensor, scales: Tensor, size: int, dtype: torch.dtype = torch.float32) -> Tensor:
     """The values of 8-bit codes, ``[..., size]``, rounded to ``dtype`` (exact in fp32 and bf16)."""
-    return _ops.decompress_activation(codes, scales, size, dtype)
+    return _native.decompress_activation(codes, scales, size, dtype)
 
 
 def mxfp4_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Tensor | None = None, *, residual: Tensor | None = None,
@@ -57,20 +56,20 @@ def mxfp4_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Tensor | None =
     activation None, "relu" or "gelu" (exact); the output in ``out_dtype`` (x's by default)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
-    return _ops.mxfp4_linear(x, codes, scales, bias, residual, ACTIVATIONS[activation], out_dtype)
+    return _native.mxfp4_linear(x, codes, scales, bias, residual, ACTIVATIONS[activation], out_dtype)
 
 
 def mxfp4_linear_grad_input(grad: Tensor, codes: Tensor, scales: Tensor, in_features: int,
                             out_dtype: torch.dtype | None = None) -> Tensor:
     """``grad W``: the gradient to that layer's input, straight through its quantization."""
-    return _ops.mxfp4_linear_grad_input(grad, codes, scales, in_features, out_dtype)
+    return _native.mxfp4_linear_grad_input(grad, codes, scales, in_features, out_dtype)
 
 
 def linear_grad_weight(grad: Tensor, codes: Tensor, scales: Tensor, in_features: int, bias: bool = True,
                        out_dtype: torch.dtype = torch.float32) -> tuple[Tensor, Tensor | None]:
     """``(grad^T Q8(x), grad summed over the rows)`` for the 8-bit codes of a layer's input x; the second is None without
     ``bias``."""
-    gw, gb = _ops.linear_grad_weight(grad, codes, scales, in_features, bias, out_dtype)
+    gw, gb = _native.linear_grad_weight(grad, codes, scales, in_features, bias, out_dtype, None)
     return gw, gb if bias else None
 
 
