@@ -98,14 +98,21 @@ __device__ __forceinline__ void sum_part(const PrepArgs& p, uint32_t group, floa
   const int64_t n = ((int64_t)(group - slice * p.sum_cols) * 64 + c) * 8, m0 = slice * p.sum_rows;
   const int64_t m1 = m0 + p.sum_rows < p.M ? m0 + p.sum_rows : p.M;
   float s[8] = {};
-  if (n < p.N)
-#pragma unroll 8
-    for (int64_t m = m0 + w; m < m1; m += 4) {
-      float v[8];
-      mx_load_row8<DT>(p.g, m * p.ld, n, p.N, v);
+  auto add = [&](int64_t m, int64_t cols) {
+    float v[8];
+    mx_load_row8<DT>(p.g, m * p.ld + n, 0, cols, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    for (int j = 0; j < 8; ++j) s[j] += v[j];
+  };
+  if (n < p.N) {
+    int64_t m = m0 + w;
+    if (n + 8 <= p.N) {  // eight rows' loads in flight, with no branch between them
+      for (; m + 28 < m1; m += 32)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) add(m + 4 * i, 8);
     }
+    for (; m < m1; m += 4) add(m, p.N - n);
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) red[w][j][c] = s[j];
   __syncthreads();

@@ -504,11 +504,18 @@ inline int64_t mx_partial_bytes(const MxPlan& pl, int64_t rows, int64_t cols) {
   return pl.splits > 1 ? pl.splits * rows * mx_pad8(cols) * 4 : 0;
 }
 
+// Whether the 128 tile takes a ring of four slots, which leaves a CU room for one work-group only: where no CU has two and
+// the reduction is long enough to fill it (515 x 4096 summed over 4096, 160 work-groups: 40.9 us with two slots, 29.5 with
+// four; 64 x 4096 codes over 4096, 32 of them: 12.2 and 12.8).
+inline bool mx_deep(const MxPlan& pl, int64_t rows, int64_t cols, int64_t stages) {
+  return mx_tiles(1, rows, cols) * pl.splits <= 256 && stages >= 24 * pl.splits;
+}
+
 // The plan of the least estimated time.  A tile's stage takes, in us on a card of 256 CUs, the larger of its latency (a
 // CU's only work-group) and its share where n of them run on a CU; a tile adds its filling and epilogue; slices add a
 // launch and their bytes at 5 TB/s.  Measured on products of 16 to 16,384 rows (bf16 ones: both gradients): a stage of
 // the 256 tile 1.3 us on part of the card and 1.65 (FP4: 2.0) on all of it, of the 128 tile 0.60 / 0.465 n (FP4: 0.73 /
-// 0.60 n), of the 64 tile 0.24 / 0.20 n (FP4: 0.41 / 0.25 n).  On
+// 0.60 n; 0.42 and 0.55 with the deeper ring), of the 64 tile 0.24 / 0.20 n (FP4: 0.41 / 0.25 n).  On
 // 171 products, each with 5 to 20 plans measured, the estimate's choice is 1.6 % slower than the best one in the mean.
 inline MxPlan mx_plan(bool fp4, int64_t rows, int64_t cols, int64_t stages) {
   MxPlan best{2, 1, 1e300};
@@ -521,7 +528,8 @@ inline MxPlan mx_plan(bool fp4, int64_t rows, int64_t cols, int64_t stages) {
       if (tile == 0) {
         us = n * (each * (groups < 192 ? 1.3 : fp4 ? 2.0 : 1.65) + 6.0);
       } else {
-        const double alone = tile == 1 ? (fp4 ? 0.73 : 0.60) : (fp4 ? 0.41 : 0.24);
+        const bool deep = tile == 1 && mx_deep({1, splits, 0}, rows, cols, stages);
+        const double alone = deep ? (fp4 ? 0.55 : 0.42) : tile == 1 ? (fp4 ? 0.73 : 0.60) : (fp4 ? 0.41 : 0.24);
         const double share = n * (tile == 1 ? (fp4 ? 0.60 : 0.465) : (fp4 ? 0.25 : 0.20));
         us = each * (alone > share ? alone : share) + n * (tile == 1 ? 2.8 : 0.8);
       }
@@ -550,10 +558,14 @@ int mx_mm(MxMm p, const MxPlan& pl, float* partial, hipStream_t s, const char* w
     p.partial = p.rows * mx_pad8(p.cols);
     p.out = MxOut{partial, DIMQ_F32, mx_pad8(p.cols), p.cols, nullptr, 0, nullptr, 0, 0};
   }
+  const int64_t unit = FP4 ? 8 : 64, stages = (p.len + unit - 1) / unit * p.planes;
   int rc;
   switch (pl.tile) {
     case 0: rc = mx_mm_launch<MxTile<FP4, CT, RT, 4, 2, 2, 4, 2>>(p, pl.splits, s, what); break;
-    case 1: rc = mx_mm_launch<MxTile<FP4, CT, RT, 2, 2, 2, 2, 2>>(p, pl.splits, s, what); break;
+    case 1:
+      if (mx_deep(pl, p.rows, p.cols, stages)) rc = mx_mm_launch<MxTile<FP4, CT, RT, 2, 2, 2, 2, 4>>(p, pl.splits, s, what);
+      else rc = mx_mm_launch<MxTile<FP4, CT, RT, 2, 2, 2, 2, 2>>(p, pl.splits, s, what);
+      break;
     default: rc = mx_mm_launch<MxTile<FP4, CT, RT, 2, 2, 1, 1, 3>>(p, pl.splits, s, what);
   }
   if (rc != DIMQ_OK || pl.splits == 1) return rc;
