@@ -2,11 +2,13 @@
 
 Public API mirrors ``dimq_backend/__init__.py`` of the reference
 (``dimq_cuda_backend/dimq_backend/__init__.py:3-37``), plus the weight-only,
-b-bit, per-channel codebook layers and ops.  The CPU reference functions of
+b-bit, per-channel codebook layers and ops, and microscaled 4-bit layers with
+8-bit activation checkpoints (``mx``).  The CPU reference functions of
 the reference package (``dimq_linear_reference`` ...) are test oracles and
 live in ``oracle/``, not here.
 """
 
+from . import mx
 from .export import (
     activation_qparams_from_minmax,
     assign_weight_indices,
@@ -25,6 +27,7 @@ from .modules import (
     DIMQCodebookLinear,
     DIMQConv2d,
     DIMQLinear,
+    DIMQMXFP4Linear,
     make_packed_layer,
     quantize_model_weight_only,
     replace_modules_with_packed_dimq,
@@ -37,6 +40,7 @@ __all__ = [
     "DIMQCodebookLinear",
     "DIMQConv2d",
     "DIMQLinear",
+    "DIMQMXFP4Linear",
     "activation_qparams_from_minmax",
     "assign_weight_indices",
     "bits_for_codebook",
@@ -50,6 +54,7 @@ __all__ = [
     "is_available",
     "load_activation_qparams",
     "make_packed_layer",
+    "mx",
     "pack_indices",
     "pack_u4_indices",
     "quantize_activation_u4",

@@ -95,7 +95,9 @@ template <int DT>
 __device__ __forceinline__ void sum_part(const PrepArgs& p, uint32_t group, float (&red)[4][8][64]) {
   const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
   const uint32_t slice = group / p.sum_cols;
-  const int64_t n = ((int64_t)(group - slice * p.sum_cols) * 64 + c) * 8, m0 = slice * p.sum_rows;
+  // a last group that is not whole starts earlier: its first columns are its neighbour's, summed alike
+  int64_t n = ((int64_t)(group - slice * p.sum_cols) * 64 + c) * 8, m0 = slice * p.sum_rows;
+  if (n < p.N && n + 8 > p.N && p.N >= 8) n = p.N - 8;
   const int64_t m1 = m0 + p.sum_rows < p.M ? m0 + p.sum_rows : p.M;
   float s[8] = {};
   auto add = [&](int64_t m, int64_t cols) {
@@ -106,7 +108,7 @@ __device__ __forceinline__ void sum_part(const PrepArgs& p, uint32_t group, floa
   };
   if (n < p.N) {
     int64_t m = m0 + w;
-    if (n + 8 <= p.N) {  // eight rows' loads in flight, with no branch between them
+    if (p.N >= 8) {  // eight rows' loads in flight, with no branch between them
       for (; m + 28 < m1; m += 32)
 #pragma unroll
         for (int i = 0; i < 8; ++i) add(m + 4 * i, 8);
@@ -121,8 +123,8 @@ __device__ __forceinline__ void sum_part(const PrepArgs& p, uint32_t group, floa
     float t[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) t[j] = (red[0][j][c] + red[1][j][c]) + (red[2][j][c] + red[3][j][c]);
-    *reinterpret_cast<float4*>(o) = make_float4(t[0], t[1], t[2], t[3]);
-    *reinterpret_cast<float4*>(o + 4) = make_float4(t[4], t[5], t[6], t[7]);
+    mx_write16(o, make_uint4(__float_as_uint(t[0]), __float_as_uint(t[1]), __float_as_uint(t[2]), __float_as_uint(t[3])));
+    mx_write16(o + 4, make_uint4(__float_as_uint(t[4]), __float_as_uint(t[5]), __float_as_uint(t[6]), __float_as_uint(t[7])));
   }
 }
 
@@ -260,10 +262,10 @@ extern "C" int dimq_mx_linear_backward(const void* g, int g_dtype, int64_t M, in
   int rc = mx_check_rows(what, g, g_dtype, M, N, ldg);
   if (rc != DIMQ_OK) return rc;
   DIMQ_CHECK(K > 0 && N > 0, "linear dimensions must be positive");
+  if (M == 0) gx = nullptr;  // no rows: nothing to write
   if (gx && ((rc = check_out(what, gx, gx_dtype)) != DIMQ_OK || (rc = check_codes(what, codes, scales, N)) != DIMQ_OK)) return rc;
   if (gw && ((rc = check_out(what, gw, gw_dtype)) != DIMQ_OK || (rc = check_codes(what, codes8, scales8, M)) != DIMQ_OK)) return rc;
   DIMQ_CHECK(!gb || is_float_dtype(gb_dtype), "bias gradient must be floating point");
-  if (M == 0) gx = nullptr;
   return backward(what, g, g_dtype, M, N, ldg, codes, scales, codes8, scales8, K, gx, gx_dtype, gw, gw_dtype, gb, gb_dtype,
                   workspace, workspace_bytes, as_stream(stream));
 }

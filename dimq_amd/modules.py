@@ -22,7 +22,7 @@ from typing import Any, Iterator, Mapping
 import torch
 import torch.nn as nn
 
-from . import ops
+from . import mx, ops
 from .codebook import assign_indices, init_centers_1d, init_centers_per_channel
 from .export import bits_for_codebook, pack_indices
 
@@ -147,6 +147,35 @@ class DIMQCodebookLinear(nn.Module):
     def from_export_layer(cls, layer: Mapping[str, Any]) -> "DIMQCodebookLinear":
         return cls(layer["packed_weight"], layer["codebook"], layer["bit_w"], layer["out_features"],
                    layer["in_features"], layer.get("bias"), activation_centers=layer.get("activation_centers"))
+
+
+class DIMQMXFP4Linear(nn.Module):
+    """Linear on a microscaled 4-bit weight and input: y = act(Q4(x) @ W^T + b + residual), W the values of the codes
+    (``mx.quantize_mxfp4``: uint8 codes [out_features, 16 * blocks], one scale byte a block of 32)."""
+
+    def __init__(self, codes, scales, in_features, bias=None, *, out_dtype: torch.dtype | None = None) -> None:
+        super().__init__()
+        self.register_buffer("codes", codes.contiguous())
+        self.register_buffer("scales", scales.contiguous())
+        self.register_buffer("bias", None if bias is None else bias.contiguous())
+        self.out_features = int(codes.shape[0])
+        self.in_features = int(in_features)
+        self.out_dtype = out_dtype
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None,
+                activation: str | None = None) -> torch.Tensor:
+        """act(linear(x) + residual); residual and activation ("relu", "gelu") are fused into the kernel."""
+        _require_gpu(x, self.codes, True, "DIMQMXFP4Linear")
+        return mx.mxfp4_linear(x, self.codes, self.scales, self.bias, residual=residual, activation=activation,
+                               out_dtype=self.out_dtype)
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, linear: nn.Linear, *, out_dtype: torch.dtype | None = None) -> "DIMQMXFP4Linear":
+        """The weight of a Linear on the GPU (``mx.MXFP4TrainLinear`` too), packed."""
+        codes, scales = mx.quantize_mxfp4(linear.weight.detach())
+        bias = None if linear.bias is None else linear.bias.detach().clone()
+        return cls(codes, scales, linear.in_features, bias, out_dtype=out_dtype)
 
 
 class DIMQCodebookConv2d(nn.Module):
