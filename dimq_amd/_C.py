@@ -129,6 +129,8 @@ _SIGS = {
     "dimq_mxfp4_linear_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "dimq_mxfp4_linear": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _i64, _vp, _int, _vp, _int, _int, _vp,
                                  _vp, _vp, _i64, _vp]),
+    "dimq_mx_linear_forward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _vp, _int, _i64, _vp, _int, _vp, _vp, _vp,
+                                      _vp, _vp, _i64, _vp]),
     "dimq_mx_linear_backward_workspace_bytes": (_i64, [_vp, _int, _i64, _i64, _i64, _i64, _int]),
     "dimq_mx_linear_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp, _int, _vp, _int,
                                        _vp, _i64, _vp]),

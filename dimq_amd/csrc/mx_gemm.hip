@@ -231,10 +231,10 @@ struct Layout {
   int64_t xc = 0, xs = 0, ws = 0, part = 0, bytes = 0;
   MxPlan plan;
   Layout(int64_t M, int64_t K, int64_t N) {
-    const int64_t b = mx_pad8(mx_blocks(K));
+    const int64_t n = mx_blocks(K), b = mx_pad8(n);
     auto take = [&](int64_t& at, int64_t n) { at = bytes, bytes += (n + 255) / 256 * 256; };
     plan = mx_plan(true, M, N, b / 8);
-    take(xc, M * b * 16);
+    take(xc, M * n * 16);
     take(xs, mx_scale_rows(M) * b);
     take(ws, mx_scale_rows(N) * b);
     take(part, mx_partial_bytes(plan, M, N));
@@ -251,40 +251,91 @@ extern "C" int64_t dimq_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64
   return Layout(M, K, N).bytes;
 }
 
+namespace dimq {
+namespace {
+
+// The layer on packed weights or, where w is given, on weights that are packed into codes and scales on the way.
+struct Layer {
+  const char* what;
+  const void* x;
+  int x_dtype;
+  int64_t M, K, ldx;
+  const void* w;
+  int w_dtype;
+  int64_t ldw;
+  uint8_t *codes, *scales;
+  int64_t N;
+  int8_t* codes8;
+  uint8_t* scales8;
+  MxOut out;
+  void* workspace;
+  int64_t workspace_bytes;
+};
+
+int run(const Layer& a, hipStream_t s) {
+  const char* what = a.what;
+  DIMQ_CHECK(a.M >= 0 && a.K > 0 && a.N > 0, "linear dimensions must be positive");
+  DIMQ_CHECK(a.out.act >= DIMQ_ACT_NONE && a.out.act <= DIMQ_ACT_GELU, "unknown activation %d", a.out.act);
+  DIMQ_CHECK(a.out.dtype == DIMQ_F32 || a.out.dtype == DIMQ_F16 || a.out.dtype == DIMQ_BF16,
+             "output dtype must be fp32, fp16 or bf16");
+  DIMQ_CHECK(!a.out.bias || is_float_dtype(a.out.bias_dtype), "bias must be floating point");
+  DIMQ_CHECK(!a.out.res || is_float_dtype(a.out.res_dtype), "residual must be floating point");
+  int rc = mx_check_rows(what, a.x, a.x_dtype, a.M, a.K, a.ldx);
+  if (rc != DIMQ_OK || (a.M == 0 && !a.w)) return rc;
+  DIMQ_CHECK(a.codes && a.scales, "%s: null pointer", what);
+  DIMQ_CHECK(aligned(a.codes, 16), "%s: codes must be 16-byte aligned", what);
+  if (a.w && (rc = mx_check_rows(what, a.w, a.w_dtype, a.N, a.K, a.ldw)) != DIMQ_OK) return rc;
+  const int64_t blocks = mx_blocks(a.K);
+  if (a.M == 0) return dimq_mx_quantize(a.w, a.w_dtype, a.N, a.K, a.ldw, a.codes, a.scales, blocks, nullptr, nullptr, s);
+  DIMQ_CHECK(a.out.y, "%s: null pointer", what);
+  if (a.codes8) {
+    DIMQ_CHECK(a.scales8, "%s: null pointer", what);
+    DIMQ_CHECK(aligned(a.codes8, 16), "%s: codes must be 16-byte aligned", what);
+  }
+  if (few_rows_pay(a.x_dtype == DIMQ_F32, a.M, a.K, a.N)) {
+    if (a.w) rc = dimq_mx_quantize(a.w, a.w_dtype, a.N, a.K, a.ldw, a.codes, a.scales, blocks, nullptr, nullptr, s);
+    if (rc == DIMQ_OK && a.codes8)
+      rc = dimq_mx_quantize(a.x, a.x_dtype, a.M, a.K, a.ldx, nullptr, nullptr, 0, a.codes8, a.scales8, s);
+    if (rc != DIMQ_OK) return rc;
+    DIMQ_CHECK((a.N + 15) / 16 < (1ll << 31), "%s: too many outputs", what);
+    return few_rows_any(a.x_dtype, {a.x, a.ldx, a.M, a.K, a.codes, a.scales, a.N, blocks,
+                                    blocks % 4 == 0 && aligned(a.scales, 4), a.out}, s);
+  }
+  const Layout at(a.M, a.K, a.N);
+  DIMQ_CHECK(a.workspace && aligned(a.workspace, 256) && a.workspace_bytes >= at.bytes,
+             "%s: the workspace is too small or not 256-byte aligned", what);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  const int64_t xr = mx_scale_rows(a.M), wr = mx_scale_rows(a.N);
+  const MxTiledOperand x{a.x, a.x_dtype, a.M, a.K, a.ldx, ws + at.xc, ws + at.xs, xr, nullptr, a.codes8, a.scales8};
+  if (a.w) {
+    rc = mx_quantize_pair(x, {a.w, a.w_dtype, a.N, a.K, a.ldw, a.codes, ws + at.ws, wr, a.scales, nullptr, nullptr}, s);
+  } else {
+    MxScaleTurn turn;
+    turn.in = a.scales, turn.out = ws + at.ws, turn.n = a.N, turn.blocks = blocks, turn.rows = wr;
+    rc = mx_quantize_tiled(x, turn, s);
+  }
+  if (rc != DIMQ_OK) return rc;
+  const MxMm p{{ws + at.xc, blocks * 16, ws + at.xs, xr}, {a.codes, blocks * 16, ws + at.ws, wr}, a.M, a.N, blocks, 1, 0, 0, a.out};
+  return mx_mm<true, false, false>(p, at.plan, reinterpret_cast<float*>(ws + at.part), s, what);
+}
+
+}  // namespace
+}  // namespace dimq
+
 extern "C" int dimq_mxfp4_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* codes,
                                  const uint8_t* scales, const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype,
                                  const void* residual, int residual_dtype, int activation, int8_t* codes8,
                                  uint8_t* scales8, void* workspace, int64_t workspace_bytes, void* stream) {
-  DIMQ_CHECK(M >= 0 && K > 0 && N > 0, "linear dimensions must be positive");
-  DIMQ_CHECK(activation >= DIMQ_ACT_NONE && activation <= DIMQ_ACT_GELU, "unknown activation %d", activation);
-  DIMQ_CHECK(y_dtype == DIMQ_F32 || y_dtype == DIMQ_F16 || y_dtype == DIMQ_BF16, "output dtype must be fp32, fp16 or bf16");
-  DIMQ_CHECK(!bias || is_float_dtype(bias_dtype), "bias must be floating point");
-  DIMQ_CHECK(!residual || is_float_dtype(residual_dtype), "residual must be floating point");
-  int rc = mx_check_rows("mxfp4_linear", x, x_dtype, M, K, ldx);
-  if (rc != DIMQ_OK || M == 0) return rc;
-  DIMQ_CHECK(codes && scales && y, "mxfp4_linear: null pointer");
-  DIMQ_CHECK(aligned(codes, 16), "mxfp4_linear: codes must be 16-byte aligned");
-  if (codes8) {
-    DIMQ_CHECK(scales8, "mxfp4_linear: null pointer");
-    DIMQ_CHECK(aligned(codes8, 16), "mxfp4_linear: codes must be 16-byte aligned");
-  }
-  const int64_t blocks = mx_blocks(K), pitch = mx_pad8(blocks);
-  hipStream_t s = as_stream(stream);
-  const MxOut out{y, y_dtype, N, N, bias, bias_dtype, residual, residual_dtype, activation};
-  if (few_rows_pay(x_dtype == DIMQ_F32, M, K, N)) {
-    if (codes8 && (rc = dimq_mx_quantize(x, x_dtype, M, K, ldx, nullptr, nullptr, 0, codes8, scales8, stream)) != DIMQ_OK) return rc;
-    DIMQ_CHECK((N + 15) / 16 < (1ll << 31), "mxfp4_linear: too many outputs");
-    return few_rows_any(x_dtype, {x, ldx, M, K, codes, scales, N, blocks, blocks % 4 == 0 && aligned(scales, 4), out}, s);
-  }
-  const Layout at(M, K, N);
-  DIMQ_CHECK(workspace && aligned(workspace, 256) && workspace_bytes >= at.bytes,
-             "mxfp4_linear: the workspace is too small or not 256-byte aligned");
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  MxScaleTurn turn;
-  turn.in = scales, turn.out = ws + at.ws, turn.n = N, turn.blocks = blocks, turn.rows = mx_scale_rows(N);
-  rc = mx_quantize_tiled(x, x_dtype, M, K, ldx, ws + at.xc, ws + at.xs, pitch, mx_scale_rows(M), codes8, scales8, turn, s);
-  if (rc != DIMQ_OK) return rc;
-  const MxMm p{{ws + at.xc, pitch * 16, ws + at.xs, mx_scale_rows(M)}, {codes, blocks * 16, ws + at.ws, mx_scale_rows(N)},
-               M, N, blocks, 1, 0, 0, out};
-  return mx_mm<true, false, false>(p, at.plan, reinterpret_cast<float*>(ws + at.part), s, "mxfp4_linear");
+  return run({"mxfp4_linear", x, x_dtype, M, K, ldx, nullptr, 0, 0, const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales), N,
+              codes8, scales8, MxOut{y, y_dtype, N, N, bias, bias_dtype, residual, residual_dtype, activation}, workspace,
+              workspace_bytes}, as_stream(stream));
+}
+
+extern "C" int dimq_mx_linear_forward(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const void* w, int w_dtype,
+                                      int64_t ldw, const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype,
+                                      uint8_t* codes, uint8_t* scales, int8_t* codes8, uint8_t* scales8, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  DIMQ_CHECK(w, "mx_linear_forward: null pointer");
+  return run({"mx_linear_forward", x, x_dtype, M, K, ldx, w, w_dtype, ldw, codes, scales, N, codes8, scales8,
+              MxOut{y, y_dtype, N, N, bias, bias_dtype, nullptr, 0, 0}, workspace, workspace_bytes}, as_stream(stream));
 }

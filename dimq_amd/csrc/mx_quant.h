@@ -91,10 +91,21 @@ struct MxScaleTurn {
   uint32_t groups = 0;  // work-groups that do it
 };
 
-// x in 4 bits as an operand of the tiled products: codes [rows, blocks, 16] and scales [blocks / 8, scale_rows, 8]
-// (blocks % 8 == 0, zeros past the row), its 8-bit form where codes8 is given, and the other operand's scales turned, in
-// one launch (mx_quant.hip).
-int mx_quantize_tiled(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes, uint8_t* scales,
-                      int64_t blocks, int64_t scale_rows, int8_t* codes8, uint8_t* scales8, MxScaleTurn turn, hipStream_t s);
+// A tensor [rows, cols] to become an operand of the tiled products: codes [rows, blocks, 16] and scales [stages of 8
+// blocks, scale_rows, 8], zeros past the row; its row-major scales and its 8-bit form where those are given.
+struct MxTiledOperand {
+  const void* x;
+  int dtype;
+  int64_t rows, cols, ld;
+  uint8_t *codes, *tiled;
+  int64_t scale_rows;
+  uint8_t* scales;
+  int8_t* codes8;
+  uint8_t* scales8;
+};
+
+// In one launch (mx_quant.hip): x, and packed weights' scales turned; x and weights.
+int mx_quantize_tiled(const MxTiledOperand& x, MxScaleTurn turn, hipStream_t s);
+int mx_quantize_pair(const MxTiledOperand& x, const MxTiledOperand& w, hipStream_t s);
 
 }  // namespace dimq

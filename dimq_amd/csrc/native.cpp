@@ -450,9 +450,8 @@ Tensor decompress_activation(const Tensor& codes, const Tensor& scales, int64_t 
   return mx_dequantize(codes, scales, size, dtype, 8, "decompress_activation");
 }
 
-// c8, s8: where x's 8-bit form goes (undefined: nowhere).
 Tensor mxfp4_linear_into(const Tensor& x, const Codes& w, const OptTensor& bias, const OptTensor& residual, int64_t activation,
-                         at::ScalarType out_dtype, const Tensor& c8, const Tensor& s8) {
+                         at::ScalarType out_dtype) {
   const Rows r(x, "mxfp4_linear", "input");
   TORCH_CHECK(mx_float(out_dtype), "mxfp4_linear: output dtype must be fp32, fp16 or bf16");
   const Bias b(bias, w.rows, "out_features");
@@ -464,7 +463,7 @@ Tensor mxfp4_linear_into(const Tensor& x, const Codes& w, const OptTensor& bias,
   const On on(x);
   const Tensor ws = workspace(dimq_mxfp4_linear_workspace_bytes(r.n, r.cols, w.rows), x);
   check_rc(dimq_mxfp4_linear(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, pu8(w.c), pu8(w.s), b.p, b.dtype, w.rows, ptr(y), dt(y),
-                             res.p, res.dtype, static_cast<int>(activation), pi8(c8), pu8(s8), ptr(ws),
+                             res.p, res.dtype, static_cast<int>(activation), nullptr, nullptr, ptr(ws),
                              ws.defined() ? ws.numel() : 0, on.stream));
   return y;
 }
@@ -474,7 +473,7 @@ Tensor mxfp4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, 
   TORCH_CHECK_NOT_IMPLEMENTED(x.is_cuda(), "mxfp4_linear expects a CUDA input");
   TORCH_CHECK(x.dim() > 0 && codes.dim() == 2, "mxfp4_linear expects an input of at least one dimension and 2-D codes");
   const Codes w(codes, scales, x.size(-1), 4, x, "mxfp4_linear");
-  return mxfp4_linear_into(x, w, bias, residual, activation, out_dtype.value_or(x.scalar_type()), Tensor(), Tensor());
+  return mxfp4_linear_into(x, w, bias, residual, activation, out_dtype.value_or(x.scalar_type()));
 }
 
 Tensor mxfp4_linear_grad_input(const Tensor& grad, const Tensor& codes, const Tensor& scales, int64_t in_features,
@@ -655,40 +654,44 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     TORCH_CHECK(w.device() == x.device(), "mx.linear: the weight must be on ", x.device().str());
     TORCH_CHECK(mx_float(x.scalar_type()), "mx.linear: input must be fp32, fp16 or bf16, not ", dtype_name(x.scalar_type()));
     TORCH_CHECK(!bias || mx_float(bias->scalar_type()), "mx.linear: bias must be fp32, fp16 or bf16");
-    const auto wq = mx_quantize(w, true, false, "mx.linear");
-    const Codes wc(wq[0], wq[1], w.size(1), 4, x, "mx.linear");
-    std::pair<Tensor, Tensor> x8;
-    if (w.requires_grad()) x8 = new_codes(x.sizes(), 8, x);
-    const Tensor y = mxfp4_linear_into(x.detach(), wc, bias ? OptTensor(bias->detach()) : bias, std::nullopt, 0,
-                                       x.scalar_type(), x8.first, x8.second);
-    const bool need_w = x.requires_grad();
-    ctx->save_for_backward({need_w ? wq[0] : Tensor(), need_w ? wq[1] : Tensor(), x8.first, x8.second});
-    ctx->saved_data["k"] = w.size(1);
-    ctx->saved_data["wdt"] = static_cast<int64_t>(w.scalar_type());
-    ctx->saved_data["b"] = static_cast<bool>(bias && bias->requires_grad());
-    ctx->saved_data["bdt"] = static_cast<int64_t>(bias ? bias->scalar_type() : at::kFloat);
+    const Rows r(x, "mx.linear", "input"), wr(w, "mx.linear", "weight");
+    const Bias b(bias, wr.n, "out_features");
+    TORCH_CHECK(!b.t.defined() || b.t.device() == x.device(), "mx.linear: the bias must be on ", x.device().str());
+    const int64_t N = w.size(0), K = w.size(1), nb = mx_blocks(K);
+    const bool to_w = w.requires_grad();
+    // codes, then scales: one allocation each
+    const auto bytes = x.options().dtype(at::kByte);
+    const Tensor wq = at::empty({N * nb * 17}, bytes), xq = to_w ? at::empty({r.n * nb * 33}, bytes) : Tensor();
+    const Tensor y = at::empty(out_shape(x, N), x.options());
+    const On on(x);
+    const Tensor ws = workspace(dimq_mxfp4_linear_workspace_bytes(r.n, K, N), x);
+    check_rc(dimq_mx_linear_forward(ptr(r.t), dt(r.t), r.n, K, r.ld, ptr(wr.t), dt(wr.t), wr.ld, b.p, b.dtype, N, ptr(y), dt(y),
+                                    pu8(wq), pu8(wq) + N * nb * 16, pi8(xq),
+                                    to_w ? pu8(xq) + r.n * nb * 32 : nullptr, ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
+    ctx->save_for_backward({x.requires_grad() ? wq : Tensor(), xq});
+    ctx->saved_data["layer"] = std::vector<int64_t>{N, K, static_cast<int64_t>(w.scalar_type()), bias && bias->requires_grad(),
+                                                    static_cast<int64_t>(bias ? bias->scalar_type() : at::kFloat)};
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("mx.linear");
     const auto saved = ctx->get_saved_variables();
-    const Tensor& g = grads[0];
-    const int64_t K = ctx->saved_data["k"].toInt();
-    const bool b = ctx->saved_data["b"].toBool();
-    const auto bdt = static_cast<at::ScalarType>(ctx->saved_data["bdt"].toInt());
-    const char* op = "mx.linear";
-    const Rows r(g, op, "gradient");
+    const Tensor &g = grads[0], &wq = saved[0], &xq = saved[1];
+    const auto layer = ctx->saved_data["layer"].toIntVector();
+    const int64_t N = layer[0], K = layer[1], nb = mx_blocks(K);
+    const bool b = layer[3];
+    const Rows r(g, "mx.linear", "gradient");
     Tensor gx, gw, gb;
-    if (saved[0].defined()) gx = at::empty(out_shape(g, K), g.options());
-    if (saved[2].defined())
-      gw = at::empty({r.cols, K}, g.options().dtype(static_cast<at::ScalarType>(ctx->saved_data["wdt"].toInt())));
-    if (b) gb = at::empty({r.cols}, g.options().dtype(bdt));
+    if (wq.defined()) gx = at::empty(out_shape(g, K), g.options());
+    if (xq.defined()) gw = at::empty({N, K}, g.options().dtype(static_cast<at::ScalarType>(layer[2])));
+    if (b) gb = at::empty({N}, g.options().dtype(static_cast<at::ScalarType>(layer[4])));
     const On on(g);
-    const Tensor ws = workspace(dimq_mx_linear_backward_workspace_bytes(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, K,
+    const Tensor ws = workspace(dimq_mx_linear_backward_workspace_bytes(ptr(r.t), dt(r.t), r.n, N, r.ld, K,
                                                                         gx.defined() + 2 * gw.defined() + 4 * b), g);
-    check_rc(dimq_mx_linear_backward(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, pu8(saved[0]), pu8(saved[1]), pi8(saved[2]),
-                                     pu8(saved[3]), K, ptr(gx), gx.defined() ? dt(gx) : 0, ptr(gw), gw.defined() ? dt(gw) : 0,
-                                     ptr(gb), b ? dt(gb) : 0, ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
+    check_rc(dimq_mx_linear_backward(ptr(r.t), dt(r.t), r.n, N, r.ld, pu8(wq), wq.defined() ? pu8(wq) + N * nb * 16 : nullptr,
+                                     pi8(xq), xq.defined() ? pu8(xq) + r.n * nb * 32 : nullptr, K, ptr(gx),
+                                     gx.defined() ? dt(gx) : 0, ptr(gw), gw.defined() ? dt(gw) : 0, ptr(gb), b ? dt(gb) : 0,
+                                     ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
     return {gx, gw, gb};
   }
 };

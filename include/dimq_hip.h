@@ -571,6 +571,15 @@ int dimq_mxfp4_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t 
                       const void* residual, int residual_dtype, int activation, int8_t* codes8, uint8_t* scales8,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
+/* A training step's forward pass: the weights w [N, K] (row stride ldw) packed
+ * into codes [N, ceil(K / 32), 16] and scales [N, ceil(K / 32)], which the
+ * backward pass reads, x's 8-bit form (nullable pair), and y = Q4(x) Q4(w)^T +
+ * bias.  Workspace as dimq_mxfp4_linear's. */
+int dimq_mx_linear_forward(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const void* w, int w_dtype,
+                           int64_t ldw, const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype, uint8_t* codes,
+                           uint8_t* scales, int8_t* codes8, uint8_t* scales8, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
 /* Straight-through gradients of that layer for the upstream g [M, N]:
  *   gx = g W             (W from its 4-bit codes)
  *   gw = g^T Q8(x)       (x from its 8-bit checkpoint), gb = sum of g over m
