@@ -41,7 +41,7 @@ struct MxOut {
 struct MxOperand {
   const uint8_t* p;
   int64_t ld;              // bytes between rows (plain: of the output index; turned: of the reduction index)
-  const uint8_t* scales;   // FP4: [stages, scale_rows, 8] bytes, scale_rows a multiple of 256 (mx_scale_rows)
+  const uint8_t* scales;   // FP4: [stages, scale_rows, 8] bytes, as many rows as whole tiles read (mx_scale_rows)
   int64_t scale_rows;
 };
 
@@ -188,10 +188,10 @@ struct MxTile {
 // the 256 bytes that the banks span.
 __device__ __forceinline__ int mx_swz(int r) { return (r >> 1) & 7; }
 // Turned (rows of `pitch` bytes, one reduction index each): a transposing read takes 64 bytes of each of 4 consecutive
-// rows; they lie in 4 quarters of the 256 bytes (of a 128-byte pitch: in the halves of two rows).
+// rows; they lie in 4 quarters of the 256 bytes (of a 128- or 384-byte pitch: in the halves of two rows).
 template <int PITCH>
 __device__ __forceinline__ int mx_swz_turned(int k) {
-  return PITCH >= 256 ? 4 * (k & 3) : 4 * ((k >> 1) & 1);
+  return PITCH % 256 == 0 ? 4 * (k & 3) : 4 * ((k >> 1) & 1);
 }
 
 template <class T>
@@ -447,7 +447,10 @@ __global__ __launch_bounds__(T::NT) void mx_mm_kernel(const MxMm p) {
   if (gridDim.y > 1) o.y = static_cast<float*>(o.y) + blockIdx.y * p.partial;
   float* park = reinterpret_cast<float*>(sm) + wave * 32 * CB * 32;
   constexpr int LPR = CB * 4, RPI = 64 / LPR;  // lanes a row, rows a pass
-  auto place = [&](int row, int chunk) MX_INLINE { return row * CB * 32 + ((chunk ^ (CB >= 2 ? row & 15 : (row >> 1) & 7)) << 2); };
+  // chunks of four values; a lane writes one of each of 16 rows: over the 256 bytes that the banks span
+  auto place = [&](int row, int chunk) MX_INLINE {
+    return row * CB * 32 + ((chunk ^ (CB == 1 ? (row >> 1) & 7 : CB % 2 == 0 ? row & 15 : row & 7)) << 2);
+  };
   const int qc = lane % LPR;
   const int64_t n = c0 + wc * CB * 32 + qc * 8;
   float bias[8] = {};
@@ -462,8 +465,9 @@ __global__ __launch_bounds__(T::NT) void mx_mm_kernel(const MxMm p) {
             make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll 4
-    for (int u = 0; u < 32 / RPI; ++u) {
+    for (int u = 0; u < (32 + RPI - 1) / RPI; ++u) {
       const int row = u * RPI + lane / LPR;
+      if (64 % LPR != 0 && (lane >= RPI * LPR || row >= 32)) continue;
       const float4 a = *reinterpret_cast<const float4*>(park + place(row, 2 * qc));
       const float4 b = *reinterpret_cast<const float4*>(park + place(row, 2 * qc + 1));
       float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -494,17 +498,21 @@ static __global__ __launch_bounds__(256) void mx_reduce_kernel(const float* part
   mx_store8<false>(o, m, n, v, bias);
 }
 
-// How a product is cut: the tile (0: 256 x 256, 1: 128 x 128, 2: 64 x 64) and the slices of its reduction.
+// How a product is cut: the tile (0: 256 x 256, 1: 128 x 128, 2: 64 x 64, 3: 256 x 192) and the slices of its reduction.
 struct MxPlan {
   int tile, splits;
   double us;  // estimated
 };
 
 inline int64_t mx_pad8(int64_t n) { return (n + 7) / 8 * 8; }
-inline int64_t mx_scale_rows(int64_t n) { return (n + 255) / 256 * 256; }
+// Rows of scales that whole tiles of any size read.
+inline int64_t mx_scale_rows(int64_t n) {
+  const int64_t a = (n + 255) / 256 * 256, b = (n + 191) / 192 * 192;
+  return a > b ? a : b;
+}
 inline int64_t mx_tiles(int tile, int64_t rows, int64_t cols) {
-  const int64_t t = 256 >> tile;
-  return ((rows + t - 1) / t) * ((cols + t - 1) / t);
+  const int64_t r = tile == 3 ? 256 : 256 >> tile, c = tile == 3 ? 192 : 256 >> tile;
+  return ((rows + r - 1) / r) * ((cols + c - 1) / c);
 }
 inline int64_t mx_partial_bytes(const MxPlan& pl, int64_t rows, int64_t cols) {
   return pl.splits > 1 ? pl.splits * rows * mx_pad8(cols) * 4 : 0;
@@ -517,22 +525,23 @@ inline bool mx_deep(const MxPlan& pl, int64_t rows, int64_t cols, int64_t stages
   return mx_tiles(1, rows, cols) * pl.splits <= 256 && stages >= 24 * pl.splits;
 }
 
-// The plan of the least estimated time.  A tile's stage takes, in us on a card of 256 CUs, the larger of its latency (a
-// CU's only work-group) and its share where n of them run on a CU; a tile adds its filling and epilogue; slices add a
-// launch and their bytes at 5 TB/s.  Measured on products of 16 to 16,384 rows (bf16 ones: both gradients): a stage of
-// the 256 tile 1.3 us on part of the card and 1.65 (FP4: 2.0) on all of it, of the 128 tile 0.60 / 0.465 n (FP4: 0.73 /
-// 0.60 n; 0.42 and 0.55 with the deeper ring), of the 64 tile 0.24 / 0.20 n (FP4: 0.41 / 0.25 n).  On
-// 171 products, each with 5 to 20 plans measured, the estimate's choice is 1.6 % slower than the best one in the mean.
+// The plan of the least estimated time, in us on a card of 256 CUs.  A stage of the two large tiles, one work-group a CU,
+// takes a + b times the share of the CUs at work (the clock falls as more of them do); one of the small tiles the larger
+// of its latency and its share where n run on a CU.  A tile adds its filling and epilogue; slices add a launch and their
+// bytes at 5 TB/s.  Measured on products of 16 to 16,384 rows, bf16 ones in both gradients; over 146 products with 4 to 25
+// plans measured each, the choice is 0.5 % slower than the best one in the mean, 20 % at worst (64 rows summed).
 inline MxPlan mx_plan(bool fp4, int64_t rows, int64_t cols, int64_t stages) {
   MxPlan best{2, 1, 1e300};
-  for (int tile = 0; tile < 3; ++tile) {
+  for (int tile = 0; tile < 4; ++tile) {
     for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (splits > 1 && stages < 4 * splits) break;
       const int64_t groups = mx_tiles(tile, rows, cols) * splits, n = (groups + 255) / 256;
-      const double each = (double)((stages + splits - 1) / splits);
+      const double each = (double)((stages + splits - 1) / splits), busy = groups < 256 ? groups / 256.0 : 1.0;
       double us;
       if (tile == 0) {
-        us = n * (each * (groups < 192 ? 1.3 : fp4 ? 2.0 : 1.65) + 6.0);
+        us = n * (each * (fp4 ? 1.0 + 1.0 * busy : 0.9 + 0.75 * busy) + 8.0);
+      } else if (tile == 3) {
+        us = n * (each * (fp4 ? 0.85 + 0.8 * busy : 0.7 + 0.62 * busy) + 7.0);
       } else {
         const bool deep = tile == 1 && mx_deep({1, splits, 0}, rows, cols, stages);
         const double alone = deep ? (fp4 ? 0.55 : 0.42) : tile == 1 ? (fp4 ? 0.73 : 0.60) : (fp4 ? 0.41 : 0.24);
@@ -568,6 +577,7 @@ int mx_mm(MxMm p, const MxPlan& pl, float* partial, hipStream_t s, const char* w
   int rc;
   switch (pl.tile) {
     case 0: rc = mx_mm_launch<MxTile<FP4, CT, RT, 4, 2, 2, 4, 2>>(p, pl.splits, s, what); break;
+    case 3: rc = mx_mm_launch<MxTile<FP4, CT, RT, 4, 2, 2, 3, 2>>(p, pl.splits, s, what); break;
     case 1:
       if (mx_deep(pl, p.rows, p.cols, stages)) rc = mx_mm_launch<MxTile<FP4, CT, RT, 2, 2, 2, 2, 4>>(p, pl.splits, s, what);
       else rc = mx_mm_launch<MxTile<FP4, CT, RT, 2, 2, 2, 2, 2>>(p, pl.splits, s, what);

@@ -25,8 +25,9 @@ def _mm(a, b):
     return (a.cuda().contiguous() @ b.cuda().contiguous()).cpu()
 
 
-# 256 x 256 tiles: outputs of several hundred of them; 128 x 128; 64 x 64, the last two rows with slices of a long reduction
-@pytest.mark.parametrize("M,K,N,dt", [(6000, 96, 1288, BF16), (4100, 1100, 2050, F32), (4097, 2080, 2049, F16),
+# 256 x 256 and 256 x 192 tiles; 128 x 128; 64 x 64, the last two with slices of a long reduction
+@pytest.mark.parametrize("M,K,N,dt", [(3000, 140, 4100, F16), (12608, 72, 1032, F32), (6000, 96, 1288, BF16),
+                                      (4100, 1100, 2050, F32), (4097, 2080, 2049, F16),
                                       (1500, 300, 2050, BF16), (3000, 1056, 1025, F32), (1030, 2560, 2050, F16),
                                       (257, 4128, 770, BF16), (100, 8200, 130, BF16), (40, 16416, 65, F32)])
 def test_linear(gpu, M, K, N, dt):
@@ -47,7 +48,8 @@ def test_linear(gpu, M, K, N, dt):
 
 GRADS = [(6000, 2080, 2050, BF16), (1500, 2080, 2056, F32), (4100, 1000, 2050, F16), (4100, 2080, 40, BF16),
          (2049, 1056, 2056, BF16), (1030, 1000, 1025, F32), (6000, 544, 40, F16), (4096, 1056, 1032, BF16),
-         (17, 96, 2056, BF16), (3000, 96, 40, F16), (64, 40, 5000, F32), (8200, 72, 136, BF16)]
+         (17, 96, 2056, BF16), (3000, 96, 40, F16), (64, 40, 5000, F32), (8200, 72, 136, BF16),
+         (515, 4128, 4096, BF16), (130, 4128, 2056, F32), (2049, 1000, 4104, F16), (4100, 1000, 4104, BF16)]
 
 
 @pytest.mark.parametrize("M,K,N,dt", GRADS)
