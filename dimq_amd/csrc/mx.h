@@ -58,62 +58,87 @@ __device__ __forceinline__ uint32_t mx_codes4(const float (&v)[8], float scale) 
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], scale, 3);
 }
 
-// Phi(-a) exp(a^2 / 2), 0 <= a, as t P(t) with t = 1 / (1 + k a): P by weighted least squares on Chebyshev nodes of t
-// over a <= 14 with P(1) = 1/2, the weights moved towards equal relative errors, and so exact at a = 0, the value of most
-// zeros of a quantized block.  FINE (fp32 outputs): 8 coefficients, 5e-7 as evaluated in fp32; otherwise 7, 1.2e-6.
-template <bool FINE>
-__device__ __forceinline__ float mx_tail_factor(float a) {
-  if constexpr (FINE) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.2333452377915607f, a, 1.0f));
-    float r = -0.067649900913238525f;
-    r = fmaf(r, t, 0.23002518713474274f);
-    r = fmaf(r, t, -0.17541733384132385f);
-    r = fmaf(r, t, 0.2041075974702835f);
-    r = fmaf(r, t, 0.023684635758399963f);
-    r = fmaf(r, t, 0.10058960318565369f);
-    r = fmaf(r, t, 0.091481544077396393f);
-    r = fmaf(r, t, 0.09317866712808609f);
+// GELU and its slope for outputs of type DT.  With a = |h|:
+//
+//   h Phi(h)              = max(h, 0) - a Phi(-a)
+//   d gelu / dh = Phi(h) + h phi(h),  Phi(h) = Phi(-a) or 1 - Phi(-a)
+//
+// which keep the negative tail's relative error where 1 + erf would cancel.  Phi(-a) exp(a^2 / 2) is t P(t) with
+// t = 1 / (1 + k a): P by weighted least squares on Chebyshev nodes of t over a <= 14 with P(1) = 1/2, the weights moved
+// towards equal relative errors, and so exact at a = 0, the value of most zeros of a quantized block.  As evaluated in
+// fp32: 8 coefficients for fp32 outputs 5e-7, 7 for fp16 1.2e-6, 6 for bf16 5.9e-6.  a comes as 64ths and stops at 64 (by
+// the multiplication's own clamp), where the tail is 0: infinity times 0.
+__device__ __forceinline__ float mx_64ths(float h) { return __builtin_amdgcn_fmed3f(fabsf(h) * 0.015625f, 0.0f, 1.0f); }
+
+// SCALE: a power of two that the coefficients take along.
+template <int DT, int SCALE = 1>
+__device__ __forceinline__ float mx_tail_factor(float b) {
+  if constexpr (DT == DIMQ_F32) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(64 * 0.2333452377915607f, b, 1.0f));
+    float r = SCALE * -0.067649900913238525f;
+    r = fmaf(r, t, SCALE * 0.23002518713474274f);
+    r = fmaf(r, t, SCALE * -0.17541733384132385f);
+    r = fmaf(r, t, SCALE * 0.2041075974702835f);
+    r = fmaf(r, t, SCALE * 0.023684635758399963f);
+    r = fmaf(r, t, SCALE * 0.10058960318565369f);
+    r = fmaf(r, t, SCALE * 0.091481544077396393f);
+    r = fmaf(r, t, SCALE * 0.09317866712808609f);
+    return r * t;
+  } else if constexpr (DT == DIMQ_F16) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(64 * 0.36f, b, 1.0f));
+    float r = SCALE * 0.04709881659085434f;
+    r = fmaf(r, t, SCALE * -0.17988737532749394f);
+    r = fmaf(r, t, SCALE * 0.18109358442700213f);
+    r = fmaf(r, t, SCALE * 0.02646958676291894f);
+    r = fmaf(r, t, SCALE * 0.13974328500731586f);
+    r = fmaf(r, t, SCALE * 0.14176884610587542f);
+    r = fmaf(r, t, SCALE * 0.14371325643352723f);
+    return r * t;
+  } else {
+    const float t = __builtin_amdgcn_rcpf(fmaf(64 * 0.31f, b, 1.0f));
+    float r = SCALE * -0.0733089938090878f;
+    r = fmaf(r, t, SCALE * 0.17872215085737886f);
+    r = fmaf(r, t, SCALE * 0.017563094188134135f);
+    r = fmaf(r, t, SCALE * 0.13253454642465368f);
+    r = fmaf(r, t, SCALE * 0.1206456834055663f);
+    r = fmaf(r, t, SCALE * 0.12384351893335482f);
     return r * t;
   }
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.36f, a, 1.0f));
-  float r = 0.04709881659085434f;
-  r = fmaf(r, t, -0.17988737532749394f);
-  r = fmaf(r, t, 0.18109358442700213f);
-  r = fmaf(r, t, 0.02646958676291894f);
-  r = fmaf(r, t, 0.13974328500731586f);
-  r = fmaf(r, t, 0.14176884610587542f);
-  r = fmaf(r, t, 0.14371325643352723f);
-  return r * t;
 }
 
-// exp(-a^2 / 4).  Products take it twice, so that they reach the subnormal numbers, which the exponential itself flushes.
-// FINE: the argument's roundings, 2^-24 of up to 150, are carried along and applied to first order.
-template <bool FINE>
-__device__ __forceinline__ float mx_exp_quarter(float a) {
+// exp(-a^2 / 4), b = a / 64.  Products take it twice, so that they reach the subnormal numbers, which the exponential itself
+// flushes.  For fp32 outputs the argument's roundings, 2^-24 of up to 150, are carried along and applied to first order;
+// otherwise the tail is 1.5e-5 off where it is 1e-37.
+template <int DT>
+__device__ __forceinline__ float mx_exp_quarter(float b) {
   constexpr float kC = -0.36067376022224085f;  // -log2(e) / 4
-  if constexpr (!FINE) return __builtin_amdgcn_exp2f(a * a * kC);
+  if constexpr (DT != DIMQ_F32) return __builtin_amdgcn_exp2f(b * b * (4096 * kC));
   constexpr float kLow = (float)(-0.36067376022224085187998 - (double)kC);
-  const float q = a * a, t = q * kC;
+  const float a = b * 64, q = a * a, t = q * kC;
   const float low = fmaf(q, kLow, fmaf(fmaf(a, a, -q), kC, fmaf(q, kC, -t)));
   const float e = __builtin_amdgcn_exp2f(t);
   return fmaf(e, low * 0.69314718055994531f, e);
 }
 
-// h Phi(h) = max(h, 0) - a Phi(-a), a = |h|, which keeps the negative tail's relative error (1e-6; not FINE, for outputs of
-// 16 bits: 1.5e-5 where the tail is 1e-37) where 1 + erf would cancel.  a stops at 40, where the tail is 0: infinity times 0.
-template <bool FINE>
+template <int DT>
 __device__ __forceinline__ float mx_gelu(float h) {
-  const float a = fminf(fabsf(h), 40.0f), m = mx_tail_factor<FINE>(a);
-  const float root = mx_exp_quarter<FINE>(a);
-  return fmaf(-(a * m * root), root, 0.5f * (h + fabsf(h)));  // the last sum keeps NaN
+  const float b = mx_64ths(h), m = mx_tail_factor<DT, -64>(b), root = mx_exp_quarter<DT>(b);
+  const float top = 0.5f * (h + fabsf(h));  // max(h, 0) that keeps NaN
+  return fmaf(b * m * root, root, top);
 }
 
-// d gelu / dh = Phi(h) + h phi(h)
-template <bool FINE>
+template <int DT>
 __device__ __forceinline__ float mx_gelu_slope(float h) {
-  const float a = fminf(fabsf(h), 40.0f), m = mx_tail_factor<FINE>(a), c = h * 0.39894228040143268f;
-  const float root = mx_exp_quarter<FINE>(a), tail = m * root * root;
-  return fmaf(c * root, root, h < 0.0f ? tail : 1.0f - tail);
+  const float b = mx_64ths(h), m = mx_tail_factor<DT>(b), c = h * 0.39894228040143268f;
+  float tail, density;
+  if constexpr (DT == DIMQ_F32) {
+    const float root = mx_exp_quarter<DT>(b);
+    tail = m * root * root, density = c * root * root;
+  } else {
+    const float e = __builtin_amdgcn_exp2f(b * b * (4096 * -0.72134752044448170f));  // flushed below 2^-126
+    tail = m * e, density = c * e;
+  }
+  return density + (h < 0.0f ? tail : 1.0f - tail);
 }
 
 }  // namespace dimq

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(512) void mx4_few_rows(const FewArgs p) {
   for (int j = 0; j < 4; ++j) {
     float t = acc[j] + bias[j] + res[j];
     if (p.out.act == DIMQ_ACT_RELU) t = t < 0.0f ? 0.0f : t;
-    if (p.out.act == DIMQ_ACT_GELU) t = mx_gelu<true>(t);
+    if (p.out.act == DIMQ_ACT_GELU) t = mx_gelu<DIMQ_F32>(t);
     if (j < left) store_from_float(p.out.y, p.out.dtype, r * p.out.ld + n4 + j, t);
   }
 }

@@ -129,7 +129,7 @@ __device__ __forceinline__ void mx_store8(const MxOut& o, int64_t m, int64_t n, 
     for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // NaN passes
   } else if (o.act == DIMQ_ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = mx_gelu<true>(v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = mx_gelu<DIMQ_F32>(v[j]);
   }
   if (left == 8) {
     if (o.dtype == DIMQ_F32) {

@@ -108,7 +108,7 @@ __device__ __forceinline__ void quant_unit(const QuantArgs& a, const FastDiv& di
   if constexpr (GELU) {
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = mx_gelu<XT == DIMQ_F32>(v[j]);
+    for (int j = 0; j < 8; ++j) y[j] = mx_gelu<XT>(v[j]);
     mx_store_row8<XT>(a.y, row * a.cols, c, a.cols, y);
   }
 }
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void mx_back_kernel(BackArgs a, FastDiv div, u
     float g[8];
     mx_load_row8<YT>(a.g, row * a.ldg, c, a.cols, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = g[j] * mx_gelu_slope<YT == DIMQ_F32>(v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = g[j] * mx_gelu_slope<YT>(v[j]);
   }
   mx_store_row8<YT>(a.y, row * a.cols, c, a.cols, v);
 }
