@@ -1,6 +1,6 @@
 // y = act(Q4(x) W^T + bias + residual) on 4-bit microscaled weights (mx.h).  Two routes:
 //
-//   few rows    one launch: each work-group quantizes x on the way to its 16 outputs, its waves share the reduction
+//   few rows    one launch: each work-group quantizes 16 rows of x on the way to 16 outputs, its waves share the reduction
 //   otherwise   x is quantized into the workspace, then the tiled product (mx_mm.h) runs on both operands' codes
 //
 // Both run on the scaled matrix instructions, whose operand of 32 codes a lane is one block and takes that block's scale.
@@ -102,8 +102,10 @@ __device__ __forceinline__ void quantize_block(const RawBlock<XT>& x, uint4& cod
       uint32_t q = 0;
       mx_each<4>([&](auto jc) {
         constexpr int j = decltype(jc)::value;
-        if constexpr (XT == DIMQ_BF16) q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, w[4 * i + j]), s, j);
-        else q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(f16x2, w[4 * i + j]), s, j);
+        if constexpr (XT == DIMQ_BF16)
+          q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, w[4 * i + j]), s, j);
+        else
+          q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(f16x2, w[4 * i + j]), s, j);
       });
       o[i] = q;
     }
@@ -113,7 +115,7 @@ __device__ __forceinline__ void quantize_block(const RawBlock<XT>& x, uint4& cod
 
 // A turn of a wave: 16 blocks from b0, lane l the blocks b0 + 4 (l / 16) .. + 3 for row l % 16 of either operand.
 template <int XT, int BOUND>
-__device__ __forceinline__ void few_rows_turn(const FewArgs& p, const uint8_t* wrow, const uint8_t* srow, int64_t xat, int r,
+__device__ __forceinline__ void few_rows_turn(const FewArgs& p, const uint8_t* wrow, const uint8_t* srow, int64_t xat, bool row,
                                               int64_t b, f32x4& acc) {
   constexpr bool whole = BOUND == kWhole;
   uint4 w[4];
@@ -127,7 +129,7 @@ __device__ __forceinline__ void few_rows_turn(const FewArgs& p, const uint8_t* w
     for (int s = 0; s < 4; ++s) ws |= (uint32_t)srow[whole || b + s < p.blocks ? b + s : 0] << (8 * s);
   }
   RawBlock<XT> raw[4] = {};
-  if (r < p.M) {  // rows that are not there cost no loads
+  if (row) {  // rows that are not there cost no loads
 #pragma unroll
     for (int s = 0; s < 4; ++s) load_block<XT, BOUND>(p.x, xat, (b + s) * 32, p.K, raw[s]);
   }
@@ -154,7 +156,7 @@ __device__ __forceinline__ void few_rows_turn(const FewArgs& p, const uint8_t* w
   });
 }
 
-// Up to 16 rows.  A work-group owns 16 outputs; its waves take the reduction in turns of 16 blocks: 64 contiguous bytes of
+// A work-group owns 16 outputs of 16 rows; its waves take the reduction in turns of 16 blocks: 64 contiguous bytes of
 // codes and one dword of scales a lane, whose bytes the four instructions select.  Bound by latency: with 8 waves a
 // work-group the 8.4 MB of a 4096 x 4096 layer are requested by the first turn of 256 work-groups, 5.5 us for one row; with
 // 16 rows, 7.8 us, also by the reads and the quantization of x, which every work-group does for itself (a launch of its own
@@ -168,35 +170,37 @@ __global__ __launch_bounds__(512) void mx4_few_rows(const FewArgs p) {
   const int64_t n = n0 + r < p.N ? n0 + r : p.N - 1;
   const uint8_t* wrow = p.codes + n * p.blocks * 16;
   const uint8_t* srow = p.scales + n * p.blocks;
-  const int64_t xat = (r < p.M ? r : 0) * p.ldx;
+  const int64_t m = (int64_t)blockIdx.y * 16 + r;
+  const bool row = m < p.M;
+  const int64_t xat = (row ? m : 0) * p.ldx;
   f32x4 acc = {};
   for (int64_t b0 = wave * 16; b0 < p.blocks; b0 += waves * 16) {
     const int64_t b = b0 + 4 * g;
-    if ((b0 + 16) * 32 <= p.K) few_rows_turn<XT, kWhole>(p, wrow, srow, xat, r, b, acc);
-    else if (p.K % 8 == 0) few_rows_turn<XT, kGroups>(p, wrow, srow, xat, r, b, acc);
-    else few_rows_turn<XT, kAny>(p, wrow, srow, xat, r, b, acc);
+    if ((b0 + 16) * 32 <= p.K) few_rows_turn<XT, kWhole>(p, wrow, srow, xat, row, b, acc);
+    else if (p.K % 8 == 0) few_rows_turn<XT, kGroups>(p, wrow, srow, xat, row, b, acc);
+    else few_rows_turn<XT, kAny>(p, wrow, srow, xat, row, b, acc);
   }
-  // the first wave adds up and stores: lane l the outputs n0 + 4 (l / 16) .. + 3 of row l % 16
+  // the first wave adds up and stores: lane l the outputs n0 + 4 (l / 16) .. + 3 of row m
   const int64_t n4 = n0 + g * 4;
   const int left = p.N - n4 < 4 ? (int)(p.N - n4) : 4;
   float bias[4] = {}, res[4] = {};
-  if (wave == 0 && r < p.M) {
+  if (wave == 0 && row) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (p.out.bias && j < left) bias[j] = load_as_float(p.out.bias, p.out.bias_dtype, n4 + j);
-      if (p.out.res && j < left) res[j] = load_as_float(p.out.res, p.out.res_dtype, r * p.out.ld + n4 + j);
+      if (p.out.res && j < left) res[j] = load_as_float(p.out.res, p.out.res_dtype, m * p.out.ld + n4 + j);
     }
   }
   red[wave * 64 + lane] = acc;
   __syncthreads();
-  if (wave != 0 || r >= p.M) return;
+  if (wave != 0 || !row) return;
   for (int w = 1; w < waves; ++w) acc += red[w * 64 + lane];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float t = acc[j] + bias[j] + res[j];
     if (p.out.act == DIMQ_ACT_RELU) t = t < 0.0f ? 0.0f : t;
     if (p.out.act == DIMQ_ACT_GELU) t = mx_gelu<DIMQ_F32>(t);
-    if (j < left) store_from_float(p.out.y, p.out.dtype, r * p.out.ld + n4 + j, t);
+    if (j < left) store_from_float(p.out.y, p.out.dtype, m * p.out.ld + n4 + j, t);
   }
 }
 
@@ -205,7 +209,7 @@ void few_rows(const FewArgs& p, hipStream_t s) {
   const int64_t turns = (p.blocks + 15) / 16;
   int waves = 1;
   while (waves < 8 && waves < turns) waves *= 2;
-  mx4_few_rows<XT><<<dim3((unsigned)((p.N + 15) / 16)), 64 * waves, 0, s>>>(p);
+  mx4_few_rows<XT><<<dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 15) / 16)), 64 * waves, 0, s>>>(p);
 }
 
 int few_rows_any(int x_dtype, const FewArgs& p, hipStream_t s) {
@@ -219,12 +223,13 @@ int few_rows_any(int x_dtype, const FewArgs& p, hipStream_t s) {
 
 // Whether the one launch is the faster route.  It takes 3.6 us and, for each 4,096 of K and each work-group of a CU, 2.3 us
 // and 0.17 a row (fp32 x: 4.0, 2.8 and 0.31); the other route 5 us for its launches and the tiled product.  Measured with
-// 16-bit x, one launch / other route: 768 -> 768 with 16 rows 4.9 us / 6.8; 4096 -> 4096 with 1 row 5.9, with 16 8.4 / 11.3;
-// 8192 -> 8192 with 1 row 14.3 / 16.3, with 16 24.4 / 16.7.
+// 16-bit x up to 256 rows, one launch / other route: 768 -> 768 with 64 rows 5.0 us / 7.3, with 256 7.5 / 7.6; 768 -> 2304 with
+// 96 8.5 / 7.4; 4096 -> 4096 with 16 8.4 / 11.3, with 32 13.9 / 12.0; 8192 -> 8192 with 1 14.3 / 16.3, with 16 24.4 / 16.7.
 bool few_rows_pay(bool f32, int64_t M, int64_t K, int64_t N) {
-  if (M > 16) return false;
-  const double units = K / 4096.0 * (double)((N + 4095) / 4096);
-  const double us = f32 ? 4.0 + units * (2.8 + 0.31 * M) : 3.6 + units * (2.3 + 0.17 * M);
+  if (M > 256) return false;
+  const int64_t groups = (N + 15) / 16 * ((M + 15) / 16), rows = M < 16 ? M : 16;
+  const double units = K / 4096.0 * (double)((groups + 255) / 256);
+  const double us = f32 ? 4.0 + units * (2.8 + 0.31 * rows) : 3.6 + units * (2.3 + 0.17 * rows);
   return us <= 5.0 + mx_plan(true, M, N, (mx_blocks(K) + 7) / 8).us;
 }
 
@@ -317,7 +322,8 @@ int run(const Layer& a, hipStream_t s) {
     rc = mx_quantize_tiled(x, turn, s);
   }
   if (rc != DIMQ_OK) return rc;
-  const MxMm p{{ws + at.xc, blocks * 16, ws + at.xs, xr}, {a.codes, blocks * 16, ws + at.ws, wr}, a.M, a.N, blocks, 1, 0, 0, a.out};
+  const MxMm p{{ws + at.xc, blocks * 16, ws + at.xs, xr}, {a.codes, blocks * 16, ws + at.ws, wr},
+               a.M, a.N, blocks, 1, 0, 0, a.out};
   return mx_mm<true, false, false>(p, at.plan, reinterpret_cast<float*>(ws + at.part), s, what);
 }
 

@@ -169,7 +169,7 @@ struct Backward {
   Backward(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K, bool to_x, bool to_w, bool to_b) {
     auto take = [&](int64_t& at, int64_t n) { at = bytes, bytes += (n + 255) / 256 * 256; };
     parts = parts_of(g_dtype);
-    copy = parts > 1 || !mx_vec_rows(g, g_dtype, N, ldg);
+    copy = parts > 1 || !mx_vec_rows(g, g_dtype, N, ldg) || ldg >= (1 << 22);  // mx_mm's limit on a row's bytes
     const int64_t whole = parts > 1 ? 64 : 1;
     wrows = (N + whole - 1) / whole * whole, xrows = (M + whole - 1) / whole * whole;
     gm = xrows, gn = mx_pad8(wrows);

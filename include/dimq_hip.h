@@ -564,7 +564,7 @@ int dimq_mx_dequantize(const void* codes, const uint8_t* scales, int bits, int64
  * nullable, any float dtype.  codes8 / scales8 (nullable): x's 8-bit form,
  * [M, ceil(K / 32), 32] and [M, ceil(K / 32)], written from the same read of x.
  * The workspace (256-byte aligned, the size the query gives, which is 0 for
- * most calls of up to 16 rows) is written on `stream`. */
+ * most calls of few rows) is written on `stream`. */
 int64_t dimq_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int dimq_mxfp4_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* codes,
                       const uint8_t* scales, const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype,

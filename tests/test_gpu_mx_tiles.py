@@ -92,7 +92,7 @@ def test_rows_that_are_not_finite(gpu):
 
 
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
-@pytest.mark.parametrize("M,K,N", [(1, 64, 33), (5, 1000, 70), (16, 4128, 48), (13, 200, 16)])
+@pytest.mark.parametrize("M,K,N", [(1, 64, 33), (5, 1000, 70), (16, 4128, 48), (13, 200, 16), (61, 776, 100), (250, 100, 50)])
 def test_few_rows_as_many(gpu, dt, M, K, N):
     """The single launch quantizes x by itself: the same rows within a larger batch give the same values, whatever they
     hold (subnormal numbers, ties, whole blocks of zeros, blocks that are not finite), up to the order of the fp32 sums."""
@@ -105,7 +105,7 @@ def test_few_rows_as_many(gpu, dt, M, K, N):
     ref, S = xq @ wq.t(), torch.nan_to_num(xq).abs() @ wq.abs().t()
     ok = S.max(dim=1).values < 1e37  # no sum overflows fp32
     _check(few[ok.to(gpu)], ref[ok], S[ok], K)
-    many = mx.mxfp4_linear(x.repeat(17, 1).to(gpu), c, s, out_dtype=F32)[:M]
+    many = mx.mxfp4_linear(x.repeat(300, 1).to(gpu), c, s, out_dtype=F32)[:M]
     _check(many[ok.to(gpu)], ref[ok], S[ok], K)
 
 
