@@ -13,8 +13,8 @@
 // bytes a lane into a ring of S slots; no register holds operands in flight and the main loop has no vector arithmetic.
 // C is the instructions' first operand, so a lane's accumulators are four neighbouring columns of one row.
 //
-// Measured: 16384 x 8192 codes summed over 8192 507 us (4,340 TFLOP/s); both bf16 gradients of 8192 x 4096 -> 4096 209 and
-// 203 us (1,315 and 1,354 TFLOP/s; the library's product of 8192^3 reaches 1,448).  Bound by the matrix unit, busy 59 %
+// Measured: 16384 x 8192 codes summed over 8192 507 to 522 us (4,340 TFLOP/s); both bf16 gradients of 8192 x 4096 -> 4096
+// 209 and 203 us (1,315 and 1,354 TFLOP/s; the library's product of 8192^3 reaches 1,448 there).  Bound by the matrix unit, busy 59 %
 // (codes) and 70 % of the cycles, at the 1.7 GHz that the card holds under this load: without any load in the loop the same
 // data take 514 us of 520 and 187 of 204.
 #pragma once

@@ -143,8 +143,8 @@ struct BackArgs {
 };
 
 // Codes to values (SLOPE 0), or the upstream gradient times GELU's slope at them.  Eight elements a lane, as above.  Bound
-// by the bytes: GELU of 12608 x 2048 bf16 and its gradient move 130 MB each in 26 and 27 us, 4.9 TB/s; 4096 x 4096 to fp32
-// 15 and 16 us, 5.2 TB/s.
+// by the bytes: 4096 x 4096 to fp32 15 and 16 us, 5.2 TB/s; GELU of 12608 x 2048 bf16 and its gradient, which move 130 MB
+// each in 23 to 27 us, also by 30 instructions an element.
 template <int BITS, int YT, bool SLOPE>
 __global__ __launch_bounds__(256) void mx_back_kernel(BackArgs a, FastDiv div, uint32_t units) {
   const uint32_t u = (blockIdx.x * 256u + threadIdx.x) >> 2;
