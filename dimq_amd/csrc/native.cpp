@@ -699,14 +699,23 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
 // gelu(h), h kept in 8 bits for the backward pass.
 struct MxGelu : torch::autograd::Function<MxGelu> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h) {
-    const auto [y, c, s] = gelu_forward(h.detach());
-    ctx->save_for_backward({c, s});
+    const Rows r(h, "gelu", "input");
+    const int64_t nb = mx_blocks(r.cols);
+    const Tensor y = at::empty(h.sizes(), h.options()), kept = at::empty({r.n * nb * 33}, h.options().dtype(at::kByte));
+    const On on(h);
+    check_rc(dimq_mx_gelu_forward(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, ptr(y), pi8(kept), pu8(kept) + r.n * nb * 32, on.stream));
+    ctx->save_for_backward({kept});  // codes, then scales
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("mx.gelu");
-    const auto saved = ctx->get_saved_variables();
-    return {gelu_backward(grads[0], saved[0], saved[1])};
+    const Tensor kept = ctx->get_saved_variables()[0];
+    const Rows g(grads[0], "gelu", "gradient");
+    const Tensor gh = at::empty(grads[0].sizes(), grads[0].options());
+    const On on(gh);
+    check_rc(dimq_mx_gelu_backward(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, pi8(kept), pu8(kept) + g.n * mx_blocks(g.cols) * 32,
+                                   ptr(gh), on.stream));
+    return {gh};
   }
 };
 
