@@ -190,7 +190,8 @@ int quant_launch(const QuantArgs& a, MxScaleTurn turn, hipStream_t s) {
     b.row0 = r;
     if (r > 0) turn.groups = 0;
     const dim3 more(grid.x + turn.groups);
-    if (b.y) mx_quant_kernel<XT, false, true, true><<<grid, 256, 0, s>>>(b, div, units);
+    if (b.y && b.codes8) mx_quant_kernel<XT, false, true, true><<<grid, 256, 0, s>>>(b, div, units);
+    else if (b.y) mx_quant_kernel<XT, false, false, true><<<grid, 256, 0, s>>>(b, div, units);
     else if (b.tiled && b.codes8) mx_quant_tiled_kernel<XT, true><<<more, 256, 0, s>>>(b, div, units, turn);
     else if (b.tiled) mx_quant_tiled_kernel<XT, false><<<more, 256, 0, s>>>(b, div, units, turn);
     else if (b.codes4 && b.codes8) mx_quant_kernel<XT, true, true, false><<<grid, 256, 0, s>>>(b, div, units);
@@ -326,7 +327,7 @@ extern "C" int dimq_mx_gelu_forward(const void* h, int dtype, int64_t rows, int6
   int rc = mx_check_rows("mx_gelu_forward", h, dtype, rows, cols, ldh);
   if (rc != DIMQ_OK) return rc;
   if (rows == 0 || cols == 0) return DIMQ_OK;
-  if ((rc = check_codes("mx_gelu_forward", codes8, scales8)) != DIMQ_OK) return rc;
+  if ((codes8 || scales8) && (rc = check_codes("mx_gelu_forward", codes8, scales8)) != DIMQ_OK) return rc;
   DIMQ_CHECK(y, "mx_gelu_forward: null pointer");
   const int64_t nb = mx_blocks(cols);
   return quant_any(dtype, {h, ldh, rows, cols, nullptr, nullptr, codes8, scales8, nb, nb, nb, y}, as_stream(stream));

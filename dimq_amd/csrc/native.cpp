@@ -647,7 +647,8 @@ void once(const char* op) {
 // y = Q4(x) Q4(w)^T + b, straight through backward: gx = g Q4(w), gw = g^T Q8(x), gb = sum g.  Kept for it: w's 4-bit
 // and x's 8-bit codes, each only where its gradient is asked for.
 struct MxLinear : torch::autograd::Function<MxLinear> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias) {
+  // keep: a backward pass may follow
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, bool keep) {
     TORCH_CHECK(x.is_cuda(), "mx.linear expects a CUDA input");
     TORCH_CHECK(w.dim() == 2 && x.dim() > 0 && x.size(-1) == w.size(1),
                 "mx.linear: input's last dimension must equal the weight's, [out_features, in_features]");
@@ -658,7 +659,7 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     const Bias b(bias, wr.n, "out_features");
     TORCH_CHECK(!b.t.defined() || b.t.device() == x.device(), "mx.linear: the bias must be on ", x.device().str());
     const int64_t N = w.size(0), K = w.size(1), nb = mx_blocks(K);
-    const bool to_w = w.requires_grad();
+    const bool to_w = keep && w.requires_grad();
     // codes, then scales: one allocation each
     const auto bytes = x.options().dtype(at::kByte);
     const Tensor wq = at::empty({N * nb * 17}, bytes), xq = to_w ? at::empty({r.n * nb * 33}, bytes) : Tensor();
@@ -692,18 +693,21 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
                                      pi8(xq), xq.defined() ? pu8(xq) + r.n * nb * 32 : nullptr, K, ptr(gx),
                                      gx.defined() ? dt(gx) : 0, ptr(gw), gw.defined() ? dt(gw) : 0, ptr(gb), b ? dt(gb) : 0,
                                      ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
-    return {gx, gw, gb};
+    return {gx, gw, gb, Tensor()};
   }
 };
 
 // gelu(h), h kept in 8 bits for the backward pass.
 struct MxGelu : torch::autograd::Function<MxGelu> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& h) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& h, bool keep) {
     const Rows r(h, "gelu", "input");
     const int64_t nb = mx_blocks(r.cols);
-    const Tensor y = at::empty(h.sizes(), h.options()), kept = at::empty({r.n * nb * 33}, h.options().dtype(at::kByte));
+    keep = keep && h.requires_grad();
+    const Tensor y = at::empty(h.sizes(), h.options());
+    const Tensor kept = keep ? at::empty({r.n * nb * 33}, h.options().dtype(at::kByte)) : Tensor();
     const On on(h);
-    check_rc(dimq_mx_gelu_forward(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, ptr(y), pi8(kept), pu8(kept) + r.n * nb * 32, on.stream));
+    check_rc(dimq_mx_gelu_forward(ptr(r.t), dt(r.t), r.n, r.cols, r.ld, ptr(y), pi8(kept),
+                                  keep ? pu8(kept) + r.n * nb * 32 : nullptr, on.stream));
     ctx->save_for_backward({kept});  // codes, then scales
     return y;
   }
@@ -715,7 +719,7 @@ struct MxGelu : torch::autograd::Function<MxGelu> {
     const On on(gh);
     check_rc(dimq_mx_gelu_backward(ptr(g.t), dt(g.t), g.n, g.cols, g.ld, pi8(kept), pu8(kept) + g.n * mx_blocks(g.cols) * 32,
                                    ptr(gh), on.stream));
-    return {gh};
+    return {gh, Tensor()};
   }
 };
 
@@ -802,7 +806,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mxfp4_linear", &mxfp4_linear, Unlocked());
   m.def("mxfp4_linear_grad_input", &mxfp4_linear_grad_input, Unlocked());
   m.def("linear_grad_weight", &linear_grad_weight, Unlocked());
-  m.def("mx_linear", [](const Tensor& x, const Tensor& w, const OptTensor& b) { return MxLinear::apply(x, w, b); },
+  m.def("mx_linear",
+        [](const Tensor& x, const Tensor& w, const OptTensor& b) { return MxLinear::apply(x, w, b, at::GradMode::is_enabled()); },
         Unlocked());
-  m.def("mx_gelu", [](const Tensor& h) { return MxGelu::apply(h); }, Unlocked());
+  m.def("mx_gelu", [](const Tensor& h) { return MxGelu::apply(h, at::GradMode::is_enabled()); }, Unlocked());
 }

@@ -606,7 +606,7 @@ int dimq_mx_linear_backward(const void* g, int g_dtype, int64_t M, int64_t N, in
                             int gx_dtype, void* gw, int gw_dtype, void* gb, int gb_dtype, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
-/* y = gelu(h) = h Phi(h) and h's 8-bit form from one read of h (y [rows, cols]
+/* y = gelu(h) = h Phi(h) and h's 8-bit form (nullable pair) from one read of h (y [rows, cols]
  * contiguous in h's dtype), and the gradient gh = g gelu'(Q8(h)) in g's dtype. */
 int dimq_mx_gelu_forward(const void* h, int dtype, int64_t rows, int64_t cols, int64_t ldh, void* y, int8_t* codes8,
                          uint8_t* scales8, void* stream);

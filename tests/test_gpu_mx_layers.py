@@ -65,6 +65,21 @@ def test_linear_of_no_rows_trains(gpu):
 
 
 @pytest.mark.gpu
+def test_without_gradients(gpu):
+    """The same values where no backward pass can follow, and nothing kept for one."""
+    from dimq_amd import mx
+    x, h = _acts(200, 96, BF16, 1).to(gpu), torch.randn(70, 129, generator=_gen(2)).to(gpu).requires_grad_()
+    w = torch.randn(48, 96, generator=_gen(3)).to(gpu).requires_grad_()
+    announce("no gradients")
+    y, z = mx.linear(x, w), mx.gelu(h)
+    with torch.no_grad():
+        y2, z2 = mx.linear(x, w), mx.gelu(h)
+    assert torch.equal(y, y2) and torch.equal(z, z2)
+    assert y.requires_grad and z.requires_grad and not y2.requires_grad and not z2.requires_grad
+    assert torch.equal(mx.gelu(h.detach()), z2) and torch.equal(mx.linear(x, w.detach()), y2)
+
+
+@pytest.mark.gpu
 def test_step_captured_in_a_graph(gpu):
     """A layer's forward and backward pass in one graph; every replay against the eager step."""
     x, w = torch.zeros(300, 160, device=gpu, dtype=BF16), torch.randn(224, 160, generator=_gen(1)).to(gpu)

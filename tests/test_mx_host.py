@@ -121,3 +121,11 @@ def test_entry_points_refuse():
     # nothing to do is no error
     assert q(None, _C.F32, 0, 32, 32, None, None, 1, None, None, None) == 0
     assert f(None, _C.F32, 0, 32, 32, None, None, None, 0, 8, None, _C.F32, None, 0, 0, *tail) == 0
+
+
+def test_gelu_refuses_half_a_kept_form():
+    from dimq_amd import _C
+    gf = _C.lib.dimq_mx_gelu_forward
+    for codes, scales in ((_p(), None), (None, _p())):
+        assert gf(_p(), _C.F32, 2, 8, 8, _p(), codes, scales, None) == 1
+        assert "null pointer" in _C.lib.dimq_last_error().decode()
