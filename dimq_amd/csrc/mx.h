@@ -123,7 +123,7 @@ __device__ __forceinline__ float mx_exp_quarter(float b) {
 template <int DT>
 __device__ __forceinline__ float mx_gelu(float h) {
   const float b = mx_64ths(h), m = mx_tail_factor<DT, -64>(b), root = mx_exp_quarter<DT>(b);
-  const float top = 0.5f * (h + fabsf(h));  // max(h, 0) that keeps NaN
+  const float top = fmaf(0.5f, fabsf(h), 0.5f * h);  // max(h, 0) that keeps NaN; halves, as the sum of both would overflow
   return fmaf(b * m * root, root, top);
 }
 
