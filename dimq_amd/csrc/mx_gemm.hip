@@ -308,6 +308,7 @@ int run(const Layer& a, hipStream_t s) {
     return few_rows_any(a.x_dtype, {a.x, a.ldx, a.M, a.K, a.codes, a.scales, a.N, blocks,
                                     blocks % 4 == 0 && aligned(a.scales, 4), a.out}, s);
   }
+  DIMQ_CHECK(a.M <= kMxMaxRows && a.N <= kMxMaxRows, "%s: too large", what);
   const Layout at(a.M, a.K, a.N);
   DIMQ_CHECK(a.workspace && aligned(a.workspace, 256) && a.workspace_bytes >= at.bytes,
              "%s: the workspace is too small or not 256-byte aligned", what);

@@ -510,6 +510,9 @@ inline int64_t mx_scale_rows(int64_t n) {
   const int64_t a = (n + 255) / 256 * 256, b = (n + 191) / 192 * 192;
   return a > b ? a : b;
 }
+// Rows and columns of a product at most: a stage of scales, 8 bytes for each of mx_scale_rows, stays below 2^31 bytes, the
+// tile kernel's 32-bit step.
+constexpr int64_t kMxMaxRows = (1 << 28) - 256;
 inline int64_t mx_tiles(int tile, int64_t rows, int64_t cols) {
   const int64_t r = tile == 3 ? 256 : 256 >> tile, c = tile == 3 ? 192 : 256 >> tile;
   return ((rows + r - 1) / r) * ((cols + c - 1) / c);
@@ -566,7 +569,7 @@ int mx_mm_launch(const MxMm& p, int splits, hipStream_t s, const char* what) {
 template <bool FP4, bool CT, bool RT>
 int mx_mm(MxMm p, const MxPlan& pl, float* partial, hipStream_t s, const char* what) {
   // a lane's offsets inside a tile and a stage's step are 32 bits
-  DIMQ_CHECK(p.len * p.planes < (1ll << 31) && p.rows < (1ll << 28) && p.cols < (1ll << 28), "%s: too large", what);
+  DIMQ_CHECK(p.len * p.planes < (1ll << 31) && p.rows <= kMxMaxRows && p.cols <= kMxMaxRows, "%s: too large", what);
   DIMQ_CHECK(p.r.ld < (1 << 23) && p.c.ld < (1 << 23), "%s: rows beyond 8 MB are not supported", what);
   const MxOut out = p.out;
   if (pl.splits > 1) {
