@@ -21,8 +21,23 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from ._C import _native
-from .ops import ACTIVATIONS
+from .ops import ACTIVATIONS, require_extension
+
+
+class _Unbuilt:
+    """Stands for the compiled half while it cannot be loaded: an operator's call looks for it again, or raises."""
+
+    def __getattr__(self, name: str):
+        global _native
+        require_extension()
+        from ._C import _native
+        return getattr(_native, name)
+
+
+try:  # now, so that torch.ops.dimq is there after the package's import
+    from ._C import _native
+except Exception:
+    _native = _Unbuilt()
 
 
 def quantize_mxfp4(x: Tensor) -> tuple[Tensor, Tensor]:
