@@ -680,11 +680,13 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     const Tensor &g = grads[0], &wq = saved[0], &xq = saved[1];
     const auto layer = ctx->saved_data["layer"].toIntVector();
     const int64_t N = layer[0], K = layer[1], nb = mx_blocks(K);
-    const bool b = layer[3];
+    // asked for by this pass, of what the forward pass kept for
+    const bool b = layer[3] && ctx->needs_input_grad(2);
     const Rows r(g, "mx.linear", "gradient");
     Tensor gx, gw, gb;
-    if (wq.defined()) gx = at::empty(out_shape(g, K), g.options());
-    if (xq.defined()) gw = at::empty({N, K}, g.options().dtype(static_cast<at::ScalarType>(layer[2])));
+    if (wq.defined() && ctx->needs_input_grad(0)) gx = at::empty(out_shape(g, K), g.options());
+    if (xq.defined() && ctx->needs_input_grad(1))
+      gw = at::empty({N, K}, g.options().dtype(static_cast<at::ScalarType>(layer[2])));
     if (b) gb = at::empty({N}, g.options().dtype(static_cast<at::ScalarType>(layer[4])));
     const On on(g);
     const Tensor ws = workspace(dimq_mx_linear_backward_workspace_bytes(ptr(r.t), dt(r.t), r.n, N, r.ld, K,
