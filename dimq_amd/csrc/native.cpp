@@ -699,6 +699,57 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
   }
 };
 
+// The layer on packed weights where a gradient may follow: straight through to the input, gx = g W; to the bias, the sum of
+// g over the rows; to the residual, g.  Nothing is kept but the weights.
+struct MxPackedLinear : torch::autograd::Function<MxPackedLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& bias, const OptTensor& residual,
+                        const Tensor& codes, const Tensor& scales, int64_t activation,
+                        std::optional<at::ScalarType> out_dtype) {
+    const Tensor y = mxfp4_linear(x, codes, scales, bias, residual, activation, out_dtype);
+    ctx->save_for_backward({codes, scales});
+    auto type = [](const OptTensor& t) { return static_cast<int64_t>(t ? t->scalar_type() : at::kFloat); };
+    ctx->saved_data["layer"] = std::vector<int64_t>{activation, x.size(-1), static_cast<int64_t>(x.scalar_type()),
+                                                    bias.has_value(), type(bias), residual.has_value(), type(residual)};
+    if (bias) ctx->saved_data["bias"] = bias->sizes().vec();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const char* op = "mxfp4_linear";
+    once(op);
+    const auto layer = ctx->saved_data["layer"].toIntVector();
+    TORCH_CHECK(layer[0] == DIMQ_ACT_NONE, op, ": no gradient through its fused activation; apply the activation to the output "
+                "of a call without one");
+    auto type = [&](int i) { return static_cast<at::ScalarType>(layer[i]); };
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& g = grads[0];
+    const int64_t K = layer[1];
+    const Rows r(g, op, "gradient");
+    const Codes w(saved[0], saved[1], K, 4, g, op);
+    // inputs are counted without the absent ones
+    Tensor gx, gb, gr;
+    if (ctx->needs_input_grad(0)) gx = at::empty(out_shape(g, K), g.options().dtype(type(2)));
+    if (layer[3] && ctx->needs_input_grad(1)) gb = at::empty(ctx->saved_data["bias"].toIntVector(), g.options().dtype(type(4)));
+    if (layer[5] && ctx->needs_input_grad(1 + layer[3])) gr = g.to(type(6));
+    if (gx.defined() || gb.defined()) {
+      const On on(g);
+      const Tensor ws = workspace(dimq_mx_linear_backward_workspace_bytes(ptr(r.t), dt(r.t), r.n, w.rows, r.ld, K,
+                                                                          gx.defined() + 4 * gb.defined()), g);
+      check_rc(dimq_mx_linear_backward(ptr(r.t), dt(r.t), r.n, w.rows, r.ld, pu8(w.c), pu8(w.s), nullptr, nullptr, K, ptr(gx),
+                                       gx.defined() ? dt(gx) : 0, nullptr, 0, ptr(gb), gb.defined() ? dt(gb) : 0, ptr(ws),
+                                       ws.defined() ? ws.numel() : 0, on.stream));
+    }
+    return {gx, gb, gr, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor mxfp4_linear_graph(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias,
+                          const OptTensor& residual, int64_t activation, std::optional<at::ScalarType> out_dtype) {
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || (bias && bias->requires_grad()) || (residual && residual->requires_grad())))
+    return MxPackedLinear::apply(x, bias, residual, codes, scales, activation, out_dtype);
+  return mxfp4_linear(x, codes, scales, bias, residual, activation, out_dtype);
+}
+
 // gelu(h), h kept in 8 bits for the backward pass.
 struct MxGelu : torch::autograd::Function<MxGelu> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, bool keep) {
@@ -785,6 +836,8 @@ TORCH_LIBRARY_IMPL(dimq, CUDA, m) {
   m.impl("gelu_backward", gelu_backward);
 }
 
+TORCH_LIBRARY_IMPL(dimq, AutogradCUDA, m) { m.impl("mxfp4_linear", mxfp4_linear_graph); }
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   namespace py = pybind11;
   using Unlocked = py::call_guard<py::gil_scoped_release>;
@@ -805,7 +858,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("quantize_and_compress", &quantize_and_compress, Unlocked());
   m.def("dequantize_mxfp4", &dequantize_mxfp4, Unlocked());
   m.def("decompress_activation", &decompress_activation, Unlocked());
-  m.def("mxfp4_linear", &mxfp4_linear, Unlocked());
+  m.def("mxfp4_linear", &mxfp4_linear_graph, Unlocked());
   m.def("mxfp4_linear_grad_input", &mxfp4_linear_grad_input, Unlocked());
   m.def("linear_grad_weight", &linear_grad_weight, Unlocked());
   m.def("mx_linear",

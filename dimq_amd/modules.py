@@ -151,7 +151,8 @@ class DIMQCodebookLinear(nn.Module):
 
 class DIMQMXFP4Linear(nn.Module):
     """Linear on a microscaled 4-bit weight and input: y = act(Q4(x) @ W^T + b + residual), W the values of the codes
-    (``mx.quantize_mxfp4``: uint8 codes [out_features, 16 * blocks], one scale byte a block of 32)."""
+    (``mx.quantize_mxfp4``: uint8 codes [out_features, 16 * blocks], one scale byte a block of 32).  The weight is frozen;
+    gradients reach x and the residual where no activation is fused."""
 
     def __init__(self, codes, scales, in_features, bias=None, *, out_dtype: torch.dtype | None = None) -> None:
         super().__init__()

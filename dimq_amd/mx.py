@@ -6,11 +6,11 @@ the low half, 16 bytes a block) or 8-bit integers -127..127 in units of 1/64 of 
 infinity stands for NaN throughout.  ``Q4(x)`` and ``Q8(x)`` are the values that x's codes stand for.
 
 * Serving: ``quantize_mxfp4`` packs a weight once; ``mxfp4_linear`` runs the layer, quantizing its input on the way in
-  (``modules.DIMQMXFP4Linear`` holds both).
+  (``modules.DIMQMXFP4Linear`` holds both), and as a frozen layer passes gradients on.
 * Training: ``linear`` (``MXFP4TrainLinear``) runs that layer on the master weights with straight-through gradients and
   keeps its input in 8 bits for the weight gradient; ``gelu`` keeps its input in 8 bits too.
 
-The functions without gradients are torch ops too (``torch.ops.dimq.quantize_mxfp4`` and so on).  All of it is for CUDA
+All but ``linear`` and ``gelu`` are torch ops too (``torch.ops.dimq.quantize_mxfp4`` and so on).  All of it is for CUDA
 (HIP) tensors in fp32, fp16 and bf16; the gradients are those of the formulas in each function's
 description and have no gradients of their own.
 """
@@ -68,7 +68,9 @@ def decompress_activation(codes: Tensor, scales: Tensor, size: int, dtype: torch
 def mxfp4_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Tensor | None = None, *, residual: Tensor | None = None,
                  activation: str | None = None, out_dtype: torch.dtype | None = None) -> Tensor:
     """``act(Q4(x) W^T + bias + residual)`` for the weight W that ``quantize_mxfp4`` packed (codes ``[out_features, ...]``);
-    activation None, "relu" or "gelu" (exact); the output in ``out_dtype`` (x's by default)."""
+    activation None, "relu" or "gelu" (exact); the output in ``out_dtype`` (x's by default).  W is frozen: gradients go
+    straight through the quantization to x (``g W``), to the bias (``sum g``) and to the residual (``g``); a backward pass
+    through a fused activation raises."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     return _native.mxfp4_linear(x, codes, scales, bias, residual, ACTIVATIONS[activation], out_dtype)
