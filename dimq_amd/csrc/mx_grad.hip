@@ -2,7 +2,8 @@
 //   to the input   gx = g W        W the 4-bit weights [N, K], summed over N
 //   to the weight  gw = g^T X      X the 8-bit checkpoint [M, K], summed over M, and gb = sum of g over M
 // Codes times scales are exact in bf16, and so is a gradient of 16 or 32 bits as a sum of bf16 parts (one for bf16, two
-// for fp16's 11 bits, three for fp32's 24), so that every product is exact and only the fp32 sums round.  W or X is
+// for fp16's 11 bits, three for fp32's 24), so that every product is exact and only the fp32 sums round; but fp32 gradients
+// below 2^-110 reach past bf16's least step 2^-133 and are taken to its nearest multiple.  W or X is
 // decoded to bf16 in the workspace once (a 256 x 256 tile would decode it again for every row tile), g is split into
 // planes of parts there unless it is bf16 in aligned rows, and the tiled product (mx_mm.h) sums over the planes one after
 // another.  One launch makes all that ready, for both gradients at once.
@@ -12,8 +13,9 @@
 namespace dimq {
 namespace {
 
-// x as NS bf16 parts that add up to it, by truncation (rounding could carry the first part to infinity); a NaN or an
-// infinity is the first part alone.
+// x as NS bf16 parts that add up to it, by truncation (rounding could carry the first part to infinity).  The last of
+// three is rounded: that changes nothing where |x| is 2^-110 or more, and below takes x to the nearest multiple of a part's
+// least step 2^-133.  A NaN or an infinity is the first part alone.
 template <int NS>
 __device__ __forceinline__ void bf16_parts(float x, uint16_t (&h)[NS]) {
   const uint32_t u = __float_as_uint(x);
@@ -25,7 +27,7 @@ __device__ __forceinline__ void bf16_parts(float x, uint16_t (&h)[NS]) {
   }
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    const uint32_t t = __float_as_uint(x) & 0xffff0000u;
+    const uint32_t t = i == 2 ? float_to_bf16_bits(x) << 16 : __float_as_uint(x) & 0xffff0000u;
     h[i] = (uint16_t)(t >> 16);
     x -= __uint_as_float(t);
   }

@@ -584,7 +584,8 @@ int dimq_mx_linear_forward(const void* x, int x_dtype, int64_t M, int64_t K, int
  *   gx = g W             (W from its 4-bit codes)
  *   gw = g^T Q8(x)       (x from its 8-bit checkpoint), gb = sum of g over m
  * Every product is exact (g as a sum of bf16 parts, codes times scales in
- * bf16), the sums are fp32 in a fixed order, outputs [M, K], [N, K], [N]
+ * bf16; an fp32 g below 2^-110 is first rounded to a multiple of 2^-133, the
+ * least step of a part), the sums are fp32 in a fixed order, outputs [M, K], [N, K], [N]
  * (nullable) contiguous in their dtypes.  M = 0 gives zeros.  The queries
  * take g because a copy is made of one that is not 16-byte aligned. */
 int64_t dimq_mx_grad_input_workspace_bytes(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K);
