@@ -134,6 +134,7 @@ _SIGS = {
     "dimq_mx_linear_backward_workspace_bytes": (_i64, [_vp, _int, _i64, _i64, _i64, _i64, _int]),
     "dimq_mx_linear_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp, _int, _vp, _int,
                                        _vp, _i64, _vp]),
+    "dimq_mx_linear_route": (_int, [_int, _int, _i64, _i64, _i64]),
     "dimq_mx_grad_input_workspace_bytes": (_i64, [_vp, _int, _i64, _i64, _i64, _i64]),
     "dimq_mxfp4_linear_grad_input": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _int, _vp, _i64, _vp]),
     "dimq_mx_grad_weight_workspace_bytes": (_i64, [_vp, _int, _i64, _i64, _i64, _i64]),

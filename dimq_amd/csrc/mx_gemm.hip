@@ -249,6 +249,12 @@ struct Layout {
 };
 
 }  // namespace
+
+int mx_forward_route(bool f32, int64_t M, int64_t K, int64_t N) {
+  const int64_t stages = (mx_blocks(K) + 7) / 8;
+  return few_rows_pay(f32, M, K, N) ? 0 : mx_route(mx_plan(true, M, N, stages), M, N, stages);
+}
+
 }  // namespace dimq
 
 using namespace dimq;

@@ -272,6 +272,15 @@ extern "C" int dimq_mx_linear_backward(const void* g, int g_dtype, int64_t M, in
                   workspace, workspace_bytes, as_stream(stream));
 }
 
+extern "C" int dimq_mx_linear_route(int product, int dtype, int64_t M, int64_t K, int64_t N) {
+  if (M <= 0 || K <= 0 || N <= 0 || product < 0 || product > 2 || (dtype != DIMQ_F32 && dtype != DIMQ_F16 && dtype != DIMQ_BF16))
+    return -1;
+  if (product == 0) return mx_forward_route(dtype == DIMQ_F32, M, K, N);
+  const Backward at(nullptr, dtype, M, N, N, K, true, true, false);
+  return product == 1 ? mx_route(at.gx, M, K, (at.wrows + 63) / 64 * at.parts)
+                      : mx_route(at.gw, N, K, (at.xrows + 63) / 64 * at.parts);
+}
+
 extern "C" int64_t dimq_mx_grad_input_workspace_bytes(const void* g, int g_dtype, int64_t M, int64_t N, int64_t ldg, int64_t K) {
   return dimq_mx_linear_backward_workspace_bytes(g, g_dtype, M, N, ldg, K, 1);
 }

@@ -558,6 +558,12 @@ inline MxPlan mx_plan(bool fp4, int64_t rows, int64_t cols, int64_t stages) {
   return best;
 }
 
+// Slices and the kernel's number (include/dimq_hip.h, dimq_mx_linear_route).
+inline int mx_route(const MxPlan& pl, int64_t rows, int64_t cols, int64_t stages) {
+  const int kernel = pl.tile == 0 ? 1 : pl.tile == 3 ? 2 : pl.tile == 2 ? 5 : mx_deep(pl, rows, cols, stages) ? 4 : 3;
+  return pl.splits * 8 + kernel;
+}
+
 template <class T>
 int mx_mm_launch(const MxMm& p, int splits, hipStream_t s, const char* what) {
   const int64_t tiles = ((p.rows + T::BR - 1) / T::BR) * ((p.cols + T::BC - 1) / T::BC);

@@ -108,4 +108,7 @@ struct MxTiledOperand {
 int mx_quantize_tiled(const MxTiledOperand& x, MxScaleTurn turn, hipStream_t s);
 int mx_quantize_pair(const MxTiledOperand& x, const MxTiledOperand& w, hipStream_t s);
 
+// dimq_mx_linear_route of the forward product (mx_gemm.hip).
+int mx_forward_route(bool f32, int64_t M, int64_t K, int64_t N);
+
 }  // namespace dimq

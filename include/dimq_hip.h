@@ -607,6 +607,14 @@ int dimq_mx_linear_backward(const void* g, int g_dtype, int64_t M, int64_t N, in
                             int gx_dtype, void* gw, int gw_dtype, void* gb, int gb_dtype, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
+/* The kernel that a product of an [M, K] input and an [N, K] weight runs on,
+ * for tuning and for tests: product 0 y (dtype: x's), 1 gx, 2 gw (g's).
+ * Returns 0 for the single launch of few rows, else 8 * slices of the
+ * reduction + 1 for 256x256 tiles, 2 for 256x192, 3 for 128x128 with two
+ * slots in the LDS, 4 for 128x128 with four, 5 for 64x64; -1 for sizes, a
+ * dtype or a product that there are none of. */
+int dimq_mx_linear_route(int product, int dtype, int64_t M, int64_t K, int64_t N);
+
 /* y = gelu(h) = h Phi(h) and h's 8-bit form (nullable pair) from one read of h (y [rows, cols]
  * contiguous in h's dtype), and the gradient gh = g gelu'(Q8(h)) in g's dtype. */
 int dimq_mx_gelu_forward(const void* h, int dtype, int64_t rows, int64_t cols, int64_t ldh, void* y, int8_t* codes8,
