@@ -347,6 +347,35 @@ Tensor max_pool2d_nhwc(const Tensor& x, int64_t kernel_h, int64_t kernel_w, int6
   return y;
 }
 
+// ---- calls past the dispatcher -----------------------------------------------------
+
+// Whether nothing stands between a call and its kernel: no dispatch mode, trace or transform on this thread (their keys
+// would be included), and no tensor subclass as input.
+bool plain(const Tensor& x) {
+  return (c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set -
+          c10::autocast_dispatch_keyset).empty() && !x.unsafeGetTensorImpl()->is_python_dispatch();
+}
+
+// F without the dispatcher, which takes 1 us of a call's 6, where that makes no difference; otherwise its operator.
+template <auto F>
+struct Direct;
+template <class R, class... A, R (*F)(const Tensor&, A...)>
+struct Direct<F> {
+  const char* name;
+  R operator()(const Tensor& x, A... a) const { return plain(x) ? F(x, a...) : op(x, a...); }
+  R op(const Tensor& x, A... a) const {  // by its Python name: a trace records calls there
+    const pybind11::gil_scoped_acquire locked;
+    return pybind11::module_::import("torch").attr("ops").attr("dimq").attr(name)(x, a...).template cast<R>();
+  }
+};
+
+// Autograd nodes that launch kernels themselves are no operators: a trace would keep their allocations and lose the rest.
+void untraced(const char* op) {
+  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer) &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+              op, " cannot be traced");
+}
+
 // ---- microscaled formats -----------------------------------------------------------
 
 bool mx_float(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
@@ -650,6 +679,7 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
   // keep: a backward pass may follow
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, bool keep) {
     TORCH_CHECK(x.is_cuda(), "mx.linear expects a CUDA input");
+    untraced("mx.linear");
     TORCH_CHECK(w.dim() == 2 && x.dim() > 0 && x.size(-1) == w.size(1),
                 "mx.linear: input's last dimension must equal the weight's, [out_features, in_features]");
     TORCH_CHECK(w.device() == x.device(), "mx.linear: the weight must be on ", x.device().str());
@@ -675,6 +705,7 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    untraced("mx.linear");
     once("mx.linear");
     const auto saved = ctx->get_saved_variables();
     const Tensor &g = grads[0], &wq = saved[0], &xq = saved[1];
@@ -699,13 +730,20 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
   }
 };
 
+// mxfp4_linear from below autograd.
+Tensor mxfp4_linear_below(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias,
+                          const OptTensor& residual, int64_t activation, std::optional<at::ScalarType> out_dtype) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  return Direct<&mxfp4_linear>{"mxfp4_linear"}(x, codes, scales, bias, residual, activation, out_dtype);
+}
+
 // The layer on packed weights where a gradient may follow: straight through to the input, gx = g W; to the bias, the sum of
 // g over the rows; to the residual, g.  Nothing is kept but the weights.
 struct MxPackedLinear : torch::autograd::Function<MxPackedLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& bias, const OptTensor& residual,
                         const Tensor& codes, const Tensor& scales, int64_t activation,
                         std::optional<at::ScalarType> out_dtype) {
-    const Tensor y = mxfp4_linear(x, codes, scales, bias, residual, activation, out_dtype);
+    const Tensor y = mxfp4_linear_below(x, codes, scales, bias, residual, activation, out_dtype);
     ctx->save_for_backward({codes, scales});
     auto type = [](const OptTensor& t) { return static_cast<int64_t>(t ? t->scalar_type() : at::kFloat); };
     ctx->saved_data["layer"] = std::vector<int64_t>{activation, x.size(-1), static_cast<int64_t>(x.scalar_type()),
@@ -714,10 +752,11 @@ struct MxPackedLinear : torch::autograd::Function<MxPackedLinear> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const char* op = "mxfp4_linear";
-    once(op);
+    const char* op = "mxfp4_linear's gradient";
+    untraced(op);
+    once("mxfp4_linear");
     const auto layer = ctx->saved_data["layer"].toIntVector();
-    TORCH_CHECK(layer[0] == DIMQ_ACT_NONE, op, ": no gradient through its fused activation; apply the activation to the output "
+    TORCH_CHECK(layer[0] == DIMQ_ACT_NONE, "mxfp4_linear: no gradient through its fused activation; apply the activation to the output "
                 "of a call without one");
     auto type = [&](int i) { return static_cast<at::ScalarType>(layer[i]); };
     const auto saved = ctx->get_saved_variables();
@@ -747,12 +786,13 @@ Tensor mxfp4_linear_graph(const Tensor& x, const Tensor& codes, const Tensor& sc
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || (bias && bias->requires_grad()) || (residual && residual->requires_grad())))
     return MxPackedLinear::apply(x, bias, residual, codes, scales, activation, out_dtype);
-  return mxfp4_linear(x, codes, scales, bias, residual, activation, out_dtype);
+  return mxfp4_linear_below(x, codes, scales, bias, residual, activation, out_dtype);
 }
 
 // gelu(h), h kept in 8 bits for the backward pass.
 struct MxGelu : torch::autograd::Function<MxGelu> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, bool keep) {
+    untraced("mx.gelu");
     const Rows r(h, "gelu", "input");
     const int64_t nb = mx_blocks(r.cols);
     keep = keep && h.requires_grad();
@@ -765,6 +805,7 @@ struct MxGelu : torch::autograd::Function<MxGelu> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    untraced("mx.gelu");
     once("mx.gelu");
     const Tensor kept = ctx->get_saved_variables()[0];
     const Rows g(grads[0], "gelu", "gradient");
@@ -852,15 +893,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("separation_loss",
         [](const Tensor& w, const Tensor& c, double eta, double eps) { return SeparationLoss::apply(w, c, eta, eps); },
         Unlocked());
-  // the microscaled ops without the dispatcher, which takes 1 us of a call's 6
-  m.def("quantize_mxfp4", &quantize_mxfp4, Unlocked());
-  m.def("compress_activation", &compress_activation, Unlocked());
-  m.def("quantize_and_compress", &quantize_and_compress, Unlocked());
-  m.def("dequantize_mxfp4", &dequantize_mxfp4, Unlocked());
-  m.def("decompress_activation", &decompress_activation, Unlocked());
-  m.def("mxfp4_linear", &mxfp4_linear_graph, Unlocked());
-  m.def("mxfp4_linear_grad_input", &mxfp4_linear_grad_input, Unlocked());
-  m.def("linear_grad_weight", &linear_grad_weight, Unlocked());
+  // the microscaled operators past the dispatcher
+  m.def("quantize_mxfp4", Direct<&quantize_mxfp4>{"quantize_mxfp4"}, Unlocked());
+  m.def("compress_activation", Direct<&compress_activation>{"compress_activation"}, Unlocked());
+  m.def("quantize_and_compress", Direct<&quantize_and_compress>{"quantize_and_compress"}, Unlocked());
+  m.def("dequantize_mxfp4", Direct<&dequantize_mxfp4>{"dequantize_mxfp4"}, Unlocked());
+  m.def("decompress_activation", Direct<&decompress_activation>{"decompress_activation"}, Unlocked());
+  m.def("mxfp4_linear", Direct<&mxfp4_linear_graph>{"mxfp4_linear"}, Unlocked());
+  m.def("mxfp4_linear_grad_input", Direct<&mxfp4_linear_grad_input>{"mxfp4_linear_grad_input"}, Unlocked());
+  m.def("linear_grad_weight", Direct<&linear_grad_weight>{"linear_grad_weight"}, Unlocked());
   m.def("mx_linear",
         [](const Tensor& x, const Tensor& w, const OptTensor& b) { return MxLinear::apply(x, w, b, at::GradMode::is_enabled()); },
         Unlocked());

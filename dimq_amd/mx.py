@@ -10,7 +10,8 @@ infinity stands for NaN throughout.  ``Q4(x)`` and ``Q8(x)`` are the values that
 * Training: ``linear`` (``MXFP4TrainLinear``) runs that layer on the master weights with straight-through gradients and
   keeps its input in 8 bits for the weight gradient; ``gelu`` keeps its input in 8 bits too.
 
-All but ``linear`` and ``gelu`` are torch ops too (``torch.ops.dimq.quantize_mxfp4`` and so on).  All of it is for CUDA
+All but ``linear`` and ``gelu`` are torch ops too (``torch.ops.dimq.quantize_mxfp4`` and so on), which traces, dispatch
+modes and vmap see; those two, and gradients through a frozen layer, refuse to be traced.  All of it is for CUDA
 (HIP) tensors in fp32, fp16 and bf16; the gradients are those of the formulas in each function's
 description and have no gradients of their own.
 """
