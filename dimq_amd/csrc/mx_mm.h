@@ -13,10 +13,11 @@
 // bytes a lane into a ring of S slots; no register holds operands in flight and the main loop has no vector arithmetic.
 // C is the instructions' first operand, so a lane's accumulators are four neighbouring columns of one row.
 //
-// Measured: 16384 x 8192 codes summed over 8192 507 to 522 us (4,340 TFLOP/s); both bf16 gradients of 8192 x 4096 -> 4096
-// 209 and 203 us (1,315 and 1,354 TFLOP/s; the library's product of 8192^3 reaches 1,448 there).  Bound by the matrix unit, busy 59 %
-// (codes) and 70 % of the cycles, at the 1.7 GHz that the card holds under this load: without any load in the loop the same
-// data take 514 us of 520 and 187 of 204.
+// Measured: 16384 x 8192 codes summed over 8192 507 to 522 us (4,210 to 4,340 TFLOP/s); both bf16 gradients of
+// 8192 x 4096 -> 4096 209 and 203 us (1,315 and 1,354 TFLOP/s; the library's product of 8192^3 reaches 1,448 there).  The
+// matrix unit is busy 59 % (codes) and 70 % of the cycles, at the 1.7 GHz that the card holds under this load.  Not bound by
+// memory: without any load in the loop the same data take 514 us of 520 and 187 of 204.  How the rest divides among the LDS
+// reads, the barriers and scheduling fences of the steps and the epilogue is not known.
 #pragma once
 
 #include <type_traits>
@@ -478,8 +479,8 @@ __global__ __launch_bounds__(T::NT) void mx_mm_kernel(const MxMm p) {
   });
 }
 
-// The slices of a split reduction, [splits, rows, pitch] fp32, added in their order.  Bound by the bytes: four slices of
-// 2304 x 768 in 6.1 us, 5.8 TB/s.
+// The slices of a split reduction, [splits, rows, pitch] fp32, added in their order.  Two slices of 2304 x 768, 14 MB in and
+// 7 MB out, take 6.4 us, of which a launch that moves next to nothing takes 4 in the same trace.
 static __global__ __launch_bounds__(256) void mx_reduce_kernel(const float* part, int64_t slice, int splits, int64_t rows,
                                                                int64_t pitch, MxOut o) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;

@@ -72,7 +72,7 @@ __device__ __forceinline__ void turn_scales(const MxScaleTurn& t, uint32_t group
 
 // A lane takes eight elements, four lanes a block: loads of 16 bytes and stores of 4, 8 and 16 next to one another
 // across the wave, the block's maximum by two lane exchanges.  Bound by the bytes: 4096 x 4096 fp32 to both formats
-// moves 67 MB in and 26 MB out, 14.8 us or 6.3 TB/s.
+// moves 67 MB in and 26 MB out, 15.9 to 16.3 us or 5.8 TB/s.
 // TILED: the 4-bit output is a tiled product's operand; its scales go there in that order, to scales4 where that is given.
 template <int XT, bool Q4, bool Q8, bool GELU, bool TILED>
 __device__ __forceinline__ void quant_unit(const QuantArgs& a, const FastDiv& div, uint32_t u, uint32_t units) {
@@ -144,7 +144,7 @@ struct BackArgs {
 
 // Codes to values (SLOPE 0), or the upstream gradient times GELU's slope at them.  Eight elements a lane, as above.  Bound
 // by the bytes: 4096 x 4096 to fp32 15 and 16 us, 5.2 TB/s; GELU of 12608 x 2048 bf16 and its gradient, which move 130 MB
-// each in 23 to 27 us, also by 30 instructions an element.
+// each in 25 to 31 and 24 to 27 us, also by 30 instructions an element.
 template <int BITS, int YT, bool SLOPE>
 __global__ __launch_bounds__(256) void mx_back_kernel(BackArgs a, FastDiv div, uint32_t units) {
   const uint32_t u = (blockIdx.x * 256u + threadIdx.x) >> 2;
