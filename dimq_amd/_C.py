@@ -39,7 +39,7 @@ lib = ctypes.CDLL(str(_LIB_PATH))
 
 from . import _native  # noqa: E402  (after the library it links, and after torch)
 
-F32, F16, BF16, F64, U8 = 0, 1, 2, 3, 4
+F32, F16, BF16, F64, U8, E4M3 = 0, 1, 2, 3, 4, 5
 NCHW, NHWC = 0, 1
 VARIANT_AUTO, VARIANT_SMALL_M, VARIANT_MFMA = 0, 1, 2
 
@@ -142,6 +142,18 @@ _SIGS = {
                                           _vp]),
     "dimq_mx_gelu_forward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "dimq_mx_gelu_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "dimq_rms_norm": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _int, _dbl, _vp, _int, _vp, _vp, _vp]),
+    "dimq_rms_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "dimq_rms_norm_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _dbl, _vp, _int, _i64, _vp, _i64, _vp, _vp,
+                                      _int, _vp, _i64, _vp]),
+    "dimq_logits_workspace_bytes": (_i64, [_i64, _i64, _int]),
+    "dimq_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "dimq_token_logprobs_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _vp, _vp, _i64, _vp, _i64, _vp,
+                                            _vp]),
+    "dimq_distill_loss": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _int, _i64, _dbl, _int, _vp, _vp, _vp, _vp,
+                                 _vp, _vp, _i64, _vp]),
+    "dimq_distill_loss_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp, _dbl, _vp, _i64, _vp, _vp,
+                                          _vp]),
     "dimq_separation_loss": (_int, [_vp, _int, _i64, _vp, _i64, _dbl, _dbl, _vp, _vp, _vp, _i64, _vp]),
 }
 

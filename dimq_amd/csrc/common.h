@@ -34,6 +34,7 @@ inline int dtype_size(int dt) {
     case DIMQ_BF16: return 2;
     case DIMQ_F64: return 8;
     case DIMQ_U8: return 1;
+    case DIMQ_E4M3: return 1;
   }
   return 0;
 }

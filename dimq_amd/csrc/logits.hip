@@ -1,0 +1,735 @@
+// Rows of logits x: log probabilities of given tokens, entropy and the largest alternatives, the distillation loss of a
+// teacher's top logits, and the gradients of both.
+//
+//   m = max x, s = sum exp(x - m), u = sum exp(x - m) (x - m)            one pass, kept as a running (m, s, u)
+//   lse = m + log s,  log p = x - lse,  entropy = -sum p log p = log s - u / s
+//
+// A row that holds a NaN or +infinity, or nothing above -infinity, has no distribution: its values are NaN and its
+// alternatives' tokens -1.  -infinity in a row has p = 0 and adds nothing; the type's lowest finite number is a number.
+//
+// Alternatives, in the same pass: of each thread's running maxima (256 to a work-group) the k-th largest is a lower bound of
+// the k-th largest logit, and only the threads whose maximum reaches it, little more than k of them, read their logits
+// again and hand on those that reach it.  Those few are ranked by counting.  Equal logits rank by token, lower first.
+//
+// Bound by bytes: a row is read once (the gradients read it once more and write theirs).  A row is cut over several
+// work-groups where there are few of them; a second launch then joins their (m, s, u) and candidates.
+#include "common.h"
+#include "rows.h"
+
+namespace dimq {
+namespace {
+
+constexpr int kLgThreads = 256;
+constexpr int kLgCand = 1024;      // candidates a work-group holds: more fall back to one pass per alternative
+constexpr int kLgTop = 128;        // most alternatives
+constexpr int kLgSplits = 32;      // most work-groups to a row
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;
+
+struct LogitArgs {
+  const void* x;
+  int64_t ldx, rows, V;
+  int splits;
+  int64_t chunk;  // elements of a split, a multiple of 8
+  float tau_inv;  // distillation: 1 / temperature
+  // scoring
+  const void* tokens;
+  int tokens64;
+  int top;
+  float* logp;
+  float* entropy;
+  float* norm;     // [rows][2] m and log s, kept for the gradients (the pair: a large lse alone would lose digits)
+  float* top_logp;
+  int64_t* top_ids;
+  // distillation
+  const void* values;
+  int values_dt;
+  const void* ids;
+  int ids64;
+  int k;
+  float* loss;     // [rows]
+  float* p;        // [rows][k] the teacher's probabilities
+  // partial results of splits
+  float* stats;    // [rows][splits][4]: m, s, u
+  uint64_t* cand;  // [rows][splits][top]
+};
+
+struct Stats {
+  float m, s, u;
+};
+
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// (m, s, u) with the maximum raised to m: s and u are sums of exp(x - m) and exp(x - m) (x - m).  The difference is held
+// above -200, whose exponential is 0, so that no 0 * infinity arises.
+template <bool U>
+__device__ __forceinline__ void raise(Stats& a, float m, float scale) {
+  const float d = fmaxf(a.m - m, -200.0f / scale), e = exp_of(d * scale);
+  if constexpr (U) a.u = e * fmaf(a.s, d, a.u);
+  a.s *= e;
+  a.m = m;
+}
+
+// Over the wave or over `n` entries: every lane's to the common maximum, then plain sums.
+template <bool U>
+__device__ __forceinline__ Stats block_stats(Stats a, float scale, float (*red)[4]) {
+  const float m = row_reduce<kLgThreads, true>(a.m, red[0]);
+  raise<U>(a, m, scale);
+  a.s = row_reduce<kLgThreads>(a.s, red[1]);
+  if constexpr (U) a.u = row_reduce<kLgThreads>(a.u, red[2]);
+  return a;
+}
+
+// Order of the logits as unsigned numbers, NaN above all, -0 equal to 0; 0 is below every logit.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 + 0 = 0
+  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_order(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// Unique keys: the larger logit first, then the lower token.
+__device__ __forceinline__ uint64_t key_of(float v, int64_t at) {
+  return static_cast<uint64_t>(order_of(v)) << 32 | (0xffffffffu - static_cast<uint32_t>(at));
+}
+
+template <int XT>
+__device__ __forceinline__ float logit(const void* row, int64_t i) {
+  return load_as_float(row, XT, i);
+}
+
+template <int XT>
+constexpr int pack_of() {
+  return XT == DIMQ_F32 ? 4 : 8;
+}
+
+// 16 aligned bytes of a row as floats.
+template <int XT>
+__device__ __forceinline__ void unpack16(const uint4& t, float (&v)[pack_of<XT>()]) {
+  const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+  if constexpr (XT == DIMQ_F32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = XT == DIMQ_F16 ? f16_bits_to_float(w[j] & 0xffffu) : bf16_bits_to_float(w[j] & 0xffffu);
+      v[2 * j + 1] = XT == DIMQ_F16 ? f16_bits_to_float(w[j] >> 16) : bf16_bits_to_float(w[j] >> 16);
+    }
+  }
+}
+
+// Elements [a, b) of a row in three parts: single ones up to the first 16-byte boundary, whole 16-byte pieces, the rest.
+struct Span {
+  int64_t a, body, b;  // body: first element of the pieces
+  int64_t pieces;
+  template <int XT>
+  __device__ __forceinline__ static Span of(const void* row, int64_t a, int64_t b) {
+    constexpr int kSize = XT == DIMQ_F32 ? 4 : 2;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row) + a * kSize;
+    int64_t head = static_cast<int64_t>((16 - (at & 15)) & 15) / kSize;
+    if (head > b - a) head = b - a;
+    return {a, a + head, b, (b - a - head) / pack_of<XT>()};
+  }
+  __device__ __forceinline__ int singles(int pack) const {
+    return static_cast<int>((body - a) + (b - body - pieces * pack));
+  }
+  __device__ __forceinline__ int64_t single(int i, int pack) const {
+    return i < body - a ? a + i : body + pieces * pack + (i - (body - a));
+  }
+};
+
+template <int N, bool U>
+__device__ __forceinline__ void add_to(Stats& st, const float (&v)[N], float scale) {
+  float cm = v[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) cm = fmaxf(cm, v[j]);
+  if (cm > st.m) raise<U>(st, cm, scale);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float d = v[j] - st.m, e = exp_of(d * scale);
+    st.s += e;
+    if constexpr (U) st.u = fmaf(e, fmaxf(d, -200.0f), st.u);
+  }
+}
+
+// The calling thread's part of [a, b): pieces tid, tid + 256, ..., and one of the single elements.
+template <int XT, bool U>
+__device__ __forceinline__ Stats stream_stats(const void* row, const Span& sp, float scale) {
+  constexpr int P = pack_of<XT>();
+  Stats st{kLowest, 0.0f, 0.0f};
+  const uint4* body = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + sp.body * (16 / P));
+  int64_t i = threadIdx.x;
+  for (; i + 3 * kLgThreads < sp.pieces; i += 4 * kLgThreads) {
+    uint4 t[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[q] = body[i + q * kLgThreads];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float v[P];
+      unpack16<XT>(t[q], v);
+      add_to<P, U>(st, v, scale);
+    }
+  }
+  for (; i < sp.pieces; i += kLgThreads) {
+    float v[P];
+    unpack16<XT>(body[i], v);
+    add_to<P, U>(st, v, scale);
+  }
+  if (static_cast<int>(threadIdx.x) < sp.singles(P)) {
+    const float v[1] = {logit<XT>(row, sp.single(threadIdx.x, P))};
+    add_to<1, U>(st, v, scale);
+  }
+  return st;
+}
+
+// Calls f(element, index) for the calling thread's part, as stream_stats goes through it.
+template <int XT, class F>
+__device__ __forceinline__ void each_of_mine(const void* row, const Span& sp, F f) {
+  constexpr int P = pack_of<XT>();
+  const uint4* body = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + sp.body * (16 / P));
+  for (int64_t i = threadIdx.x; i < sp.pieces; i += kLgThreads) {
+    float v[P];
+    unpack16<XT>(body[i], v);
+#pragma unroll
+    for (int j = 0; j < P; ++j) f(v[j], sp.body + i * P + j);
+  }
+  if (static_cast<int>(threadIdx.x) < sp.singles(P)) {
+    const int64_t at = sp.single(threadIdx.x, P);
+    f(logit<XT>(row, at), at);
+  }
+}
+
+struct TopShared {
+  alignas(16) uint32_t maxima[kLgThreads];
+  uint8_t owners[kLgThreads];
+  uint64_t cand[kLgCand];
+  int count, nowners;
+  uint32_t bound;
+};
+
+// Ranks n unique keys and writes the first `top`, in order, to out(rank, key); with fewer the rest are out(rank, 0).
+template <class Out>
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int top, Out out) {
+  for (int c = threadIdx.x; c < n; c += kLgThreads) {
+    const uint64_t key = keys[c];
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += keys[i] > key;
+    if (rank < top) out(rank, key);
+  }
+  for (int r = n + threadIdx.x; r < top; r += kLgThreads) out(r, 0);
+}
+
+// The `top` largest keys of the work-group's span.  `mine`: the largest order_of() of the thread's elements (0: none).
+template <int XT, class Out>
+__device__ __forceinline__ void span_top(const void* row, const Span& sp, uint32_t mine, int top, TopShared& sh, Out out) {
+  sh.maxima[threadIdx.x] = mine;
+  if (threadIdx.x == 0) sh.count = 0, sh.nowners = 0;
+  __syncthreads();
+  // the top-th largest of the 256 maxima: the thread with top - 1 others before it
+  int before = 0;
+  for (int i = 0; i < kLgThreads; i += 4) {
+    const uint4 o = *reinterpret_cast<const uint4*>(&sh.maxima[i]);
+    const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) before += w[j] > mine || (w[j] == mine && i + j < static_cast<int>(threadIdx.x));
+  }
+  if (before == top - 1) sh.bound = mine;
+  __syncthreads();
+  const uint32_t bound = sh.bound;
+  if (mine >= bound) sh.owners[atomicAdd(&sh.nowners, 1)] = static_cast<uint8_t>(threadIdx.x);
+  __syncthreads();
+  // the owners' elements once more, shared out over the whole work-group so that their loads go out together
+  constexpr int P = pack_of<XT>();
+  const int no = sh.nowners;
+  const int items = no * static_cast<int>((sp.pieces + kLgThreads - 1) / kLgThreads);  // at most 2^29 + 2^8
+  const uint4* body = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + sp.body * (16 / P));
+  auto test = [&](float v, int64_t at) {
+    if (order_of(v) < bound) return;
+    const int i = atomicAdd(&sh.count, 1);
+    if (i < kLgCand) sh.cand[i] = key_of(v, at);
+  };
+  for (int base = threadIdx.x; base < items; base += 4 * kLgThreads) {
+    uint4 t[4];
+    int64_t at[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int item = base + q * kLgThreads;
+      const int64_t i = item < items ? sh.owners[item % no] + item / no * static_cast<int64_t>(kLgThreads) : sp.pieces;
+      at[q] = i < sp.pieces ? i : -1;
+      t[q] = body[at[q] < 0 ? 0 : at[q]];  // there is a piece: items > 0
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (at[q] < 0) continue;
+      float v[P];
+      unpack16<XT>(t[q], v);
+#pragma unroll
+      for (int j = 0; j < P; ++j) test(v[j], sp.body + at[q] * P + j);
+    }
+  }
+  if (static_cast<int>(threadIdx.x) < sp.singles(P)) {
+    const int64_t at = sp.single(threadIdx.x, P);
+    test(logit<XT>(row, at), at);
+  }
+  __syncthreads();
+  const int n = sh.count;
+  if (n <= kLgCand) {  // the order of the list does not matter: its keys are ranked
+    rank_keys(sh.cand, n, top, out);
+    return;
+  }
+  // many equal to the bound: one pass for each alternative, the largest key below the last
+  uint64_t last = ~0ull;
+  for (int r = 0; r < top; ++r) {
+    uint64_t best = 0;
+    if (mine >= bound) {
+      each_of_mine<XT>(row, sp, [&](float v, int64_t at) {
+        const uint64_t key = key_of(v, at);
+        if (key < last && key > best) best = key;
+      });
+    }
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) {
+      const uint64_t o = __shfl_xor(best, s, 64);
+      best = o > best ? o : best;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.cand[threadIdx.x >> 6] = best;
+    __syncthreads();
+    for (int w = 0; w < kLgThreads / 64; ++w) best = sh.cand[w] > best ? sh.cand[w] : best;
+    last = best;
+    if (threadIdx.x == 0) out(r, best);
+  }
+}
+
+__device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
+  return is64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+__device__ __forceinline__ float nan32() { return __uint_as_float(0x7fc00000u); }
+
+// Whether (m, s) is a distribution's: no NaN, no +infinity, something above -infinity.
+__device__ __forceinline__ bool proper(const Stats& st) { return st.s > 0.0f && st.s < __uint_as_float(0x7f800000u); }
+
+template <int XT>
+__device__ __forceinline__ void finish_score(const LogitArgs& a, int64_t row, const void* xr, const Stats& st) {
+  if (threadIdx.x != 0) return;
+  const bool ok = proper(st);
+  const float ls = ok ? logf(st.s) : nan32();
+  const int64_t token = index_at(a.tokens, a.tokens64, row);
+  a.logp[row] = token < 0 ? 0.0f : ok && token < a.V ? (logit<XT>(xr, token) - st.m) - ls : nan32();
+  a.entropy[row] = ok ? ls - st.u / st.s : nan32();
+  if (a.norm) a.norm[2 * row] = st.m, a.norm[2 * row + 1] = ls;
+}
+
+__device__ __forceinline__ void put_top(const LogitArgs& a, int64_t row, int r, uint64_t key, const Stats& st, bool ok) {
+  const float v = of_order(static_cast<uint32_t>(key >> 32));
+  a.top_logp[row * a.top + r] = ok ? (v - st.m) - logf(st.s) : nan32();
+  a.top_ids[row * a.top + r] = ok ? static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key)) : -1;
+}
+
+// Whether a teacher entry counts: its token is given and its value is not -infinity.
+__device__ __forceinline__ bool kept(int64_t id, float value) { return id >= 0 && value != __uint_as_float(0xff800000u); }
+
+// The teacher's softmax over a row's kept entries, and the row's loss.
+template <int XT>
+__device__ __forceinline__ void finish_distill(const LogitArgs& a, int64_t row, const void* xr, const Stats& st, float (*red)[4]) {
+  const float ls = logf(st.s), tau = 1.0f / a.tau_inv;
+  float m = kLowest, some = 0.0f;
+  for (int j = threadIdx.x; j < a.k; j += kLgThreads) {
+    const float v = load_as_float(a.values, a.values_dt, row * a.k + j);
+    if (!kept(index_at(a.ids, a.ids64, row * a.k + j), v)) continue;
+    m = fmaxf(m, v);
+    some = 1.0f;
+  }
+  __syncthreads();
+  m = row_reduce<kLgThreads, true>(m, red[0]);
+  some = row_reduce<kLgThreads, true>(some, red[1]);
+  float s = 0.0f;
+  for (int j = threadIdx.x; j < a.k; j += kLgThreads) {
+    const float v = load_as_float(a.values, a.values_dt, row * a.k + j);
+    if (kept(index_at(a.ids, a.ids64, row * a.k + j), v)) s += exp_of((v - m) * a.tau_inv);
+  }
+  s = row_reduce<kLgThreads>(s, red[2]);
+  const float lt = logf(s);
+  float loss = 0.0f;
+  for (int j = threadIdx.x; j < a.k; j += kLgThreads) {
+    const int64_t id = index_at(a.ids, a.ids64, row * a.k + j);
+    const float v = load_as_float(a.values, a.values_dt, row * a.k + j);
+    float p = 0.0f;
+    if (kept(id, v)) {
+      const float lp = (v - m) * a.tau_inv - lt;
+      p = exp_of(lp);
+      const float lq = id < a.V ? (logit<XT>(xr, id) - st.m) * a.tau_inv - ls : nan32();
+      if (p != 0.0f) loss += p * (lp - lq);
+    }
+    a.p[row * a.k + j] = p;
+  }
+  __syncthreads();
+  loss = row_reduce<kLgThreads>(loss, red[0]);
+  if (threadIdx.x == 0) {
+    // a row without entries has no loss, whatever its logits: log s of +infinity marks it.  One whose loss is NaN (its
+    // logits', its values' or a token's beyond the vocabulary) has NaN gradients.
+    if (!proper(st)) loss = nan32();
+    a.loss[row] = some == 0.0f ? 0.0f : loss * tau * tau;
+    a.norm[2 * row] = st.m;
+    a.norm[2 * row + 1] = some == 0.0f ? __uint_as_float(0x7f800000u) : loss == loss ? ls : nan32();
+  }
+}
+
+// One split of one row: grid (splits, rows).
+template <int XT, bool DISTILL>
+__global__ __launch_bounds__(kLgThreads) void logits_kernel(const LogitArgs a) {
+  __shared__ float red[3][4];
+  __shared__ TopShared sh;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const char* xr = static_cast<const char*>(a.x) + row * a.ldx * (XT == DIMQ_F32 ? 4 : 2);
+    const int64_t from = blockIdx.x * a.chunk, to = from + a.chunk < a.V ? from + a.chunk : a.V;
+    const Span sp = Span::of<XT>(xr, from, to);
+    const float scale = DISTILL ? a.tau_inv : 1.0f;
+    const Stats mine = stream_stats<XT, !DISTILL>(xr, sp, scale);
+    const Stats st = block_stats<!DISTILL>(mine, scale, red);
+    if (a.splits > 1) {
+      if (threadIdx.x == 0) {
+        float* to_stats = a.stats + (row * a.splits + blockIdx.x) * 4;
+        to_stats[0] = st.m, to_stats[1] = st.s, to_stats[2] = st.u;
+      }
+    } else if constexpr (DISTILL) {
+      finish_distill<XT>(a, row, xr, st, red);
+    } else {
+      finish_score<XT>(a, row, xr, st);
+    }
+    if constexpr (!DISTILL) {
+      if (a.top > 0) {
+        // the thread's maximum, 0 where it saw nothing above -infinity: a lower bound needs no more, but with fewer than
+        // `top` such threads every element is a candidate
+        const uint32_t m = mine.s > 0.0f ? order_of(mine.m) : 1u;
+        uint64_t* cand = a.cand + (row * a.splits + blockIdx.x) * a.top;
+        const bool ok = proper(st);
+        if (a.splits > 1) {
+          span_top<XT>(xr, sp, m, a.top, sh, [&](int r, uint64_t key) { cand[r] = key; });
+        } else if (ok) {
+          span_top<XT>(xr, sp, m, a.top, sh, [&](int r, uint64_t key) { put_top(a, row, r, key, st, true); });
+        } else {
+          for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, st, false);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the splits of a row.
+template <int XT, bool DISTILL>
+__global__ __launch_bounds__(kLgThreads) void logits_join_kernel(const LogitArgs a) {
+  __shared__ float red[3][4];
+  __shared__ uint64_t keys[DISTILL ? 1 : kLgSplits * kLgTop];
+  const int64_t row = blockIdx.x;
+  const char* xr = static_cast<const char*>(a.x) + row * a.ldx * (XT == DIMQ_F32 ? 4 : 2);
+  Stats st{kLowest, 0.0f, 0.0f};
+  if (static_cast<int>(threadIdx.x) < a.splits) {
+    const float* from = a.stats + (row * a.splits + threadIdx.x) * 4;
+    st = {from[0], from[1], from[2]};
+  }
+  st = block_stats<!DISTILL>(st, DISTILL ? a.tau_inv : 1.0f, red);
+  if constexpr (DISTILL) {
+    finish_distill<XT>(a, row, xr, st, red);
+  } else {
+    finish_score<XT>(a, row, xr, st);
+    if (a.top > 0) {
+      const int n = a.splits * a.top;
+      for (int i = threadIdx.x; i < n; i += kLgThreads) keys[i] = a.cand[row * n + i];
+      __syncthreads();
+      const bool ok = proper(st);
+      if (ok) rank_keys(keys, n, a.top, [&](int r, uint64_t key) { put_top(a, row, r, key, st, true); });
+      else
+        for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, st, false);
+    }
+  }
+}
+
+// The sum of the rows' losses, or their mean over the rows that keep an entry (0 without any), and what that divides by.  One work-group, a fixed order.
+__global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ loss, const float* __restrict__ norm,
+                                                           int64_t rows, int mean, float* out, float* divisor) {
+  __shared__ float red[2][16];
+  float s = 0.0f, n = 0.0f;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+    s += loss[i];
+    n += norm[2 * i + 1] != __uint_as_float(0x7f800000u) ? 1.0f : 0.0f;
+  }
+  s = row_reduce<1024>(s, red[0]);
+  n = row_reduce<1024>(n, red[1]);
+  if (threadIdx.x == 0) {
+    const float by = mean ? fmaxf(n, 1.0f) : 1.0f;
+    out[0] = s / by;
+    divisor[0] = by;
+  }
+}
+
+struct GradArgs {
+  const void* x;
+  int64_t ldx, rows, V, chunk;
+  const float* norm;
+  void* gx;
+  // scoring
+  const void* tokens;
+  int tokens64;
+  const float* entropy;
+  const float* ga;  // [rows], nullable; strides 0 or 1
+  const float* gb;
+  int64_t sa, sb;
+  // distillation
+  float tau, tau_inv;
+  const void* ids;
+  int ids64;
+  int k;
+  const float* p;
+  const float* by;  // nullable
+};
+
+// grid (chunks, rows): the gradient of one chunk of a row.
+//   scoring        a ([v = token] - p) - b p (log p + H)
+//   distillation   tau c (q - p_teacher), the teacher's entries subtracted after the chunk is written
+template <int XT, bool DISTILL>
+__global__ __launch_bounds__(kLgThreads) void logits_grad_kernel(const GradArgs a) {
+  constexpr int P = pack_of<XT>(), kSize = XT == DIMQ_F32 ? 4 : 2;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const char* xr = static_cast<const char*>(a.x) + row * a.ldx * kSize;
+    char* gr = static_cast<char*>(a.gx) + row * a.V * kSize;
+    const int64_t from = blockIdx.x * a.chunk, to = from + a.chunk < a.V ? from + a.chunk : a.V;
+    const float m = a.norm[2 * row], ls = a.norm[2 * row + 1];
+    float ca = a.ga ? a.ga[row * a.sa] : 0.0f, cb = 0.0f, H = 0.0f;
+    int64_t token = -1;
+    bool none;  // nothing reaches this row, whatever it holds
+    if constexpr (DISTILL) {
+      ca *= a.tau / (a.by ? a.by[0] : 1.0f);
+      none = ls == __uint_as_float(0x7f800000u) || ca == 0.0f;
+    } else {
+      token = index_at(a.tokens, a.tokens64, row);
+      if (token < 0) ca = 0.0f;
+      cb = a.gb ? a.gb[row * a.sb] : 0.0f;
+      none = ca == 0.0f && cb == 0.0f;
+      H = a.entropy[row];
+      if (cb == 0.0f) H = 0.0f;
+      if (token >= a.V && ca != 0.0f) ca = nan32();
+    }
+    auto grad = [&](float x, int64_t at) {
+      float g;
+      if constexpr (DISTILL) {
+        g = ca * exp_of(fmaf(x - m, a.tau_inv, -ls));
+      } else {
+        const float lp = (x - m) - ls, p = exp_of(lp);
+        const float t = fmaf(cb, fmaxf(lp, -200.0f) + H, ca);  // p = 0: no 0 * infinity
+        g = (at == token ? ca : 0.0f) - p * t;
+      }
+      return none ? 0.0f : g;
+    };
+    Span sp = Span::of<XT>(xr, from, to);
+    // pieces are written whole only where both rows reach a 16-byte boundary together
+    if (((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(gr)) & 15) != 0) {
+      for (int64_t i = from + threadIdx.x; i < to; i += kLgThreads)
+        store_from_float(gr, XT, i, grad(logit<XT>(xr, i), i));
+    } else {
+      const uint4* body = reinterpret_cast<const uint4*>(xr + sp.body * kSize);
+      uint4* out = reinterpret_cast<uint4*>(gr + sp.body * kSize);
+      auto put = [&](int64_t i, const uint4& t) {
+        float v[P];
+        unpack16<XT>(t, v);
+#pragma unroll
+        for (int j = 0; j < P; ++j) v[j] = grad(v[j], sp.body + i * P + j);
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (XT == DIMQ_F32) o[j] = __float_as_uint(v[j]);
+          else o[j] = XT == DIMQ_F16 ? f16x2_rne(v[2 * j], v[2 * j + 1]) : bf16x2_rne(v[2 * j], v[2 * j + 1]);
+        }
+        out[i] = make_uint4(o[0], o[1], o[2], o[3]);
+      };
+      int64_t i = threadIdx.x;
+      for (; i + 3 * kLgThreads < sp.pieces; i += 4 * kLgThreads) {
+        uint4 t[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) t[q] = body[i + q * kLgThreads];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) put(i + q * kLgThreads, t[q]);
+      }
+      for (; i < sp.pieces; i += kLgThreads) put(i, body[i]);
+      if (static_cast<int>(threadIdx.x) < sp.singles(P)) {
+        const int64_t at = sp.single(threadIdx.x, P);
+        store_from_float(gr, XT, at, grad(logit<XT>(xr, at), at));
+      }
+    }
+    if constexpr (DISTILL) {
+      if (none) continue;
+      __syncthreads();  // the chunk is written before its entries are written again
+      for (int j = threadIdx.x; j < a.k; j += kLgThreads) {
+        const int64_t id = index_at(a.ids, a.ids64, row * a.k + j);
+        if (id < from || id >= to) continue;
+        // the first of equal tokens takes all of their probability
+        bool first = true;
+        float p = 0.0f;
+        for (int i = 0; i < a.k; ++i) {
+          if (index_at(a.ids, a.ids64, row * a.k + i) != id) continue;
+          if (i < j) first = false;
+          p += a.p[row * a.k + i];
+        }
+        if (first) store_from_float(gr, XT, id, ca * (exp_of(fmaf(logit<XT>(xr, id) - m, a.tau_inv, -ls)) - p));
+      }
+    }
+  }
+}
+
+// Splits of a row: one where the rows alone fill the chip (four work-groups a CU), else as many as do, of at least 4,096
+// elements.
+int row_splits(int64_t rows, int64_t V) {
+  const int64_t want = (4 * static_cast<int64_t>(device_cus()) + rows - 1) / rows, most = (V + 4095) / 4096;
+  const int64_t n = want < most ? want : most;
+  return static_cast<int>(n < 1 ? 1 : n > kLgSplits ? kLgSplits : n);
+}
+int64_t split_chunk(int64_t V, int splits) { return ((V + splits - 1) / splits + 7) / 8 * 8; }
+
+int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
+
+bool float_logits(int dt) { return dt == DIMQ_F32 || dt == DIMQ_F16 || dt == DIMQ_BF16; }
+
+int check_logits(const char* what, const void* x, int dtype, int64_t rows, int64_t V, int64_t ldx) {
+  DIMQ_CHECK(float_logits(dtype), "%s: logits must be fp32, fp16 or bf16", what);
+  DIMQ_CHECK(rows >= 0 && V > 0, "%s: there must be at least one logit a row", what);
+  DIMQ_CHECK(V < (int64_t)1 << 31, "%s: rows of 2^31 logits or more are not supported", what);
+  DIMQ_CHECK(rows <= 1 || ldx >= V, "%s: row stride is below the row length", what);
+  DIMQ_CHECK(rows == 0 || x, "%s: null pointer", what);
+  return DIMQ_OK;
+}
+
+template <bool DISTILL>
+int launch_rows(const LogitArgs& a, int dtype, hipStream_t s) {
+  // a grid's second dimension ends at 65,535: more rows are taken in turn
+  const dim3 grid(a.splits, static_cast<unsigned>(a.rows < 65535 ? a.rows : 65535));
+  switch (dtype) {
+    case DIMQ_F32: hipLaunchKernelGGL((logits_kernel<DIMQ_F32, DISTILL>), grid, dim3(kLgThreads), 0, s, a); break;
+    case DIMQ_F16: hipLaunchKernelGGL((logits_kernel<DIMQ_F16, DISTILL>), grid, dim3(kLgThreads), 0, s, a); break;
+    default: hipLaunchKernelGGL((logits_kernel<DIMQ_BF16, DISTILL>), grid, dim3(kLgThreads), 0, s, a);
+  }
+  if (a.splits > 1) {
+    const dim3 one(static_cast<unsigned>(a.rows));
+    switch (dtype) {
+      case DIMQ_F32: hipLaunchKernelGGL((logits_join_kernel<DIMQ_F32, DISTILL>), one, dim3(kLgThreads), 0, s, a); break;
+      case DIMQ_F16: hipLaunchKernelGGL((logits_join_kernel<DIMQ_F16, DISTILL>), one, dim3(kLgThreads), 0, s, a); break;
+      default: hipLaunchKernelGGL((logits_join_kernel<DIMQ_BF16, DISTILL>), one, dim3(kLgThreads), 0, s, a);
+    }
+  }
+  return check_launch(DISTILL ? "top_logits_distillation_loss" : "token_logprobs");
+}
+
+template <bool DISTILL>
+int launch_grad(GradArgs& a, int dtype, hipStream_t s) {
+  // chunks of at least 8,192 elements, and enough of them for four work-groups a CU
+  const int64_t want = (4 * static_cast<int64_t>(device_cus()) + a.rows - 1) / a.rows, most = (a.V + 8191) / 8192;
+  const int64_t n = want < 1 ? 1 : want < most ? want : most;
+  a.chunk = split_chunk(a.V, static_cast<int>(n));
+  const dim3 grid(static_cast<unsigned>((a.V + a.chunk - 1) / a.chunk), static_cast<unsigned>(a.rows < 65535 ? a.rows : 65535));
+  switch (dtype) {
+    case DIMQ_F32: hipLaunchKernelGGL((logits_grad_kernel<DIMQ_F32, DISTILL>), grid, dim3(kLgThreads), 0, s, a); break;
+    case DIMQ_F16: hipLaunchKernelGGL((logits_grad_kernel<DIMQ_F16, DISTILL>), grid, dim3(kLgThreads), 0, s, a); break;
+    default: hipLaunchKernelGGL((logits_grad_kernel<DIMQ_BF16, DISTILL>), grid, dim3(kLgThreads), 0, s, a);
+  }
+  return check_launch(DISTILL ? "top_logits_distillation_loss backward" : "token_logprobs backward");
+}
+
+}  // namespace
+}  // namespace dimq
+
+using namespace dimq;
+
+extern "C" int64_t dimq_logits_workspace_bytes(int64_t rows, int64_t vocab, int top) {
+  if (rows <= 0 || vocab <= 0 || top < 0) return 0;
+  const int splits = row_splits(rows, vocab);
+  return splits == 1 ? 0 : up16(rows * splits * 16) + up16(rows * splits * static_cast<int64_t>(top) * 8);
+}
+
+extern "C" int dimq_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ldx, const void* tokens,
+                                   int tokens64, int top, float* logprobs, float* entropy, float* norm, float* top_logprobs,
+                                   int64_t* top_ids, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_logits("token_logprobs", logits, dtype, rows, vocab, ldx);
+  if (rc != DIMQ_OK) return rc;
+  DIMQ_CHECK(top >= 0 && top <= kLgTop && top <= vocab, "token_logprobs: top must be in [0, %d] and not above the vocabulary",
+             kLgTop);
+  if (rows == 0) return DIMQ_OK;
+  DIMQ_CHECK(tokens && logprobs && entropy && (top == 0 || (top_logprobs && top_ids)), "token_logprobs: null pointer");
+  DIMQ_CHECK(workspace_bytes >= dimq_logits_workspace_bytes(rows, vocab, top) && aligned(workspace, 16),
+             "token_logprobs: the workspace is too small or not 16-byte aligned");
+  LogitArgs a{};
+  a.x = logits, a.ldx = ldx, a.rows = rows, a.V = vocab;
+  a.splits = row_splits(rows, vocab);
+  a.chunk = split_chunk(vocab, a.splits);
+  a.tau_inv = 1.0f, a.tokens = tokens, a.tokens64 = tokens64, a.top = top;
+  a.logp = logprobs, a.entropy = entropy, a.norm = norm, a.top_logp = top_logprobs, a.top_ids = top_ids;
+  a.stats = static_cast<float*>(workspace);
+  a.cand = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + up16(rows * a.splits * 16));
+  return launch_rows<false>(a, dtype, as_stream(stream));
+}
+
+extern "C" int dimq_token_logprobs_backward(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ldx,
+                                            const void* tokens, int tokens64, const float* norm, const float* entropy,
+                                            const float* grad_logprobs, int64_t stride_logprobs, const float* grad_entropy,
+                                            int64_t stride_entropy, void* grad_logits, void* stream) {
+  const int rc = check_logits("token_logprobs backward", logits, dtype, rows, vocab, ldx);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0) return DIMQ_OK;
+  DIMQ_CHECK(tokens && norm && entropy && grad_logits, "token_logprobs backward: null pointer");
+  GradArgs a{};
+  a.x = logits, a.ldx = ldx, a.rows = rows, a.V = vocab, a.norm = norm, a.gx = grad_logits;
+  a.tokens = tokens, a.tokens64 = tokens64, a.entropy = entropy;
+  a.ga = grad_logprobs, a.sa = stride_logprobs, a.gb = grad_entropy, a.sb = stride_entropy;
+  return launch_grad<false>(a, dtype, as_stream(stream));
+}
+
+extern "C" int dimq_distill_loss(const void* student, int dtype, int64_t rows, int64_t vocab, int64_t ldx, const void* values,
+                                 int values_dtype, const void* ids, int ids64, int64_t k, double temperature, int reduction,
+                                 float* row_loss, float* loss, float* divisor, float* norm, float* p,
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_logits("top_logits_distillation_loss", student, dtype, rows, vocab, ldx);
+  if (rc != DIMQ_OK) return rc;
+  DIMQ_CHECK(float_logits(values_dtype), "top_logits_distillation_loss: teacher values must be fp32, fp16 or bf16");
+  DIMQ_CHECK(k >= 0 && k < 1 << 20, "top_logits_distillation_loss: at most 2^20 teacher entries a row");
+  DIMQ_CHECK(temperature >= 1e-30 && temperature <= 1e30,
+             "top_logits_distillation_loss: the temperature must be in [1e-30, 1e30]");
+  DIMQ_CHECK(reduction >= 0 && reduction <= 2, "top_logits_distillation_loss: unknown reduction");
+  const hipStream_t s = as_stream(stream);
+  if (rows > 0) {
+    DIMQ_CHECK(row_loss && norm && (k == 0 || (values && ids && p)), "top_logits_distillation_loss: null pointer");
+    DIMQ_CHECK(workspace_bytes >= dimq_logits_workspace_bytes(rows, vocab, 0) && aligned(workspace, 16),
+               "top_logits_distillation_loss: the workspace is too small or not 16-byte aligned");
+    LogitArgs a{};
+    a.x = student, a.ldx = ldx, a.rows = rows, a.V = vocab;
+    a.splits = row_splits(rows, vocab);
+    a.chunk = split_chunk(vocab, a.splits);
+    a.tau_inv = static_cast<float>(1.0 / temperature);
+    a.values = values, a.values_dt = values_dtype, a.ids = ids, a.ids64 = ids64, a.k = static_cast<int>(k);
+    a.loss = row_loss, a.norm = norm, a.p = p, a.stats = static_cast<float*>(workspace);
+    const int r = launch_rows<true>(a, dtype, s);
+    if (r != DIMQ_OK) return r;
+  }
+  if (reduction != 0) {
+    DIMQ_CHECK(loss && divisor, "top_logits_distillation_loss: null pointer");
+    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, row_loss, norm, rows, reduction == 1, loss, divisor);
+  }
+  return check_launch("top_logits_distillation_loss");
+}
+
+extern "C" int dimq_distill_loss_backward(const void* student, int dtype, int64_t rows, int64_t vocab, int64_t ldx,
+                                          const void* ids, int ids64, int64_t k, const float* p, const float* norm,
+                                          double temperature, const float* grad, int64_t grad_stride, const float* divisor,
+                                          void* grad_student, void* stream) {
+  const int rc = check_logits("top_logits_distillation_loss backward", student, dtype, rows, vocab, ldx);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0) return DIMQ_OK;
+  DIMQ_CHECK(k >= 0 && k < 1 << 20 && (k == 0 || (ids && p)) && norm && grad && grad_student,
+             "top_logits_distillation_loss backward: null pointer");
+  GradArgs a{};
+  a.x = student, a.ldx = ldx, a.rows = rows, a.V = vocab, a.norm = norm, a.gx = grad_student;
+  a.ga = grad, a.sa = grad_stride, a.tau = static_cast<float>(temperature), a.tau_inv = static_cast<float>(1.0 / temperature);
+  a.ids = ids, a.ids64 = ids64, a.k = static_cast<int>(k), a.p = p, a.by = divisor;
+  return launch_grad<true>(a, dtype, as_stream(stream));
+}

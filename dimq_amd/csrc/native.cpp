@@ -8,6 +8,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -817,6 +818,8 @@ struct MxGelu : torch::autograd::Function<MxGelu> {
   }
 };
 
+#include "native_lm.h"
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(dimq, m) {
@@ -853,6 +856,10 @@ TORCH_LIBRARY_FRAGMENT(dimq, m) {
         "ScalarType? out_dtype=None, ScalarType? bias_dtype=None) -> (Tensor, Tensor)");
   m.def("gelu_forward(Tensor h) -> (Tensor, Tensor, Tensor)");
   m.def("gelu_backward(Tensor grad, Tensor codes, Tensor scales) -> Tensor");
+  m.def("rms_norm(Tensor x, Tensor? weight, float eps, Tensor? residual=None, ScalarType? out_dtype=None) "
+        "-> (Tensor, Tensor)");
+  m.def("rms_norm_e4m3(Tensor x, Tensor? weight, float eps, Tensor? residual=None) -> (Tensor, Tensor, Tensor)");
+  m.def("token_logprobs(Tensor logits, Tensor tokens, int top=0) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(dimq, CUDA, m) {
@@ -875,9 +882,17 @@ TORCH_LIBRARY_IMPL(dimq, CUDA, m) {
   m.impl("linear_grad_weight", linear_grad_weight);
   m.impl("gelu_forward", gelu_forward);
   m.impl("gelu_backward", gelu_backward);
+  m.impl("rms_norm", rms_norm);
+  m.impl("rms_norm_e4m3", rms_norm_e4m3);
+  m.impl("token_logprobs", token_logprobs);
 }
 
-TORCH_LIBRARY_IMPL(dimq, AutogradCUDA, m) { m.impl("mxfp4_linear", mxfp4_linear_graph); }
+TORCH_LIBRARY_IMPL(dimq, AutogradCUDA, m) {
+  m.impl("mxfp4_linear", mxfp4_linear_graph);
+  m.impl("rms_norm", rms_norm_graph);
+  m.impl("rms_norm_e4m3", torch::autograd::autogradNotImplementedFallback());
+  m.impl("token_logprobs", token_logprobs_graph);
+}
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   namespace py = pybind11;
@@ -904,6 +919,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_grad_weight", Direct<&linear_grad_weight>{"linear_grad_weight"}, Unlocked());
   m.def("mx_linear",
         [](const Tensor& x, const Tensor& w, const OptTensor& b) { return MxLinear::apply(x, w, b, at::GradMode::is_enabled()); },
+        Unlocked());
+  m.def("rms_norm", Direct<&rms_norm_graph>{"rms_norm"}, Unlocked());
+  m.def("rms_norm_e4m3", &rms_norm_e4m3_graph, Unlocked());
+  m.def("token_logprobs", Direct<&token_logprobs_graph>{"token_logprobs"}, Unlocked());
+  m.def("distill_loss",
+        [](const Tensor& x, const Tensor& v, const Tensor& ids, double temperature, int64_t reduction) {
+          return DistillLoss::apply(x, v, ids, temperature, reduction, at::GradMode::is_enabled());
+        },
         Unlocked());
   m.def("mx_gelu", [](const Tensor& h) { return MxGelu::apply(h, at::GradMode::is_enabled()); }, Unlocked());
 }

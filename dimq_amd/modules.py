@@ -288,6 +288,35 @@ class DIMQLayerNorm(nn.LayerNorm):
         return ops.layer_norm(x, self.weight, self.bias, self.eps, self.out_dtype)
 
 
+class DIMQRMSNorm(nn.RMSNorm):
+    """nn.RMSNorm over the last dimension on the HIP kernel, with gradients: fp32, fp16 and bf16 CUDA inputs, the residual's
+    addition fused in, and ``e4m3`` for the 8-bit rows that DIMQGroupedLinear takes.  Same parameters and state dict; other
+    inputs raise."""
+
+    @classmethod
+    def from_rms_norm(cls, norm: nn.RMSNorm) -> "DIMQRMSNorm":
+        if len(norm.normalized_shape) != 1:
+            raise ValueError("DIMQRMSNorm normalizes over the last dimension only")
+        new = cls(norm.normalized_shape[0], eps=norm.eps, elementwise_affine=norm.elementwise_affine, device="meta")
+        new.weight = norm.weight
+        return new
+
+    def _eps(self, x: torch.Tensor) -> float:
+        if not x.is_cuda:
+            raise RuntimeError("DIMQRMSNorm runs on CUDA (HIP) tensors only")
+        if x.shape[-1:] != self.normalized_shape:
+            raise RuntimeError(f"DIMQRMSNorm: input's last dimension must be {self.normalized_shape[0]}")
+        return torch.finfo(x.dtype).eps if self.eps is None else self.eps
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """The norm of x; with a residual (norm, x + residual)."""
+        return ops.rms_norm(x, self.weight, self._eps(x), residual=residual)
+
+    def e4m3(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """(codes, scales) of the norm's rows; with a residual (codes, scales, x + residual)."""
+        return ops.rms_norm_e4m3(x, self.weight, self._eps(x), residual=residual)
+
+
 class DIMQMaxPool2d(nn.MaxPool2d):
     """nn.MaxPool2d whose forward runs the HIP max-pool kernel (channels-last
     fp16/bf16 CUDA inputs, dilation 1, floor mode).  Other inputs raise: the

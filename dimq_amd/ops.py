@@ -322,6 +322,44 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
     return torch.ops.dimq.layer_norm(x, int(x.shape[-1]), weight, bias, float(eps), out_dtype)
 
 
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *,
+             residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, h = x; with a residual (x's shape and dtype)
+    ``(y, h)``, h = x + residual rounded to their dtype.  x in fp32, fp16 or bf16, y in ``out_dtype`` (x's by default).
+    Gradients reach x, the residual and the weight; they have none of their own."""
+    require_extension()
+    from ._C import _native
+
+    y, h = _native.rms_norm(x, weight, float(eps), residual, out_dtype)
+    return y if residual is None else (y, h)
+
+
+def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *,
+                  residual: torch.Tensor | None = None):
+    """``rms_norm`` with its rows in 8 bits, the input that ``dimq_linear_grouped`` takes: ``(codes, scales)``, with a
+    residual ``(codes, scales, h)``.  codes: torch.float8_e4m3fn of y / scale, to nearest even; scales: fp32, max|y| / 448
+    of each row (at least 2^-126; 0 for a row of zeros).  A row with a y that is not finite has the scale NaN.  For serving:
+    it has no gradients."""
+    require_extension()
+    from ._C import _native
+
+    codes, scales, h = _native.rms_norm_e4m3(x, weight, float(eps), residual)
+    return (codes, scales) if residual is None else (codes, scales, h)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """``(logprobs, entropy, top_logprobs, top_ids)`` of rows of logits ``[..., vocab]`` in fp32, fp16 or bf16, p their
+    softmax: log p of each row's token (tokens ``[...]``, int64 or int32; 0 for a negative token, NaN for one beyond the
+    vocabulary), the entropy -sum p log p, and the ``top`` (at most 128) largest log p with their tokens, in order, the lower
+    token first among equals.  The values are fp32.  A row that holds a NaN or +infinity, or nothing above -infinity, has
+    no distribution: its values are NaN, its alternatives' tokens -1.  Gradients reach the logits from the log
+    probabilities and the entropy (zero where both of a row's are); they have none of their own."""
+    require_extension()
+    from ._C import _native
+
+    return _native.token_logprobs(logits, tokens, int(top))
+
+
 def max_pool2d_nhwc(x: torch.Tensor, kernel_size, stride=None, padding=0) -> torch.Tensor:
     """2-D max pooling of a channels-last fp16/bf16 tensor on the HIP kernel (the ResNet workload's stem pool)."""
     require_extension()

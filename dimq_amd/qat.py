@@ -12,6 +12,8 @@ results, for CUDA (HIP) tensors.
 * ``dimq_softmin_loss`` -- the Gibbs softmin distortion, forward and backward kernels.
 * ``separation_loss`` -- the hinge margin over centre pairs (margin from ``std(w)``, no
   gradient to ``w``).
+* ``top_logits_distillation_loss`` -- the distance of a quantized language model's logits to the
+  top logits that its teacher kept (no reference counterpart).
 
 ``chunk_size`` is accepted for signature compatibility: the kernels stream the weights and
 need no chunking.  The functions with a backward of their own are autograd nodes of the compiled
@@ -76,3 +78,19 @@ def separation_loss(w: Tensor, centers: Tensor, eta: float = 1.0, eps: float = 1
     if centers.numel() <= 1:
         return centers.new_zeros((), dtype=torch.float32)
     return _native.separation_loss(w, centers, float(eta), float(eps))
+
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def top_logits_distillation_loss(student: Tensor, teacher_values: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
+                                 reduction: str = "mean") -> Tensor:
+    """``t^2 sum_j p_j (log p_j - log q[id_j])`` of each row of student logits ``[..., vocab]`` (fp32, fp16 or bf16), with
+    ``p = softmax(values / t)`` over the teacher's entries ``[..., k]`` (its logits or log probabilities, and int64 or int32
+    tokens, as ``ops.token_logprobs`` returns them) and ``q = softmax(student / t)``.  Entries with a negative token or a
+    value of -infinity are left out; a row without entries has loss 0 and no gradient, whatever its logits.
+    ``reduction`` "mean" (over the rows with entries; 0 without any), "sum" or "none"; the loss is fp32.  A token beyond the
+    vocabulary, or logits without a distribution, give NaN.  The gradient reaches the student alone and has none of its own."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"unsupported reduction {reduction!r}")
+    return _native.distill_loss(student, teacher_values, teacher_ids, float(temperature), _REDUCTIONS[reduction])

@@ -29,7 +29,8 @@ enum dimq_dtype {
   DIMQ_F16 = 1,
   DIMQ_BF16 = 2,
   DIMQ_F64 = 3,
-  DIMQ_U8 = 4
+  DIMQ_U8 = 4,
+  DIMQ_E4M3 = 5 /* 4 exponent and 3 mantissa bits, finite and NaN (largest 448) */
 };
 
 /* Return codes. */
@@ -621,6 +622,68 @@ int dimq_mx_gelu_forward(const void* h, int dtype, int64_t rows, int64_t cols, i
                          uint8_t* scales8, void* stream);
 int dimq_mx_gelu_backward(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ldg, const int8_t* codes8,
                           const uint8_t* scales8, void* gh, void* stream);
+
+/* --------------------------------------------------------------------------
+ * 5. Operators of language models (no reference counterpart)
+ * Float tensors are fp32, fp16 or bf16 unless said otherwise; rows have a
+ * stride in elements, outputs are contiguous.  Workspaces are 16-byte aligned,
+ * of the size their query gives (0: null), written on `stream`, and free for
+ * another call on that stream behind this one.  Results do not depend on
+ * scheduling.
+ * ------------------------------------------------------------------------ */
+
+/* h = x + residual rounded to their dtype (residual and h nullable, together)
+ * and y = h / sqrt(mean(h^2) + eps) * weight (nullable) of rows of `dim`; y in a
+ * float dtype (scales null), or DIMQ_E4M3: codes of y / scale, nearest even,
+ * with scales[row] = max|y| / 448 (at least 2^-126; 0 for a row of zeros, NaN
+ * for a row with a y that is not finite). */
+int dimq_rms_norm(const void* x, int x_dtype, int64_t rows, int64_t dim, int64_t ldx, const void* residual, int64_t ldr,
+                  const void* weight, int w_dtype, double eps, void* y, int y_dtype, float* scales, void* h, void* stream);
+
+/* Gradients for gy (y's) and gh (h's own, nullable; h's dtype): gx, x's and the
+ * residual's alike, in h's dtype, and gw [dim] (each nullable).  The workspace
+ * is for gw alone. */
+int64_t dimq_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
+int dimq_rms_norm_backward(const void* h, int h_dtype, int64_t rows, int64_t dim, int64_t ldh, const void* weight,
+                           int w_dtype, double eps, const void* gy, int gy_dtype, int64_t ldgy, const void* gh,
+                           int64_t ldgh, void* gx, void* gw, int gw_dtype, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
+/* Of rows of `vocab` logits, p their softmax: logprobs[row] = log p of the row's
+ * token (int64 if tokens64, else int32; 0 for a negative one, NaN for one beyond
+ * the vocabulary), entropy[row] = -sum p log p, and the `top` (at most 128)
+ * largest log p with their tokens, ties by the lower token.  A row with a NaN or
+ * +infinity, or nothing above -infinity, has NaNs and tokens -1.  norm
+ * (nullable): [rows, 2], the maximum and log sum exp(x - maximum), for the
+ * backward pass. */
+int64_t dimq_logits_workspace_bytes(int64_t rows, int64_t vocab, int top);
+int dimq_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ldx, const void* tokens,
+                        int tokens64, int top, float* logprobs, float* entropy, float* norm, float* top_logprobs,
+                        int64_t* top_ids, void* workspace, int64_t workspace_bytes, void* stream);
+/* grad_logits [rows, vocab] in the logits' dtype, from the gradients of logprobs
+ * and entropy (each nullable, with its stride); zeros where a row gets none. */
+int dimq_token_logprobs_backward(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ldx,
+                                 const void* tokens, int tokens64, const float* norm, const float* entropy,
+                                 const float* grad_logprobs, int64_t stride_logprobs, const float* grad_entropy,
+                                 int64_t stride_entropy, void* grad_logits, void* stream);
+
+/* Distillation from a teacher's k top logits a row (values, ids [rows, k]; an
+ * entry with a negative id or a value of -infinity is left out):
+ *   row_loss = t^2 sum_j p_j (log p_j - log q[id_j]),
+ *   p = softmax(values / t) over the kept entries, q = softmax(student / t),
+ * 0 for a row without entries.  reduction 0: row_loss alone; 1 the mean over the
+ * rows with entries (0 if there are none), 2 the sum, into loss, and what that
+ * divides by into divisor (one float each).  norm [rows, 2] and p [rows, k] are kept for
+ * the backward pass.  Workspace: dimq_logits_workspace_bytes(rows, vocab, 0). */
+int dimq_distill_loss(const void* student, int dtype, int64_t rows, int64_t vocab, int64_t ldx, const void* values,
+                      int values_dtype, const void* ids, int ids64, int64_t k, double temperature, int reduction,
+                      float* row_loss, float* loss, float* divisor, float* norm, float* p, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+/* grad_student[row, v] = grad[row * grad_stride] t (q_v - p_v) / divisor (nullable: 1). */
+int dimq_distill_loss_backward(const void* student, int dtype, int64_t rows, int64_t vocab, int64_t ldx, const void* ids,
+                               int ids64, int64_t k, const float* p, const float* norm, double temperature,
+                               const float* grad, int64_t grad_stride, const float* divisor, void* grad_student,
+                               void* stream);
 
 #ifdef __cplusplus
 }
