@@ -70,13 +70,22 @@ __device__ __forceinline__ void raise(Stats& a, float m, float scale) {
   a.m = m;
 }
 
-// Over the wave or over `n` entries: every lane's to the common maximum, then plain sums.
+// Two sums over the work-group behind one barrier.
+__device__ __forceinline__ void block_add2(float& a, float& b, float (*red)[4]) {
+  a = wave_add(a);
+  b = wave_add(b);
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = a, red[1][threadIdx.x >> 6] = b;
+  __syncthreads();
+  a = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
+  b = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+}
+
+// Every thread's to the common maximum, then plain sums.
 template <bool U>
 __device__ __forceinline__ Stats block_stats(Stats a, float scale, float (*red)[4]) {
   const float m = row_reduce<kLgThreads, true>(a.m, red[0]);
   raise<U>(a, m, scale);
-  a.s = row_reduce<kLgThreads>(a.s, red[1]);
-  if constexpr (U) a.u = row_reduce<kLgThreads>(a.u, red[2]);
+  block_add2(a.s, a.u, red + 1);
   return a;
 }
 
@@ -203,41 +212,53 @@ __device__ __forceinline__ void each_of_mine(const void* row, const Span& sp, F 
 
 struct TopShared {
   alignas(16) uint32_t maxima[kLgThreads];
-  uint8_t owners[kLgThreads];
   uint64_t cand[kLgCand];
+  uint8_t owners[kLgThreads];
   int count, nowners;
   uint32_t bound;
 };
 
-// Ranks n unique keys and writes the first `top`, in order, to out(rank, key); with fewer the rest are out(rank, 0).
+// A lower bound of the top-th largest logit's order, from the largest order each thread knows of (0: none): the top-th
+// largest of these, found by counting.  Their last 8 bits give way to the thread's number, so that no two are alike and a
+// comparison is all it takes; the bound is only lower for it.
+__device__ __forceinline__ uint32_t bound_of(uint32_t mine, int top, TopShared& sh) {
+  const uint32_t key = (mine & ~0xffu) | (255u - threadIdx.x);
+  sh.maxima[threadIdx.x] = key;
+  if (threadIdx.x == 0) sh.count = 0, sh.nowners = 0;
+  __syncthreads();
+  int before = 0;
+#pragma unroll 16
+  for (int i = 0; i < kLgThreads; i += 4) {
+    const uint4 o = *reinterpret_cast<const uint4*>(&sh.maxima[i]);
+    before += (o.x > key) + (o.y > key) + (o.z > key) + (o.w > key);
+  }
+  if (before == top - 1) sh.bound = mine & ~0xffu;
+  __syncthreads();
+  return sh.bound;
+}
+
+__device__ __forceinline__ void push(TopShared& sh, uint64_t key) {
+  const int i = atomicAdd(&sh.count, 1);  // the order of the list does not matter: its keys are ranked
+  if (i < kLgCand) sh.cand[i] = key;
+}
+
+// Ranks n unique keys and hands the first `top`, which there are, to out(rank, key).
 template <class Out>
 __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int top, Out out) {
   for (int c = threadIdx.x; c < n; c += kLgThreads) {
     const uint64_t key = keys[c];
     int rank = 0;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) rank += keys[i] > key;
     if (rank < top) out(rank, key);
   }
-  for (int r = n + threadIdx.x; r < top; r += kLgThreads) out(r, 0);
 }
 
-// The `top` largest keys of the work-group's span.  `mine`: the largest order_of() of the thread's elements (0: none).
+// The `top` largest keys of the work-group's span, or all of a shorter one with keys 0 behind them.  `mine`: the largest
+// order_of() of the thread's elements, or less.
 template <int XT, class Out>
 __device__ __forceinline__ void span_top(const void* row, const Span& sp, uint32_t mine, int top, TopShared& sh, Out out) {
-  sh.maxima[threadIdx.x] = mine;
-  if (threadIdx.x == 0) sh.count = 0, sh.nowners = 0;
-  __syncthreads();
-  // the top-th largest of the 256 maxima: the thread with top - 1 others before it
-  int before = 0;
-  for (int i = 0; i < kLgThreads; i += 4) {
-    const uint4 o = *reinterpret_cast<const uint4*>(&sh.maxima[i]);
-    const uint32_t w[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) before += w[j] > mine || (w[j] == mine && i + j < static_cast<int>(threadIdx.x));
-  }
-  if (before == top - 1) sh.bound = mine;
-  __syncthreads();
-  const uint32_t bound = sh.bound;
+  const uint32_t bound = bound_of(mine, top, sh);
   if (mine >= bound) sh.owners[atomicAdd(&sh.nowners, 1)] = static_cast<uint8_t>(threadIdx.x);
   __syncthreads();
   // the owners' elements once more, shared out over the whole work-group so that their loads go out together
@@ -246,9 +267,7 @@ __device__ __forceinline__ void span_top(const void* row, const Span& sp, uint32
   const int items = no * static_cast<int>((sp.pieces + kLgThreads - 1) / kLgThreads);  // at most 2^29 + 2^8
   const uint4* body = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + sp.body * (16 / P));
   auto test = [&](float v, int64_t at) {
-    if (order_of(v) < bound) return;
-    const int i = atomicAdd(&sh.count, 1);
-    if (i < kLgCand) sh.cand[i] = key_of(v, at);
+    if (order_of(v) >= bound) push(sh, key_of(v, at));
   };
   for (int base = threadIdx.x; base < items; base += 4 * kLgThreads) {
     uint4 t[4];
@@ -275,8 +294,9 @@ __device__ __forceinline__ void span_top(const void* row, const Span& sp, uint32
   }
   __syncthreads();
   const int n = sh.count;
-  if (n <= kLgCand) {  // the order of the list does not matter: its keys are ranked
+  if (n <= kLgCand) {
     rank_keys(sh.cand, n, top, out);
+    for (int r = n + threadIdx.x; r < top; r += kLgThreads) out(r, 0);
     return;
   }
   // many equal to the bound: one pass for each alternative, the largest key below the last
@@ -312,13 +332,22 @@ __device__ __forceinline__ float nan32() { return __uint_as_float(0x7fc00000u); 
 // Whether (m, s) is a distribution's: no NaN, no +infinity, something above -infinity.
 __device__ __forceinline__ bool proper(const Stats& st) { return st.s > 0.0f && st.s < __uint_as_float(0x7f800000u); }
 
-template <int XT>
-__device__ __forceinline__ void finish_score(const LogitArgs& a, int64_t row, const void* xr, const Stats& st) {
+// A row's token and its logit, loaded ahead of the pass over the row.
+struct TokenLogit {
+  int64_t token;
+  float x;
+  template <int XT>
+  __device__ __forceinline__ static TokenLogit of(const LogitArgs& a, int64_t row, const void* xr) {
+    const int64_t t = index_at(a.tokens, a.tokens64, row);
+    return {t, logit<XT>(xr, t >= 0 && t < a.V ? t : 0)};
+  }
+};
+
+__device__ __forceinline__ void finish_score(const LogitArgs& a, int64_t row, const TokenLogit& t, const Stats& st) {
   if (threadIdx.x != 0) return;
   const bool ok = proper(st);
   const float ls = ok ? logf(st.s) : nan32();
-  const int64_t token = index_at(a.tokens, a.tokens64, row);
-  a.logp[row] = token < 0 ? 0.0f : ok && token < a.V ? (logit<XT>(xr, token) - st.m) - ls : nan32();
+  a.logp[row] = t.token < 0 ? 0.0f : ok && t.token < a.V ? (t.x - st.m) - ls : nan32();
   a.entropy[row] = ok ? ls - st.u / st.s : nan32();
   if (a.norm) a.norm[2 * row] = st.m, a.norm[2 * row + 1] = ls;
 }
@@ -332,62 +361,76 @@ __device__ __forceinline__ void put_top(const LogitArgs& a, int64_t row, int r, 
 // Whether a teacher entry counts: its token is given and its value is not -infinity.
 __device__ __forceinline__ bool kept(int64_t id, float value) { return id >= 0 && value != __uint_as_float(0xff800000u); }
 
-// The teacher's softmax over a row's kept entries, and the row's loss.
-template <int XT>
-__device__ __forceinline__ void finish_distill(const LogitArgs& a, int64_t row, const void* xr, const Stats& st, float (*red)[4]) {
-  const float ls = logf(st.s), tau = 1.0f / a.tau_inv;
-  float m = kLowest, some = 0.0f;
-  for (int j = threadIdx.x; j < a.k; j += kLgThreads) {
-    const float v = load_as_float(a.values, a.values_dt, row * a.k + j);
-    if (!kept(index_at(a.ids, a.ids64, row * a.k + j), v)) continue;
-    m = fmaxf(m, v);
-    some = 1.0f;
-  }
-  __syncthreads();
-  m = row_reduce<kLgThreads, true>(m, red[0]);
-  some = row_reduce<kLgThreads, true>(some, red[1]);
-  float s = 0.0f;
-  for (int j = threadIdx.x; j < a.k; j += kLgThreads) {
-    const float v = load_as_float(a.values, a.values_dt, row * a.k + j);
-    if (kept(index_at(a.ids, a.ids64, row * a.k + j), v)) s += exp_of((v - m) * a.tau_inv);
-  }
-  s = row_reduce<kLgThreads>(s, red[2]);
-  const float lt = logf(s);
-  float loss = 0.0f;
-  for (int j = threadIdx.x; j < a.k; j += kLgThreads) {
+// A teacher's entry: value (-infinity: left out), token and the student's logit there.
+struct Entry {
+  float v, x;
+  bool beyond;
+  template <int XT>
+  __device__ __forceinline__ static Entry of(const LogitArgs& a, int64_t row, const void* xr, int64_t j) {
+    if (j >= a.k) return {__uint_as_float(0xff800000u), 0.0f, false};
     const int64_t id = index_at(a.ids, a.ids64, row * a.k + j);
     const float v = load_as_float(a.values, a.values_dt, row * a.k + j);
-    float p = 0.0f;
-    if (kept(id, v)) {
-      const float lp = (v - m) * a.tau_inv - lt;
-      p = exp_of(lp);
-      const float lq = id < a.V ? (logit<XT>(xr, id) - st.m) * a.tau_inv - ls : nan32();
-      if (p != 0.0f) loss += p * (lp - lq);
-    }
-    a.p[row * a.k + j] = p;
+    const bool in = id >= 0 && id < a.V;
+    return {kept(id, v) ? v : __uint_as_float(0xff800000u), logit<XT>(xr, in ? id : 0), id >= a.V};
   }
-  __syncthreads();
-  loss = row_reduce<kLgThreads>(loss, red[0]);
+  __device__ __forceinline__ bool counts() const { return v != __uint_as_float(0xff800000u); }
+};
+
+// The teacher's softmax over a row's kept entries, and the row's loss.  With e_j = exp((v_j - m) / t) and s their sum,
+// sum_j p_j (log p_j - log q_j) = sum_j e_j ((v_j - m) / t - log q_j) / s - log s: two reductions.  `first`: the thread's
+// first entry, loaded ahead of the pass over the row (the others are loaded where they are used).
+template <int XT>
+__device__ __forceinline__ void finish_distill(const LogitArgs& a, int64_t row, const void* xr, const Entry& first,
+                                               const Stats& st, float (*red)[4]) {
+  const float ls = logf(st.s), tau = 1.0f / a.tau_inv;
+  const float none = __uint_as_float(0xff800000u);
+  float m = none;
+  auto each = [&](auto f) {
+    f(first, static_cast<int64_t>(threadIdx.x));
+    for (int64_t j = threadIdx.x + kLgThreads; j < a.k; j += kLgThreads) f(Entry::of<XT>(a, row, xr, j), j);
+  };
+  each([&](const Entry& e, int64_t) {
+    if (e.counts()) m = fmaxf(m, e.v == e.v ? e.v : kLowest);
+  });
+  m = row_reduce<kLgThreads, true>(m, red[0]);
+  float s = 0.0f, w = 0.0f;
+  each([&](const Entry& e, int64_t) {
+    if (!e.counts()) return;
+    const float d = (e.v - m) * a.tau_inv, p = exp_of(d);
+    s += p;
+    if (p != 0.0f) w += p * (d - (e.beyond ? nan32() : (e.x - st.m) * a.tau_inv - ls));
+  });
+  block_add2(s, w, red + 1);
+  const float r = 1.0f / s;
+  each([&](const Entry& e, int64_t j) {
+    if (j < a.k) a.p[row * a.k + j] = e.counts() ? exp_of((e.v - m) * a.tau_inv) * r : 0.0f;
+  });
   if (threadIdx.x == 0) {
     // a row without entries has no loss, whatever its logits: log s of +infinity marks it.  One whose loss is NaN (its
     // logits', its values' or a token's beyond the vocabulary) has NaN gradients.
-    if (!proper(st)) loss = nan32();
-    a.loss[row] = some == 0.0f ? 0.0f : loss * tau * tau;
+    const float loss = proper(st) ? w / s - logf(s) : nan32();
+    a.loss[row] = m == none ? 0.0f : loss * tau * tau;
     a.norm[2 * row] = st.m;
-    a.norm[2 * row + 1] = some == 0.0f ? __uint_as_float(0x7f800000u) : loss == loss ? ls : nan32();
+    a.norm[2 * row + 1] = m == none ? __uint_as_float(0x7f800000u) : loss == loss ? ls : nan32();
   }
 }
 
 // One split of one row: grid (splits, rows).
 template <int XT, bool DISTILL>
 __global__ __launch_bounds__(kLgThreads) void logits_kernel(const LogitArgs a) {
-  __shared__ float red[3][4];
+  __shared__ float red[6][4];
   __shared__ TopShared sh;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const char* xr = static_cast<const char*>(a.x) + row * a.ldx * (XT == DIMQ_F32 ? 4 : 2);
     const int64_t from = blockIdx.x * a.chunk, to = from + a.chunk < a.V ? from + a.chunk : a.V;
     const Span sp = Span::of<XT>(xr, from, to);
     const float scale = DISTILL ? a.tau_inv : 1.0f;
+    TokenLogit token;
+    Entry entry;
+    if (a.splits == 1) {
+      if constexpr (DISTILL) entry = Entry::of<XT>(a, row, xr, threadIdx.x);
+      else token = TokenLogit::of<XT>(a, row, xr);
+    }
     const Stats mine = stream_stats<XT, !DISTILL>(xr, sp, scale);
     const Stats st = block_stats<!DISTILL>(mine, scale, red);
     if (a.splits > 1) {
@@ -396,9 +439,9 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const LogitArgs a) {
         to_stats[0] = st.m, to_stats[1] = st.s, to_stats[2] = st.u;
       }
     } else if constexpr (DISTILL) {
-      finish_distill<XT>(a, row, xr, st, red);
+      finish_distill<XT>(a, row, xr, entry, st, red + 3);
     } else {
-      finish_score<XT>(a, row, xr, st);
+      finish_score(a, row, token, st);
     }
     if constexpr (!DISTILL) {
       if (a.top > 0) {
@@ -423,8 +466,9 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const LogitArgs a) {
 // Joins the splits of a row.
 template <int XT, bool DISTILL>
 __global__ __launch_bounds__(kLgThreads) void logits_join_kernel(const LogitArgs a) {
-  __shared__ float red[3][4];
+  __shared__ float red[6][4];
   __shared__ uint64_t keys[DISTILL ? 1 : kLgSplits * kLgTop];
+  __shared__ TopShared sh;
   const int64_t row = blockIdx.x;
   const char* xr = static_cast<const char*>(a.x) + row * a.ldx * (XT == DIMQ_F32 ? 4 : 2);
   Stats st{kLowest, 0.0f, 0.0f};
@@ -432,20 +476,36 @@ __global__ __launch_bounds__(kLgThreads) void logits_join_kernel(const LogitArgs
     const float* from = a.stats + (row * a.splits + threadIdx.x) * 4;
     st = {from[0], from[1], from[2]};
   }
-  st = block_stats<!DISTILL>(st, DISTILL ? a.tau_inv : 1.0f, red);
   if constexpr (DISTILL) {
-    finish_distill<XT>(a, row, xr, st, red);
+    const Entry entry = Entry::of<XT>(a, row, xr, threadIdx.x);
+    st = block_stats<false>(st, a.tau_inv, red);
+    finish_distill<XT>(a, row, xr, entry, st, red + 3);
   } else {
-    finish_score<XT>(a, row, xr, st);
-    if (a.top > 0) {
-      const int n = a.splits * a.top;
-      for (int i = threadIdx.x; i < n; i += kLgThreads) keys[i] = a.cand[row * n + i];
-      __syncthreads();
-      const bool ok = proper(st);
-      if (ok) rank_keys(keys, n, a.top, [&](int r, uint64_t key) { put_top(a, row, r, key, st, true); });
-      else
-        for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, st, false);
+    const TokenLogit token = TokenLogit::of<XT>(a, row, xr);
+    const int n = a.splits * a.top;
+    uint64_t mine = 0;
+    for (int i = threadIdx.x; i < n; i += kLgThreads) {
+      const uint64_t key = a.cand[row * n + i];
+      keys[i] = key;
+      mine = key > mine ? key : mine;
     }
+    st = block_stats<true>(st, 1.0f, red);
+    finish_score(a, row, token, st);
+    if (a.top == 0) return;
+    if (!proper(st)) {
+      for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, st, false);
+      return;
+    }
+    // as in span_top, over the splits' keys: there are at least `top` of them that are not 0
+    const uint32_t bound = bound_of(static_cast<uint32_t>(mine >> 32), a.top, sh);
+    for (int i = threadIdx.x; i < n; i += kLgThreads) {
+      const uint64_t key = keys[i];
+      if (key != 0 && static_cast<uint32_t>(key >> 32) >= bound) push(sh, key);
+    }
+    __syncthreads();
+    auto put = [&](int r, uint64_t key) { put_top(a, row, r, key, st, true); };
+    if (sh.count <= kLgCand) rank_keys(sh.cand, sh.count, a.top, put);
+    else rank_keys(keys, n, a.top, put);  // zeros rank behind all others
   }
 }
 

@@ -224,17 +224,21 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     const Tensor v = values.detach().contiguous();
     const int64_t k = id.size(-1);
     const auto f = student.options().dtype(at::kFloat);
-    const Tensor each = at::empty(student.sizes().slice(0, student.dim() - 1), f), loss = at::empty({}, f);
-    const Tensor norm = at::empty({x.n, 2}, f), p = at::empty({x.n, k}, f), by = at::empty({}, f);
+    const bool none = reduction == 0;
+    const Tensor loss = none ? at::empty(student.sizes().slice(0, student.dim() - 1), f) : at::empty({}, f);
+    // what the backward pass reads in one allocation: the divisor, norm [rows, 2], p [rows, k]; the rows' losses and the
+    // workspace (16-byte aligned) in another
+    const Tensor kept = at::empty({4 + x.n * (2 + k)}, f);
+    const int64_t bytes = dimq_logits_workspace_bytes(x.n, x.cols, 0);
+    const Tensor ws = at::empty({bytes / 4 + (none ? 0 : x.n)}, f);
     const On on(student);
-    const Tensor ws = workspace(dimq_logits_workspace_bytes(x.n, x.cols, 0), student);
     check_rc(dimq_distill_loss(ptr(x.t), dt(x.t), x.n, x.cols, x.ld, ptr(v), dt(v), ptr(id), id.scalar_type() == at::kLong, k,
-                               temperature, static_cast<int>(reduction), f32(each), f32(loss), f32(by), f32(norm), f32(p), ptr(ws),
-                               ws.defined() ? ws.numel() : 0, on.stream));
-    if (keep && student.requires_grad()) ctx->save_for_backward({student, ids, norm, p, by});
+                               temperature, static_cast<int>(reduction), none ? f32(loss) : f32(ws) + bytes / 4, f32(loss), f32(kept),
+                               f32(kept) + 4, f32(kept) + 4 + 2 * x.n, ptr(ws), bytes, on.stream));
+    if (keep && student.requires_grad()) ctx->save_for_backward({student, id, kept});
     ctx->saved_data["temperature"] = temperature;
-    ctx->saved_data["none"] = reduction == 0;
-    return reduction == 0 ? each : loss;
+    ctx->saved_data["none"] = none;
+    return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* op = "top_logits_distillation_loss's gradient";
@@ -244,12 +248,12 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     const Tensor& student = saved[0];
     const bool none = ctx->saved_data["none"].toBool();
     const LogitRows x(student, op);
-    const Tensor id = index_rows(saved[1], student, 0, op, "teacher ids");
+    const Tensor &id = saved[1], &kept = saved[2];
     const Tensor g = grads[0].detach().reshape({-1}), gx = at::empty(student.sizes(), student.options());
     const On on(student);
     check_rc(dimq_distill_loss_backward(ptr(x.t), dt(x.t), x.n, x.cols, x.ld, ptr(id), id.scalar_type() == at::kLong, id.size(-1),
-                                        f32(saved[3]), f32(saved[2]), ctx->saved_data["temperature"].toDouble(), f32(g),
-                                        none ? g.stride(0) : 0, none ? nullptr : f32(saved[4]), ptr(gx), on.stream));
+                                        f32(kept) + 4 + 2 * x.n, f32(kept) + 4, ctx->saved_data["temperature"].toDouble(), f32(g),
+                                        none ? g.stride(0) : 0, none ? nullptr : f32(kept), ptr(gx), on.stream));
     return {gx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

@@ -39,18 +39,36 @@ struct RmsArgs {
 
 constexpr float kE4m3Max = 448.0f;
 
-// Scale and reciprocal of a row whose largest |y| is `top`.  A scale below 2^-126 would have no reciprocal; rows that
-// small take the least normal one (their codes then stay below 448), a zero row takes 0 and codes 0.
-__device__ __forceinline__ void e4m3_scale(float top, bool finite, float& scale, float& inv) {
-  const float s = fmaxf(top / kE4m3Max, 0x1p-126f);
-  scale = !finite ? __uint_as_float(0x7fc00000u) : top == 0.0f ? 0.0f : s;
-  inv = finite ? 1.0f / s : 0.0f;
+// Codes of a row.  With s = f 2^e, 1 <= f < 2, the row's y is n f for n = (h 2^e) w, which is exact for bf16 and fp16 rows
+// and weights, and a code is the rounded 448 n / max|n|: f cancels, and the quotient, corrected by its remainder, meets the
+// ties between two codes as exactly as they are (with y / scale formed through s, a third of the rows of 4,096 bf16 elements
+// had a code on the wrong side of one).  The least scale is 2^-126: below it there would be no reciprocal.
+struct E4m3Row {
+  float den, inv, scale;
+  // top: max|n|, infinite where a y is not finite
+  __device__ __forceinline__ E4m3Row(float top, float f) {
+    den = fmaxf(top, kE4m3Max * 0x1p-126f / f);
+    inv = 1.0f / den;
+    scale = den * f / kE4m3Max;
+    if (top == 0.0f) scale = 0.0f;
+    if (!(top * f < __uint_as_float(0x7f800000u))) inv = 0.0f, den = 0.0f, scale = __uint_as_float(0x7fc00000u);
+  }
+  __device__ __forceinline__ float code(float n) const {
+    const float a = n * (kE4m3Max / 512), q = a * inv;  // by 512 at the end: 448 n may be beyond fp32
+    return __builtin_amdgcn_fmed3f(512 * fmaf(fmaf(-q, den, a), inv, q), -kE4m3Max, kE4m3Max);
+  }
+};
+
+// s as f 2^e; a mean square beyond fp32 gives s = 0, y = 0.
+__device__ __forceinline__ float power_below(float s) { return __uint_as_float(__float_as_uint(s) & 0x7f800000u); }
+__device__ __forceinline__ float factor_above(float s) {
+  return __uint_as_float((__float_as_uint(s) & 0x007fffffu) | 0x3f800000u);
 }
 
-__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float inv) {
+__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], const E4m3Row& r) {
   float q[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = __builtin_amdgcn_fmed3f(v[j] * inv, -kE4m3Max, kE4m3Max);
+  for (int j = 0; j < 8; ++j) q[j] = r.code(v[j]);
   uint32_t a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
   uint32_t b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
@@ -108,24 +126,24 @@ __global__ __launch_bounds__(threads_of<T>()) void rms_norm_kernel(const RmsArgs
     sq = row_reduce<T>(sq, red[0]);
     const float s = 1.0f / sqrtf(sq / static_cast<float>(a.D) + a.eps);
     if constexpr (Q) {
+      const float e = power_below(s);
       float top = 0.0f;
       bool fine = true;
 #pragma unroll
       for (int c = 0; c < NCH; ++c)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          v[c][j] = v[c][j] * s * w[c][j];
+          v[c][j] = v[c][j] * e * w[c][j];
           top = fmaxf(top, fabsf(v[c][j]));
           fine &= fabsf(v[c][j]) < __uint_as_float(0x7f800000u);
         }
       // a value that is not finite becomes the row's largest
       top = row_reduce<T, true>(fine ? top : __uint_as_float(0x7f800000u), red[1]);
-      float scale, inv;
-      e4m3_scale(top, top < __uint_as_float(0x7f800000u), scale, inv);
+      const E4m3Row q8(top, factor_above(s));
       uint8_t* yr = static_cast<uint8_t*>(a.y) + row * a.D;
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const uint2 o = e4m3x8(v[c], inv);
+        const uint2 o = e4m3x8(v[c], q8);
         if constexpr (VEC == 8) {
           if (8 * (t + T * c) < a.D) *reinterpret_cast<uint2*>(yr + 8 * (t + T * c)) = o;
         } else {
@@ -136,7 +154,7 @@ __global__ __launch_bounds__(threads_of<T>()) void rms_norm_kernel(const RmsArgs
           }
         }
       }
-      if (t == 0) a.scale[row] = scale;
+      if (t == 0) a.scale[row] = q8.scale;
     } else {
       char* yr = static_cast<char*>(a.y) + row * a.D * (a.ydt == DIMQ_F32 ? 4 : 2);
 #pragma unroll
@@ -171,23 +189,24 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const RmsArgs a, in
     const float s = 1.0f / sqrtf(sq / static_cast<float>(a.D) + a.eps);
     const void* src = a.r ? a.h : a.x;  // each thread reads back what it wrote itself
     const int64_t base = a.r ? hrow : row * a.ldx;
-    float scale = 0.0f, inv = 1.0f;
+    const float e = Q ? power_below(s) : s;
+    E4m3Row q8(1.0f, 1.0f);
     if constexpr (Q) {
       float top = 0.0f;
       bool fine = true;
       for (int i = t; i < a.D; i += 1024) {
-        const float v = load_as_float(src, xdt, base + i) * s * (a.w ? load_as_float(a.w, a.wdt, i) : 1.0f);
+        const float v = load_as_float(src, xdt, base + i) * e * (a.w ? load_as_float(a.w, a.wdt, i) : 1.0f);
         top = fmaxf(top, fabsf(v));
         fine &= fabsf(v) < __uint_as_float(0x7f800000u);
       }
       top = row_reduce<1024, true>(fine ? top : __uint_as_float(0x7f800000u), red[1]);
-      e4m3_scale(top, top < __uint_as_float(0x7f800000u), scale, inv);
-      if (t == 0) a.scale[row] = scale;
+      q8 = E4m3Row(top, factor_above(s));
+      if (t == 0) a.scale[row] = q8.scale;
     }
     for (int i = t; i < a.D; i += 1024) {
-      const float v = load_as_float(src, xdt, base + i) * s * (a.w ? load_as_float(a.w, a.wdt, i) : 1.0f);
+      const float v = load_as_float(src, xdt, base + i) * e * (a.w ? load_as_float(a.w, a.wdt, i) : 1.0f);
       if constexpr (Q) {
-        const float q = __builtin_amdgcn_fmed3f(v * inv, -kE4m3Max, kE4m3Max);
+        const float q = q8.code(v);
         static_cast<uint8_t*>(a.y)[hrow + i] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false));
       } else {
         store_from_float(a.y, a.ydt, hrow + i, v);
@@ -259,8 +278,23 @@ __global__ __launch_bounds__(threads_of<T>()) void rms_norm_grad_kernel(const Rm
     if constexpr (T > 64) __syncthreads();
   }
   if (!a.part) return;
-  // a row of part for each of the work-group's rows in flight
-  float* pr = a.part + (static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / T) * a.D;
+  float* pr = a.part + static_cast<int64_t>(blockIdx.x) * a.D;
+  if constexpr (kRows > 1) {  // the waves' sums, added in order through the LDS
+    __shared__ float sum[kRows][T * NCH * 8];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[threadIdx.x / T][(8 * c + j) * T + t] = gw[c][j];
+    __syncthreads();
+    if (threadIdx.x >= T) return;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = (8 * c + j) * T + t;
+        gw[c][j] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
+      }
+  }
 #pragma unroll
   for (int c = 0; c < NCH; ++c) row_store<DIMQ_F32, T, VEC>(pr, t, c, a.D, gw[c]);
 }
@@ -296,26 +330,29 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(const RmsArgs 
   }
 }
 
-// gw[d] = sum of part's rows: 64 columns a work-group, 4 waves take every fourth row each.
-__global__ __launch_bounds__(256) void rms_norm_sum_kernel(const float* __restrict__ part, int n, int D, void* gw, int dt) {
-  __shared__ float sum[4][64];
+// gw[d] = sum of part's rows: 64 columns a work-group, 16 waves take every sixteenth row each.
+__global__ __launch_bounds__(1024) void rms_norm_sum_kernel(const float* __restrict__ part, int n, int D, void* gw, int dt) {
+  __shared__ float sum[16][64];
   const int d = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
   float s = 0.0f;
   if (d < D) {
     int i = wave;
-    for (; i + 28 < n; i += 32) {  // eight loads in flight
+    for (; i + 112 < n; i += 128) {  // eight loads in flight
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = part[static_cast<int64_t>(i + 4 * j) * D + d];
+      for (int j = 0; j < 8; ++j) v[j] = part[static_cast<int64_t>(i + 16 * j) * D + d];
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += v[j];
     }
-    for (; i < n; i += 4) s += part[static_cast<int64_t>(i) * D + d];
+    for (; i < n; i += 16) s += part[static_cast<int64_t>(i) * D + d];
   }
   sum[wave][threadIdx.x & 63] = s;
   __syncthreads();
-  if (wave == 0 && d < D)
-    store_from_float(gw, dt, d, (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]));
+  if (wave != 0 || d >= D) return;
+  s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) s += sum[w][threadIdx.x];
+  store_from_float(gw, dt, d, s);
 }
 
 // Threads a row and 8-element chunks a thread: a wave for rows of up to 1,024 elements, a work-group of 256 for up to
@@ -391,13 +428,7 @@ int check_rms(const char* what, const void* x, int x_dtype, int64_t rows, int64_
 }
 
 // Work-groups of the backward pass: each writes its sums of gy u, so no more than half the forward pass's.
-unsigned grad_groups(int64_t rows, int64_t dim) {
-  const RowPlan p = row_plan(dim);
-  return row_groups(rows, p, p.threads == 64 ? 512 : 1024);
-}
-int64_t grad_part_rows(int64_t rows, int64_t dim) {
-  return static_cast<int64_t>(grad_groups(rows, dim)) * (row_plan(dim).threads == 64 ? 4 : 1);
-}
+unsigned grad_groups(int64_t rows, int64_t dim) { return row_groups(rows, row_plan(dim), 1024); }
 
 }  // namespace
 }  // namespace dimq
@@ -452,7 +483,7 @@ extern "C" int dimq_rms_norm(const void* x, int x_dtype, int64_t rows, int64_t d
 
 extern "C" int64_t dimq_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim) {
   if (rows <= 0 || dim <= 0) return 0;
-  return row_plan(dim).threads == 0 ? (rows < 256 ? rows : 256) * dim * 4 : grad_part_rows(rows, dim) * dim * 4;
+  return row_plan(dim).threads == 0 ? (rows < 256 ? rows : 256) * dim * 4 : static_cast<int64_t>(grad_groups(rows, dim)) * dim * 4;
 }
 
 extern "C" int dimq_rms_norm_backward(const void* h, int h_dtype, int64_t rows, int64_t dim, int64_t ldh, const void* weight,
@@ -480,7 +511,7 @@ extern "C" int dimq_rms_norm_backward(const void* h, int h_dtype, int64_t rows, 
       parts = rows < 256 ? rows : 256;
       hipLaunchKernelGGL(rms_norm_grad_long_kernel, dim3(static_cast<unsigned>(parts)), dim3(1024), 0, s, a, h_dtype);
     } else {
-      parts = grad_part_rows(rows, dim);
+      parts = grad_groups(rows, dim);
       const int size = dtype_size(h_dtype);
       const bool vec = dim % 8 == 0 && vec_rows(h, ldh, rows, size) && vec_rows(gy, ldgy, rows, dtype_size(gy_dtype)) &&
                        vec_rows(gh, ldgh, rows, size) && vec_rows(gx, dim, rows, size) && vec_rows(weight, 0, 1, 1) &&
@@ -494,7 +525,7 @@ extern "C" int dimq_rms_norm_backward(const void* h, int h_dtype, int64_t rows, 
     }
   }
   if (gw)  // no rows: zeros
-    hipLaunchKernelGGL(rms_norm_sum_kernel, dim3(static_cast<unsigned>((dim + 63) / 64)), dim3(256), 0, s,
+    hipLaunchKernelGGL(rms_norm_sum_kernel, dim3(static_cast<unsigned>((dim + 63) / 64)), dim3(1024), 0, s,
                        static_cast<const float*>(workspace), static_cast<int>(parts), static_cast<int>(dim), gw, gw_dtype);
   return check_launch("rms_norm_backward");
 }
