@@ -26,8 +26,10 @@ from .modules import (
     DIMQCodebookConv2d,
     DIMQCodebookLinear,
     DIMQConv2d,
+    DIMQGroupedLinear,
     DIMQLinear,
     DIMQMXFP4Linear,
+    DIMQRMSNorm,
     make_packed_layer,
     quantize_model_weight_only,
     replace_modules_with_packed_dimq,
@@ -39,8 +41,10 @@ __all__ = [
     "DIMQCodebookConv2d",
     "DIMQCodebookLinear",
     "DIMQConv2d",
+    "DIMQGroupedLinear",
     "DIMQLinear",
     "DIMQMXFP4Linear",
+    "DIMQRMSNorm",
     "activation_qparams_from_minmax",
     "assign_weight_indices",
     "bits_for_codebook",

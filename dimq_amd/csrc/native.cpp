@@ -859,6 +859,8 @@ TORCH_LIBRARY_FRAGMENT(dimq, m) {
   m.def("rms_norm(Tensor x, Tensor? weight, float eps, Tensor? residual=None, ScalarType? out_dtype=None) "
         "-> (Tensor, Tensor)");
   m.def("rms_norm_e4m3(Tensor x, Tensor? weight, float eps, Tensor? residual=None) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_grouped(Tensor x, Tensor codes, Tensor scales, Tensor? zeros, int group_size, Tensor? bias=None, "
+        "Tensor? x_scales=None, Tensor? residual=None, int activation=0, ScalarType? out_dtype=None) -> Tensor");
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top=0) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
@@ -885,12 +887,14 @@ TORCH_LIBRARY_IMPL(dimq, CUDA, m) {
   m.impl("rms_norm", rms_norm);
   m.impl("rms_norm_e4m3", rms_norm_e4m3);
   m.impl("token_logprobs", token_logprobs);
+  m.impl("linear_grouped", linear_grouped);
 }
 
 TORCH_LIBRARY_IMPL(dimq, AutogradCUDA, m) {
   m.impl("mxfp4_linear", mxfp4_linear_graph);
   m.impl("rms_norm", rms_norm_graph);
   m.impl("rms_norm_e4m3", torch::autograd::autogradNotImplementedFallback());
+  m.impl("linear_grouped", torch::autograd::autogradNotImplementedFallback());
   m.impl("token_logprobs", token_logprobs_graph);
 }
 
@@ -922,6 +926,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         Unlocked());
   m.def("rms_norm", Direct<&rms_norm_graph>{"rms_norm"}, Unlocked());
   m.def("rms_norm_e4m3", &rms_norm_e4m3_graph, Unlocked());
+  m.def("linear_grouped", &linear_grouped_graph, Unlocked());
   m.def("token_logprobs", Direct<&token_logprobs_graph>{"token_logprobs"}, Unlocked());
   m.def("distill_loss",
         [](const Tensor& x, const Tensor& v, const Tensor& ids, double temperature, int64_t reduction) {

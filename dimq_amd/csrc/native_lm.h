@@ -257,3 +257,81 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     return {gx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
+
+// ---- 4-bit weights with group scales -----------------------------------------------
+
+Tensor linear_grouped(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& zeros, int64_t group,
+                      const OptTensor& bias, const OptTensor& x_scales, const OptTensor& residual, int64_t activation,
+                      std::optional<at::ScalarType> out_dtype) {
+  const char* op = "linear_grouped";
+  TORCH_CHECK_NOT_IMPLEMENTED(x.is_cuda(), op, " expects a CUDA input");
+  const bool q8 = x.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(q8 || mx_float(x.scalar_type()), op, ": input must be fp32, fp16, bf16 or float8_e4m3fn, not ",
+              dtype_name(x.scalar_type()));
+  TORCH_CHECK(x.dim() > 0 && codes.dim() == 2 && scales.dim() == 2, op,
+              " expects an input of at least one dimension, 2-D codes and 2-D scales");
+  const int64_t K = x.size(-1), N = codes.size(0), nb = mx_blocks(K);
+  TORCH_CHECK(K > 0 && N > 0, "linear dimensions must be positive");
+  TORCH_CHECK(group > 0 && group % 32 == 0, op, ": the group size must be a positive multiple of 32");
+  const int64_t G = (K + group - 1) / group;
+  const auto here = [&](const Tensor& t, const char* what) {
+    TORCH_CHECK(t.device() == x.device(), op, ": ", what, " must be on ", x.device().str());
+  };
+  here(codes, "codes");
+  here(scales, "scales");
+  TORCH_CHECK(codes.scalar_type() == at::kByte, op, ": codes must be uint8");
+  TORCH_CHECK(mx_float(scales.scalar_type()), op, ": scales must be fp32, fp16 or bf16");
+  TORCH_CHECK(codes.size(1) == nb * 16, op, ": rows of ", K, " have codes [out_features, ", nb * 16, "], not ",
+              tuple_of(codes.sizes()));
+  TORCH_CHECK(scales.size(0) == N && scales.size(1) == G, op, ": groups of ", group, " have scales (", N, ", ", G, "), not ",
+              tuple_of(scales.sizes()));
+  Tensor z;
+  if (zeros) {
+    here(*zeros, "zeros");
+    TORCH_CHECK(zeros->scalar_type() == at::kByte && zeros->sizes() == scales.sizes(), op,
+                ": zeros must be uint8 of the scales' shape");
+    z = zeros->contiguous();
+  }
+  TORCH_CHECK(q8 == x_scales.has_value(), op, ": float8_e4m3fn inputs, and no others, take x_scales");
+  Tensor xs;
+  if (q8) {
+    here(*x_scales, "x_scales");
+    TORCH_CHECK(x_scales->scalar_type() == at::kFloat && x_scales->sizes() == x.sizes().slice(0, x.dim() - 1), op,
+                ": x_scales must be fp32, one for each row");
+    xs = x_scales->contiguous();
+  }
+  Tensor c = codes.contiguous();
+  if (reinterpret_cast<uintptr_t>(c.data_ptr()) % 16) c = c.clone();
+  const Tensor s = scales.detach().contiguous();
+  const int64_t M = x.numel() / K;
+  Tensor t = x.detach();
+  if (x.dim() != 2) t = t.reshape({M, K});
+  if ((K > 1 && t.stride(1) != 1) || (M > 1 && t.stride(0) < K)) t = t.contiguous();
+  const int64_t ld = M > 1 ? t.stride(0) : K;
+  const at::ScalarType odt = out_dtype.value_or(q8 ? at::kBFloat16 : x.scalar_type());
+  TORCH_CHECK(mx_float(odt), op, ": output dtype must be fp32, fp16 or bf16");
+  const Bias b(bias, N, "out_features");
+  const std::vector<int64_t> shape = out_shape(x, N);
+  const Residual r(residual, shape, at::MemoryFormat::Contiguous);
+  if (bias) here(*bias, "bias");
+  if (residual) here(*residual, "residual");
+  const int xdt = q8 ? static_cast<int>(DIMQ_E4M3) : dt(x);
+  const Tensor y = at::empty(shape, x.options().dtype(odt));
+  const On on(x);
+  const Tensor ws = workspace(dimq_linear_grouped_workspace_bytes(ptr(t), xdt, M, K, ld, N), c);
+  check_rc(dimq_linear_grouped(ptr(t), xdt, M, K, ld, static_cast<float*>(ptr(xs)), u8(c), ptr(s), dt(s),
+                               static_cast<uint8_t*>(ptr(z)), group, b.p, b.dtype, N, ptr(y), dt(y), r.p, r.dtype,
+                               static_cast<int>(activation), ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
+  return y;
+}
+
+// The weights are frozen and the layer is for serving: where a gradient may be asked for, the operator's own graph refuses
+// it in the backward pass.
+Tensor linear_grouped_graph(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& zeros, int64_t group,
+                            const OptTensor& bias, const OptTensor& x_scales, const OptTensor& residual, int64_t activation,
+                            std::optional<at::ScalarType> out_dtype) {
+  const Direct<&linear_grouped> direct{"linear_grouped"};
+  return wants_grad(x) || wants_grad(scales) || wants_grad(bias) || wants_grad(x_scales) || wants_grad(residual)
+             ? direct.op(x, codes, scales, zeros, group, bias, x_scales, residual, activation, out_dtype)
+             : direct(x, codes, scales, zeros, group, bias, x_scales, residual, activation, out_dtype);
+}

@@ -179,6 +179,42 @@ class DIMQMXFP4Linear(nn.Module):
         return cls(codes, scales, linear.in_features, bias, out_dtype=out_dtype)
 
 
+class DIMQGroupedLinear(nn.Module):
+    """Linear on 4-bit weights with a scale and a zero point per group of a row's elements (``ops.quantize_grouped``): a
+    float input, or (codes, scales) of 8-bit rows as DIMQRMSNorm.e4m3 gives them.  Frozen, for serving."""
+
+    def __init__(self, codes, scales, zeros, group_size, in_features, bias=None, *,
+                 out_dtype: torch.dtype | None = None) -> None:
+        super().__init__()
+        self.register_buffer("codes", codes.contiguous())
+        self.register_buffer("scales", scales.contiguous())
+        self.register_buffer("zeros", None if zeros is None else zeros.contiguous())
+        self.register_buffer("bias", None if bias is None else bias.contiguous())
+        self.out_features = int(codes.shape[0])
+        self.in_features = int(in_features)
+        self.group_size = int(group_size)
+        self.out_dtype = out_dtype
+
+    def forward(self, x, residual: torch.Tensor | None = None, activation: str | None = None) -> torch.Tensor:
+        """act(linear(x) + residual); residual and activation ("relu", "gelu") are fused into the kernel."""
+        x, x_scales = x if isinstance(x, tuple) else (x, None)
+        _require_gpu(x, self.codes, True, "DIMQGroupedLinear")
+        if x.shape[-1] != self.in_features:
+            raise RuntimeError(f"DIMQGroupedLinear: input's last dimension must be {self.in_features}")
+        return ops.dimq_linear_grouped(x, self.codes, self.scales, self.zeros, self.group_size, self.bias,
+                                       x_scales=x_scales, residual=residual, activation=activation,
+                                       out_dtype=self.out_dtype)
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, linear: nn.Linear, group_size: int = 128, *, symmetric: bool = False,
+                    scale_dtype: torch.dtype = torch.float16,
+                    out_dtype: torch.dtype | None = None) -> "DIMQGroupedLinear":
+        codes, scales, zeros = ops.quantize_grouped(linear.weight, group_size, symmetric=symmetric, scale_dtype=scale_dtype)
+        bias = None if linear.bias is None else linear.bias.detach().clone()
+        return cls(codes, scales, zeros, group_size, linear.in_features, bias, out_dtype=out_dtype)
+
+
 class DIMQCodebookConv2d(nn.Module):
     """Weight-only Conv2d with b-bit codebook indices (conv_kcrs layout)."""
 

@@ -322,6 +322,52 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
     return torch.ops.dimq.layer_norm(x, int(x.shape[-1]), weight, bias, float(eps), out_dtype)
 
 
+def quantize_grouped(w: torch.Tensor, group_size: int = 128, *, symmetric: bool = False,
+                     scale_dtype: torch.dtype = torch.float16):
+    """``(codes, scales, zeros)`` of a weight ``[out_features, in_features]`` in 4 bits with a scale per group of
+    ``group_size`` (a multiple of 32) elements of a row, for :func:`dimq_linear_grouped`.  The grid runs from a group's
+    smallest value (0 if that is positive) to its largest (0 if negative) in 15 steps, with a zero point that stands for 0
+    exactly; ``symmetric``: around 0 (codes 1..15, zero point 8, zeros None).  codes: uint8 ``[out_features, 16 * blocks]``,
+    rows padded to blocks of 32, two a byte, the earlier element in the low half.  Done once, at load, in torch operations;
+    a weight that is not finite raises."""
+    if w.dim() != 2 or w.numel() == 0:
+        raise RuntimeError("quantize_grouped expects a weight [out_features, in_features]")
+    if group_size <= 0 or group_size % 32:
+        raise RuntimeError("quantize_grouped: the group size must be a positive multiple of 32")
+    w = w.detach().float()
+    if not bool(torch.isfinite(w).all()):
+        raise RuntimeError("quantize_grouped: the weight must be finite")
+    n, k = w.shape
+    groups, blocks = -(-k // group_size), -(-k // 32)
+    v = torch.nn.functional.pad(w, (0, groups * group_size - k)).view(n, groups, group_size)
+    low, high = v.amin(2).clamp(max=0), v.amax(2).clamp(min=0)
+    steps = torch.maximum(-low, high) / 7 if symmetric else (high - low) / 15
+    # a scale that its type rounds to 0 could not be divided by
+    scales = steps.clamp(min=torch.finfo(scale_dtype).tiny, max=torch.finfo(scale_dtype).max).to(scale_dtype)
+    s = scales.float()
+    zeros = None if symmetric else torch.round(-low / s).clamp(0, 15)
+    q = torch.round(v / s[..., None] + (8 if symmetric else zeros[..., None])).clamp(0, 15).to(torch.uint8)
+    q = torch.nn.functional.pad(q.view(n, -1)[:, :k], (0, blocks * 32 - k)).view(n, blocks * 16, 2)
+    return q[..., 0] + q[..., 1] * 16, scales, None if symmetric else zeros.to(torch.uint8)
+
+
+def dimq_linear_grouped(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None,
+                        group_size: int, bias: torch.Tensor | None = None, *, x_scales: torch.Tensor | None = None,
+                        residual: torch.Tensor | None = None, activation: str | None = None,
+                        out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``act(x W^T + bias + residual)`` with ``W[n, k] = scales[n, k // group_size] * (q[n, k] - zeros[n, k // group_size])``,
+    q the 4-bit codes as :func:`quantize_grouped` packs them, zeros (uint8, at most 15) 8 where None.  x in fp32, fp16 or
+    bf16, or in torch.float8_e4m3fn with ``x_scales`` (fp32, one for each row, as :func:`rms_norm_e4m3` gives), which
+    multiplies the row.  Neither x nor W is rounded, sums are fp32; a row of x that holds a NaN or an infinity gives outputs that
+    are not finite; the output in ``out_dtype`` (x's by default, bf16 for
+    float8).  For serving: a backward pass through it raises."""
+    require_extension()
+    from ._C import _native
+
+    return _native.linear_grouped(x, codes, scales, zeros, int(group_size), bias, x_scales, residual,
+                                  ACTIVATIONS[activation], out_dtype)
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *,
              residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
     """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, h = x; with a residual (x's shape and dtype)

@@ -685,6 +685,20 @@ int dimq_distill_loss_backward(const void* student, int dtype, int64_t rows, int
                                const float* grad, int64_t grad_stride, const float* divisor, void* grad_student,
                                void* stream);
 
+/* y = act(c[m] sum_g s[n, g] sum_{k in g} (q[n, k] - z[n, g]) x[m, k] + bias[n] +
+ * residual[m, n]) for 4-bit weights with a scale per group of `group` (a
+ * multiple of 32) elements of a row: codes [N, ceil(K / 32), 16], two a byte,
+ * the earlier element in the low half (16-byte aligned), scales [N, G] and zeros
+ * [N, G] (0..15; nullable: 8), G = ceil(K / group).  x in a float dtype, or
+ * DIMQ_E4M3 with x_scales[m] = c (else null).  Exact products, fp32 sums in a
+ * fixed order, one rounding to y_dtype; bias [N] and residual [M, N] nullable,
+ * any float dtype. */
+int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int64_t N);
+int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const float* x_scales,
+                        const uint8_t* codes, const void* scales, int scales_dtype, const uint8_t* zeros, int64_t group,
+                        const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype, const void* residual,
+                        int residual_dtype, int activation, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
