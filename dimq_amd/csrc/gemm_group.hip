@@ -10,7 +10,7 @@
 // conversion a pair makes bf16 or fp16 numbers of them.  sum x of a group comes from the same instructions against ones.  An
 // fp32 x is the sum of three bf16 numbers of 8 bits each; e4m3 rows are converted to bf16 (exactly).  The e4m3 matrix
 // instructions would take these rows and the bytes as they are, at twice the rate, but they cut addends off below the
-// largest: against 64 bits, sums of 32 products were up to 4,700 2^-24 of their terms' magnitudes off, in bf16 under 2.
+// largest: against 64 bits, sums of 32 products were up to 4,700 2^-24 of their terms' magnitudes off, in bf16 0.1.
 //
 // Which 32 k of an instruction's share a lane holds is free as long as both operands agree: lane l (column or row l % 16,
 // quarter l / 16) takes 2 LB consecutive k of a "span" of 8 LB, its codes one load of LB bytes.  A span lies in one group:
@@ -44,6 +44,7 @@ struct GroupArgs {
   int splits;
   float* part;            // [splits][M][N]
   int64_t tiles_m, tiles_n;
+  const float* sums;      // [M][spans of whole k steps]
 };
 
 constexpr int x_size(int xt) { return xt == DIMQ_F32 ? 4 : xt == DIMQ_E4M3 ? 1 : 2; }
@@ -81,18 +82,20 @@ __device__ __forceinline__ void decode_span(const uint32_t (&codes)[LB / 4], uin
   }
 }
 
-// acc + a span's products.
+// acc + the products of step j of a span, and of all of it.
+template <int MT, int LB>
+__device__ __forceinline__ floatx4 mul_step(const uint32_t (&a)[LB], const uint32_t (&b)[LB], int j, floatx4 acc) {
+  const u32x4 u = {a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]};
+  const u32x4 v = {b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]};
+  if constexpr (MT == DIMQ_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u), __builtin_bit_cast(bf16x8, v), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, u), __builtin_bit_cast(half8, v), acc, 0, 0, 0);
+}
 template <int MT, int LB>
 __device__ __forceinline__ floatx4 mul_span(const uint32_t (&a)[LB], const uint32_t (&b)[LB], floatx4 acc) {
 #pragma unroll
-  for (int j = 0; j < LB / 4; ++j) {
-    const u32x4 u = {a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]};
-    const u32x4 v = {b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]};
-    if constexpr (MT == DIMQ_BF16)
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u), __builtin_bit_cast(bf16x8, v), acc, 0, 0, 0);
-    else
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, u), __builtin_bit_cast(half8, v), acc, 0, 0, 0);
-  }
+  for (int j = 0; j < LB / 4; ++j) acc = mul_step<MT, LB>(a, b, j, acc);
   return acc;
 }
 
@@ -303,84 +306,130 @@ __global__ __launch_bounds__(64 * kFewWaves) void group_few_kernel(const GroupAr
 }
 
 // ---- many rows ----------------------------------------------------------------------------------------------------
-// 128 x 128 outputs a work-group of 4 waves of 64 x 64 each.  A k step is 128: x of all 128 rows and the columns' codes come
-// into the LDS by direct loads, a step ahead, and the codes are decoded behind the LDS.  x is read in place where its rows
-// are whole steps and aligned, else from a padded copy (group_copy_kernel).
+// The zero points' part of the product, sum_g s z sum_{k in g} x, is a product of its own with a reduction 8 LB times
+// shorter: a first launch sums x over each span (and copies x where its rows are not whole k steps, aligned and of 16 bits),
+// and after the main loop those sums and s z, each as three bf16 parts, go through the matrix instructions once.  Against
+// ones in the loop the sums cost a fifth of its matrix instructions, and taken off each span's product half of its fmas.
+//
+// Then 128 x 128 outputs a work-group of 4 waves of 64 x 64 each.  A k step is 128: x of all 128 rows and the columns' codes
+// come into the LDS by direct loads, a step ahead, and the codes are decoded behind the LDS.
 constexpr int kTile = 128, kTileK = 128, kTileThreads = 256;
 
-// x's rows padded with zeros to whole k steps: [planes][M][ksteps 128].
-template <int XT>
-__global__ __launch_bounds__(256) void group_copy_kernel(const GroupArgs p, uint8_t* out) {
-  const int64_t kp = p.ksteps * kTileK, per = kp / 8, total = p.M * per;
+// sums [M][spans of whole k steps]; out (nullable): x padded with zeros to whole k steps, [planes][M][ksteps 128].
+template <int XT, int LB>
+__global__ __launch_bounds__(256) void group_prep_kernel(const GroupArgs p, uint8_t* out, float* sums) {
+  const uint32_t per = static_cast<uint32_t>(p.ksteps) * (kTileK / 8);  // a multiple of 16: 16 neighbouring lanes share a row
+  const int64_t total = p.M * per, kp = p.ksteps * kTileK;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t m = i / per, k0 = (i - m * per) * 8;
     RawX<XT, 4> r;
     r.load(p, m, k0, p.vec && k0 + 8 <= p.K);
     uint32_t a[planes_of(XT)][4];
     r.planes(a);
+    if (out) {
 #pragma unroll
-    for (int q = 0; q < planes_of(XT); ++q) {
-      uint8_t* to = out + q * p.plane + (m * kp + k0) * 2;
-      *reinterpret_cast<uint4*>(to) = make_uint4(a[q][0], a[q][1], a[q][2], a[q][3]);
+      for (int q = 0; q < planes_of(XT); ++q)
+        *reinterpret_cast<uint4*>(out + q * p.plane + (m * kp + k0) * 2) = make_uint4(a[q][0], a[q][1], a[q][2], a[q][3]);
     }
+    float s = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if constexpr (XT == DIMQ_F32) s += __uint_as_float(r.w[q]);
+      else if constexpr (XT == DIMQ_F16) s += f16_bits_to_float((r.w[q >> 1] >> (16 * (q & 1))) & 0xffffu);
+      else s += bf16_bits_to_float((a[0][q >> 1] >> (16 * (q & 1))) & 0xffffu);
+    }
+#pragma unroll
+    for (int w = 1; w < LB; w *= 2) s += __shfl_xor(s, w, 64);
+    if ((threadIdx.x & (LB - 1)) == 0) sums[(m * kp + k0) / (8 * LB)] = s;
   }
+}
+
+// 16 bytes a lane from base (the same in all lanes) + off into the LDS at lds + 16 lane.  Inline, as dma16 (common.h), so
+// that the waits are the kernel's: the load must not follow a vector instruction that wrote its scalar address (a
+// readfirstlane, or a spilled register's v_readlane) by fewer than five wait states, which the compiler does not see to here.
+__device__ __forceinline__ void group_dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // MT: type of x in the LDS; P: its planes, one after another within a k step.
 template <int MT, int LB, int P>
 __global__ __launch_bounds__(kTileThreads, 2) void group_tile_kernel(const GroupArgs p) {
-  constexpr int ES = 2, SP = 8 * LB, NS = kTileK / SP;
-  constexpr int RowBytes = kTileK * ES, Chunks = RowBytes / 16, StageBytes = kTile * RowBytes, CodeBytes = kTile * 64;
+  constexpr int SP = 8 * LB, NS = kTileK / SP;
+  constexpr int RowBytes = kTileK * 2, Chunks = RowBytes / 16, StageBytes = kTile * RowBytes, CodeBytes = kTile * 64;
   __shared__ __attribute__((aligned(1024))) uint8_t xs[2][StageBytes];
   __shared__ __attribute__((aligned(1024))) uint8_t cs[2][CodeBytes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
   const int wm = wave & 1, wn = wave >> 1;
   // neighbouring work-groups are on different XCDs: each XCD takes a contiguous part of the tiles, rows fastest, so that its
   // L2 holds a few columns' codes and x
-  const int64_t tiles = p.tiles_m * p.tiles_n;
-  int64_t tile = blockIdx.x;
-  {
-    const int64_t per = tiles / 8, xcd = tile % 8, rest = tiles - per * 8;
-    tile = xcd * per + (xcd < rest ? xcd : rest) + tile / 8;
-  }
-  const int64_t m0 = tile % p.tiles_m * kTile, n0 = tile / p.tiles_m * kTile;
-  const int64_t steps_each = (p.ksteps + p.splits - 1) / p.splits;
-  const int64_t step0 = blockIdx.y * steps_each, step1 = step0 + steps_each < p.ksteps ? step0 + steps_each : p.ksteps;
+  const uint32_t tiles = static_cast<uint32_t>(p.tiles_m * p.tiles_n), per = tiles / 8, rest = tiles % 8, xcd = blockIdx.x % 8;
+  const uint32_t tile = xcd * per + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+  const uint32_t tm = static_cast<uint32_t>(p.tiles_m);
+  const int64_t m0 = static_cast<int64_t>(tile % tm) * kTile, n0 = static_cast<int64_t>(tile / tm) * kTile;
+  const int ksteps = static_cast<int>(p.ksteps), steps_each = (ksteps + p.splits - 1) / p.splits;
+  const int step0 = blockIdx.y * steps_each, step1 = step0 + steps_each < ksteps ? step0 + steps_each : ksteps;
   const uint32_t ldsx = lds_address(&xs[0][0]), ldsc = lds_address(&cs[0][0]);
+  const int rows = p.M - m0 < kTile ? static_cast<int>(p.M - m0) : kTile, cols = p.N - n0 < kTile ? static_cast<int>(p.N - n0) : kTile;
 
-  // stage of x: a wave's load is 1 KB, 1024 / RowBytes rows of Chunks pieces; chunk c of row r lies at slot c ^ (r % Chunks)
-  constexpr int kLoads = StageBytes / 1024 / 4, kRowsPerLoad = 1024 / RowBytes;
-  auto fetch_x = [&](int64_t step, int plane, int slot) {
-    const uint8_t* base = static_cast<const uint8_t*>(p.x) + plane * p.plane + step * RowBytes;
+  // Stage of x: a wave's load is 1 KB, 4 rows of 16 pieces; piece c of row r lies at slot c ^ (r % 16).  Offsets from the
+  // tile's first row stay below 2^32 (checked on the host).
+  constexpr int kLoads = StageBytes / 1024 / 4;
+  uint32_t xoff[kLoads], coff[2];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int r0 = (wave * kLoads + i) * kRowsPerLoad, r = r0 + lane / Chunks, c = (lane % Chunks) ^ (r % Chunks);
-      const int64_t m = m0 + r < p.M ? m0 + r : p.M - 1;
-      dma16(base + m * p.ldx * ES + c * 16, ldsx + slot * StageBytes + r0 * RowBytes);
-    }
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = (wave * kLoads + i) * 4 + lane / Chunks, c = (lane % Chunks) ^ (r % Chunks);
+    xoff[i] = static_cast<uint32_t>(r < rows ? r : rows - 1) * static_cast<uint32_t>(p.ldx * 2) + c * 16;
+  }
+  // stage of codes: 64 bytes a column
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (wave * 2 + i) * 16 + lane / 4;
+    coff[i] = static_cast<uint32_t>(r < cols ? r : cols - 1) * static_cast<uint32_t>(p.pitch) + lane % 4 * 16;
+  }
+  const uint8_t* xbase = static_cast<const uint8_t*>(p.x) + m0 * p.ldx * 2;
+  const uint8_t* cbase = p.codes + n0 * p.pitch;
+  auto fetch_x = [&](int step, int plane, int slot) {
+    const uint8_t* base = uniform(xbase + plane * p.plane + static_cast<int64_t>(step) * RowBytes);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) group_dma16(base, xoff[i], ldsx + slot * StageBytes + (wave * kLoads + i) * 1024);
   };
-  // stage of codes: 64 bytes a column; past the row's last block that block again (x is 0 there)
-  auto fetch_codes = [&](int64_t step, int slot) {
+  auto fetch_codes = [&](int step, int slot) {
+    const uint8_t* base = uniform(cbase + static_cast<int64_t>(step) * 64);
+    // past the row's last block that block again (x is 0 there)
+    const int over = (step + 1) * 64 - static_cast<int>(p.pitch), back = over > 0 ? lane % 4 * 16 + over - 48 : 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r0 = (wave * 2 + i) * 16;
-      const int64_t n = n0 + r0 + lane / 4, at = step * 64 + lane % 4 * 16;
-      dma16(p.codes + (n < p.N ? n : p.N - 1) * p.pitch + (at < p.pitch ? at : p.pitch - 16), ldsc + slot * CodeBytes + r0 * 64);
-    }
+    for (int i = 0; i < 2; ++i)
+      group_dma16(base, coff[i] - (back > 0 ? back : 0), ldsc + slot * CodeBytes + (wave * 2 + i) * 1024);
+  };
+  // scales of 4 blocks of 16 columns in a step (their bits; load_scale); the spans' groups are counted up
+  const int wide = p.s_dt == DIMQ_F32, group_spans = static_cast<int>(p.group / SP);
+  uint32_t goff[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int n = wn * 64 + c * 16 + col;
+    goff[c] = static_cast<uint32_t>(n < cols ? n : cols - 1) * static_cast<uint32_t>(p.groups);
+  }
+  const uint16_t* sbase = static_cast<const uint16_t*>(p.scales) + ((n0 * p.groups) << wide);
+  const uint32_t groups = static_cast<uint32_t>(p.groups);
+  auto raw_scale = [&](int c, uint32_t at) -> RawScale {
+    const uint32_t i = (goff[c] + at) << wide;
+    return {sbase[i], sbase[i + wide]};
   };
   RawScale rs[4][NS];
-  uint32_t zr[4][NS];
-  auto fetch_scales = [&](int64_t step) {
+  uint32_t g = static_cast<uint32_t>(step0) * NS / group_spans, phase = static_cast<uint32_t>(step0) * NS % group_spans;
+  auto fetch_scales = [&]() {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      int64_t g = (step * kTileK + s * SP) / p.group;
-      if (g >= p.groups) g = p.groups - 1;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int64_t n = n0 + wn * 64 + c * 16 + col, at = (n < p.N ? n : p.N - 1) * p.groups + g;
-        rs[c][s] = load_scale(p, at);
-        zr[c][s] = p.zeros ? p.zeros[at] : 8u;
-      }
+      for (int c = 0; c < 4; ++c) rs[c][s] = raw_scale(c, g < groups ? g : groups - 1);
+      if (++phase == static_cast<uint32_t>(group_spans)) phase = 0, ++g;
     }
   };
 
@@ -391,27 +440,27 @@ __global__ __launch_bounds__(kTileThreads, 2) void group_tile_kernel(const Group
     for (int c = 0; c < 4; ++c) acc[t][c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
   if (step0 < step1) {
-    fetch_scales(step0);
+    fetch_scales();
     fetch_codes(step0, 0);
     fetch_x(step0, 0, 0);
   }
   int slot = 0, cslot = 0;
-  for (int64_t step = step0; step < step1; ++step) {
-    float sc[4][NS], zc[4][NS];
+  for (int step = step0; step < step1; ++step) {
+    float sc[4][NS];
 #pragma unroll 1  // unrolled, the planes would keep their codes decoded and spill
     for (int plane = 0; plane < P; ++plane) {
       wait_vmcnt<0>();
       __syncthreads();  // this stage is in the LDS, and the other one is free
       if (plane == 0) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-          for (int s = 0; s < NS; ++s) sc[c][s] = scale_of(p, rs[c][s]), zc[c][s] = static_cast<float>(zr[c][s]);
+          for (int c = 0; c < 4; ++c) sc[c][s] = scale_of(p, rs[c][s]);
       }
       if (plane + 1 < P) {
         fetch_x(step, plane + 1, slot ^ 1);
       } else if (step + 1 < step1) {
-        fetch_scales(step + 1);
+        fetch_scales();
         fetch_codes(step + 1, cslot ^ 1);
         fetch_x(step + 1, 0, slot ^ 1);
       }
@@ -419,17 +468,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void group_tile_kernel(const Group
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         uint32_t a[4][LB];
-        floatx4 sx[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int r = wm * 64 + t * 16 + col;
-          const int byte = (s * SP + quarter * 2 * LB) * ES;  // of the row
+          const int r = wm * 64 + t * 16 + col, c0 = (s * SP + quarter * 2 * LB) / 8;  // piece of the row
 #pragma unroll
           for (int i = 0; i < LB / 4; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(st + r * RowBytes + (((byte / 16 + i) ^ (r % Chunks)) << 4));
+            const uint4 v = *reinterpret_cast<const uint4*>(st + r * RowBytes + (((c0 + i) ^ (r % Chunks)) << 4));
             a[t][4 * i] = v.x, a[t][4 * i + 1] = v.y, a[t][4 * i + 2] = v.z, a[t][4 * i + 3] = v.w;
           }
-          sx[t] = sum_span<MT, LB>(a[t], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -445,17 +491,66 @@ __global__ __launch_bounds__(kTileThreads, 2) void group_tile_kernel(const Group
             w[0] = *reinterpret_cast<const uint32_t*>(q);
           }
           decode_span<MT, LB>(w, b);
+          floatx4 v[4];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const floatx4 v = mul_span<MT, LB>(a[t], b, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+          for (int t = 0; t < 4; ++t) v[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][c][i] = fmaf(sc[c][s], fmaf(-zc[c][s], sx[t][i], v[i]), acc[t][c][i]);
-          }
+          for (int j = 0; j < LB / 4; ++j)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[t] = mul_step<MT, LB>(a[t], b, j, v[t]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][c][i] = fmaf(sc[c][s], v[t][i], acc[t][c][i]);
         }
       }
       slot ^= 1;
     }
     cslot ^= 1;
+  }
+  // acc -= (sums of x) (s z)^T, the first of the k ranges for all of them; of the parts' products those above 2^-24
+  if (blockIdx.y == 0) {
+    const uint8_t* zbase = p.zeros ? p.zeros + n0 * p.groups : nullptr;
+    const int spans = ksteps * NS;
+    const float* sums = p.sums + m0 * spans;
+#pragma unroll 1
+    for (int g0 = 0; g0 < spans; g0 += 32) {
+      const int mine = g0 + quarter * 8;
+      uint32_t a[4][3][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int r = wm * 64 + t * 16 + col;
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = sums[static_cast<int64_t>(r < rows ? r : rows - 1) * spans + (mine + e < spans ? mine + e : spans - 1)];
+          v[e] = mine + e < spans ? __float_as_uint(f) : 0u;
+        }
+        split3(v, a[t][0], a[t][1], a[t][2]);
+      }
+      uint32_t at[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        at[e] = static_cast<uint32_t>(mine + e) / static_cast<uint32_t>(group_spans);
+        if (at[e] >= groups) at[e] = groups - 1;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[8], b[3][4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float z = static_cast<float>(zbase ? zbase[goff[c] + at[e]] : 8u);
+          v[e] = __float_as_uint(-scale_of(p, raw_scale(c, at[e])) * z);
+        }
+        split3(v, b[0], b[1], b[2]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int j = 0; i + j < 3; ++j)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[t][c] = mul_step<DIMQ_BF16, 4>(a[t][i], b[j], 0, acc[t][c]);
+      }
+    }
   }
   // 16 rows of the wave at a time through the LDS, so that a store is 64 neighbouring columns
   __syncthreads();
@@ -507,8 +602,9 @@ constexpr int64_t kFewRows = 64;  // rows of the first kernel
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
 struct TilePlan {
-  int64_t ksteps, tm, tn, copy_bytes, part_bytes;
+  int64_t ksteps, tm, tn, copy_bytes, sum_bytes, part_bytes;
   int splits;
+  int64_t bytes() const { return copy_bytes + sum_bytes + part_bytes; }
 };
 // Tiles that leave CUs idle are cut along k, into parts of at least four steps.
 TilePlan tile_plan(int xt, int64_t M, int64_t K, int64_t N, bool in_place) {
@@ -521,6 +617,7 @@ TilePlan tile_plan(int xt, int64_t M, int64_t K, int64_t N, bool in_place) {
   t.splits = static_cast<int>(s < 1 ? 1 : s);
   t.splits = static_cast<int>((t.ksteps + (t.ksteps + t.splits - 1) / t.splits - 1) / ((t.ksteps + t.splits - 1) / t.splits));
   t.copy_bytes = in_place ? 0 : up256(M * t.ksteps * kTileK * 2) * planes_of(xt);
+  t.sum_bytes = up256(M * t.ksteps * (kTileK / 32) * 4);  // spans of 32 at the least
   t.part_bytes = t.splits > 1 ? t.splits * M * N * 4 : 0;
   return t;
 }
@@ -528,8 +625,9 @@ TilePlan tile_plan(int xt, int64_t M, int64_t K, int64_t N, bool in_place) {
 bool rows_aligned(const void* x, int xt, int64_t M, int64_t ldx) {
   return aligned(x, 16) && (M <= 1 || ldx * x_size(xt) % 16 == 0);
 }
+constexpr int64_t kMostApart = 1 << 23;  // elements between rows that the tiles read: 128 of them stay below 2^32 bytes
 bool rows_in_place(const void* x, int xt, int64_t M, int64_t K, int64_t ldx) {
-  return x_size(xt) == 2 && K % kTileK == 0 && rows_aligned(x, xt, M, ldx);
+  return x_size(xt) == 2 && K % kTileK == 0 && rows_aligned(x, xt, M, ldx) && ldx < kMostApart;
 }
 
 template <int XT, int LB>
@@ -545,14 +643,17 @@ template <int XT, int LB>
 void launch_tile(GroupArgs p, const TilePlan& t, uint8_t* ws, hipStream_t s) {
   constexpr int ML = mul_type(XT), P = planes_of(XT);
   p.ksteps = t.ksteps, p.tiles_m = t.tm, p.tiles_n = t.tn, p.splits = t.splits;
+  float* sums = reinterpret_cast<float*>(ws + t.copy_bytes);
+  p.plane = t.copy_bytes / P;
+  const int64_t blocks = (p.M * t.ksteps * (kTileK / 8) + 255) / 256;
+  hipLaunchKernelGGL((group_prep_kernel<XT, LB>), dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, p,
+                     t.copy_bytes ? ws : nullptr, sums);
   if (t.copy_bytes) {
-    p.plane = t.copy_bytes / P;
-    const int64_t blocks = (p.M * t.ksteps * (kTileK / 8) + 255) / 256;
-    hipLaunchKernelGGL((group_copy_kernel<XT>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, p, ws);
     p.x = ws;
     p.ldx = t.ksteps * kTileK;
   }
-  p.part = reinterpret_cast<float*>(ws + t.copy_bytes);
+  p.sums = sums;
+  p.part = reinterpret_cast<float*>(ws + t.copy_bytes + t.sum_bytes);
   const dim3 grid(static_cast<unsigned>(t.tm * t.tn), static_cast<unsigned>(t.splits));
   hipLaunchKernelGGL((group_tile_kernel<ML, LB, P>), grid, dim3(kTileThreads), 0, s, p);
   if (t.splits > 1) {
@@ -570,7 +671,7 @@ extern "C" int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtyp
   if (M <= kFewRows || K <= 0 || N <= 0) return 0;
   if (x_dtype != DIMQ_F32 && x_dtype != DIMQ_F16 && x_dtype != DIMQ_BF16 && x_dtype != DIMQ_E4M3) return 0;
   const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
-  return t.copy_bytes + t.part_bytes;
+  return t.bytes();
 }
 
 extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const float* x_scales,
@@ -621,9 +722,10 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
     DIMQ_GROUP_XT(launch_few, p, s)
   } else {
     const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
-    DIMQ_CHECK(workspace_bytes >= t.copy_bytes + t.part_bytes && aligned(workspace, 16),
+    DIMQ_CHECK(workspace_bytes >= t.bytes() && aligned(workspace, 16),
                "linear_grouped: the workspace is too small or not 16-byte aligned");
     DIMQ_CHECK(t.tm * t.tn < (int64_t)1 << 24, "linear_grouped: too many outputs for one launch");
+    DIMQ_CHECK(t.ksteps * kTileK < kMostApart, "linear_grouped: more than 64 rows must be shorter than 2^23 elements");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     DIMQ_GROUP_XT(launch_tile, p, t, ws, s)
   }
