@@ -44,7 +44,9 @@ struct GroupArgs {
   int splits;
   float* part;            // [splits][M][N]
   int64_t tiles_m, tiles_n;
-  const float* sums;      // [M][spans of whole k steps]
+  int64_t span_blocks;    // blocks of 32 spans
+  const uint8_t* sums;    // the zero points' product
+  const uint8_t* szs;
 };
 
 constexpr int x_size(int xt) { return xt == DIMQ_F32 ? 4 : xt == DIMQ_E4M3 ? 1 : 2; }
@@ -68,17 +70,24 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t bytes, float by) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, by, HIGH));
 }
 
-// A lane's codes of a span as the instructions' operand.
+// Eight codes as one step's operand, and a lane's codes of a span.
+template <int MT>
+__device__ __forceinline__ void decode_step(uint32_t codes, uint32_t (&b)[4]) {
+  uint32_t lo, hi;
+  code_bytes(codes, lo, hi);
+  b[0] = code_pair<MT, false>(lo, 512.0f);
+  b[1] = code_pair<MT, true>(lo, 512.0f);
+  b[2] = code_pair<MT, false>(hi, 512.0f);
+  b[3] = code_pair<MT, true>(hi, 512.0f);
+}
 template <int MT, int LB>
 __device__ __forceinline__ void decode_span(const uint32_t (&codes)[LB / 4], uint32_t (&b)[LB]) {
 #pragma unroll
   for (int j = 0; j < LB / 4; ++j) {
-    uint32_t lo, hi;
-    code_bytes(codes[j], lo, hi);
-    b[4 * j] = code_pair<MT, false>(lo, 512.0f);
-    b[4 * j + 1] = code_pair<MT, true>(lo, 512.0f);
-    b[4 * j + 2] = code_pair<MT, false>(hi, 512.0f);
-    b[4 * j + 3] = code_pair<MT, true>(hi, 512.0f);
+    uint32_t s[4];
+    decode_step<MT>(codes[j], s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[4 * j + i] = s[i];
   }
 }
 
@@ -219,6 +228,35 @@ __device__ __forceinline__ void put_output(const GroupArgs& p, int64_t m, int64_
   store_from_float(p.y, p.y_dt, off, epi1(p.epi, off, v));
 }
 
+// Outputs off .. off + left - 1 of one row, their bias in them already.
+__device__ __forceinline__ void put8(const GroupArgs& p, int64_t off, int left, float (&v)[8]) {
+  if (p.epi.res) {
+    for (int j = 0; j < 8; ++j)
+      if (j < left) v[j] += load_as_float(p.epi.res, p.epi.res_dt, off + j);
+  }
+  if (p.epi.act) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act_apply(v[j], p.epi.act);
+  }
+  if (left == 8) {  // 16 bytes to a multiple of the element's size
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (p.y_dt == DIMQ_F32) {
+      u4* to = reinterpret_cast<u4*>(static_cast<float*>(p.y) + off);
+      to[0] = u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      to[1] = u4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+    } else {
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[j] = p.y_dt == DIMQ_F16 ? f16x2_rne(v[2 * j], v[2 * j + 1]) : bf16x2_rne(v[2 * j], v[2 * j + 1]);
+      *reinterpret_cast<u4*>(static_cast<uint16_t*>(p.y) + off) = u4{o[0], o[1], o[2], o[3]};
+    }
+    return;
+  }
+  for (int j = 0; j < 8; ++j)
+    if (j < left) store_from_float(p.y, p.y_dt, off + j, v[j]);
+}
+
 // ---- few rows -----------------------------------------------------------------------------------------------------
 // 16 MT rows by 16 columns a work-group; its 8 waves share out the spans, and their sums meet in the LDS.  A wave's loads
 // of U spans go out together.  Rows past M re-read the last one; they are not stored.
@@ -311,14 +349,42 @@ __global__ __launch_bounds__(64 * kFewWaves) void group_few_kernel(const GroupAr
 // and after the main loop those sums and s z, each as three bf16 parts, go through the matrix instructions once.  Against
 // ones in the loop the sums cost a fifth of its matrix instructions, and taken off each span's product half of its fmas.
 //
-// Then 128 x 128 outputs a work-group of 4 waves of 64 x 64 each.  A k step is 128: x of all 128 rows and the columns' codes
-// come into the LDS by direct loads, a step ahead, and the codes are decoded behind the LDS.
-constexpr int kTile = 128, kTileK = 128, kTileThreads = 256;
+// Then 128 x 256 outputs a work-group of 8 waves of 64 x 64 each.  A k step is 128: x of the 128 rows, the columns' codes and
+// scales come into a ring of three slots in the LDS by direct loads, two steps ahead, and the codes are decoded behind the
+// LDS.  No other load is in the loop, so the kernel's own counted wait is the only one.  With 128 x 128 tiles, two slots and
+// two work-groups a CU the waves stood a third of the time at the barrier: 2048 x 4096 -> 4096 in 150 us.
+constexpr int kTileM = 128, kTileN = 256, kTileK = 128, kTileThreads = 512;
+constexpr int kSlots = 3;
 
-// sums [M][spans of whole k steps]; out (nullable): x padded with zeros to whole k steps, [planes][M][ksteps 128].
+// Both operands of the zero points' product: [row][blocks of 32 spans][3 parts][32 spans] in bf16, zeros behind the last span.
+constexpr int kPartBytes = 3 * 32 * 2;  // of a block
+
+// sums: x's, [M]; szs: -s z, [N]; out (nullable): x padded with zeros to whole k steps, [planes][M][ksteps 128].
 template <int XT, int LB>
-__global__ __launch_bounds__(256) void group_prep_kernel(const GroupArgs p, uint8_t* out, float* sums) {
-  const uint32_t per = static_cast<uint32_t>(p.ksteps) * (kTileK / 8);  // a multiple of 16: 16 neighbouring lanes share a row
+__global__ __launch_bounds__(256) void group_prep_kernel(const GroupArgs p, uint8_t* out, uint8_t* sums, uint8_t* szs) {
+  constexpr int SP = 8 * LB;
+  const int64_t blocks = p.span_blocks;
+  if (blockIdx.y == 1) {  // 8 spans a thread
+    const uint32_t group_spans = static_cast<uint32_t>(p.group / SP), per = static_cast<uint32_t>(blocks) * 4;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < p.N * per; i += static_cast<int64_t>(gridDim.x) * 256) {
+      const int64_t n = i / per;
+      const uint32_t first = static_cast<uint32_t>(i - n * per) * 8;
+      uint32_t v[8], o[3][4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t g = (first + e) / group_spans;
+        const int64_t at = n * p.groups + (g < p.groups ? g : p.groups - 1);
+        const float sz = -scale_of(p, load_scale(p, at)) * static_cast<float>(p.zeros ? p.zeros[at] : 8u);
+        v[e] = g < p.groups ? __float_as_uint(sz) : 0u;
+      }
+      split3(v, o[0], o[1], o[2]);
+      uint8_t* to = szs + (n * blocks + first / 32) * kPartBytes + first % 32 * 2;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * 64) = make_uint4(o[q][0], o[q][1], o[q][2], o[q][3]);
+    }
+    return;
+  }
+  const uint32_t per = static_cast<uint32_t>(blocks) * (32 * SP / 8);  // a multiple of 16: 16 neighbouring lanes share a row
   const int64_t total = p.M * per, kp = p.ksteps * kTileK;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t m = i / per, k0 = (i - m * per) * 8;
@@ -326,7 +392,7 @@ __global__ __launch_bounds__(256) void group_prep_kernel(const GroupArgs p, uint
     r.load(p, m, k0, p.vec && k0 + 8 <= p.K);
     uint32_t a[planes_of(XT)][4];
     r.planes(a);
-    if (out) {
+    if (out && k0 < kp) {
 #pragma unroll
       for (int q = 0; q < planes_of(XT); ++q)
         *reinterpret_cast<uint4*>(out + q * p.plane + (m * kp + k0) * 2) = make_uint4(a[q][0], a[q][1], a[q][2], a[q][3]);
@@ -340,7 +406,15 @@ __global__ __launch_bounds__(256) void group_prep_kernel(const GroupArgs p, uint
     }
 #pragma unroll
     for (int w = 1; w < LB; w *= 2) s += __shfl_xor(s, w, 64);
-    if ((threadIdx.x & (LB - 1)) == 0) sums[(m * kp + k0) / (8 * LB)] = s;
+    if ((threadIdx.x & (LB - 1)) == 0) {
+      const uint32_t v[8] = {__float_as_uint(s), 0, 0, 0, 0, 0, 0, 0};
+      uint32_t o[3][4];
+      split3(v, o[0], o[1], o[2]);
+      const int64_t span = k0 / SP;
+      uint8_t* to = sums + (m * blocks + span / 32) * kPartBytes + span % 32 * 2;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint16_t*>(to + q * 64) = static_cast<uint16_t>(o[q][0]);
+    }
   }
 }
 
@@ -358,13 +432,29 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// MT: type of x in the LDS; P: its planes, one after another within a k step.
+__device__ __forceinline__ void group_dma4(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+
+// A span's group, counted up.
+struct GroupCount {
+  uint32_t g, phase, each, last;
+  __device__ __forceinline__ GroupCount(uint32_t span, uint32_t group_spans, uint32_t groups)
+      : g(span / group_spans), phase(span % group_spans), each(group_spans), last(groups - 1) {}
+  __device__ __forceinline__ uint32_t next() {
+    const uint32_t at = g < last ? g : last;  // spans behind the row's end: x is 0 there
+    if (++phase == each) phase = 0, ++g;
+    return at;
+  }
+};
+
+// MT: type of x in the LDS; P: its planes, one after another within a k step (each a stage of its own).
 template <int MT, int LB, int P>
-__global__ __launch_bounds__(kTileThreads, 2) void group_tile_kernel(const GroupArgs p) {
+__global__ __launch_bounds__(kTileThreads) void group_tile_kernel(const GroupArgs p) {
   constexpr int SP = 8 * LB, NS = kTileK / SP;
-  constexpr int RowBytes = kTileK * 2, Chunks = RowBytes / 16, StageBytes = kTile * RowBytes, CodeBytes = kTile * 64;
-  __shared__ __attribute__((aligned(1024))) uint8_t xs[2][StageBytes];
-  __shared__ __attribute__((aligned(1024))) uint8_t cs[2][CodeBytes];
+  constexpr int RowBytes = kTileK * 2, Chunks = RowBytes / 16;
+  constexpr int XBytes = kTileM * RowBytes, CodeBytes = kTileN * 64, SlotBytes = XBytes + CodeBytes + NS * kTileN * 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kSlots * SlotBytes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
   const int wm = wave & 1, wn = wave >> 1;
   // neighbouring work-groups are on different XCDs: each XCD takes a contiguous part of the tiles, rows fastest, so that its
@@ -372,211 +462,228 @@ __global__ __launch_bounds__(kTileThreads, 2) void group_tile_kernel(const Group
   const uint32_t tiles = static_cast<uint32_t>(p.tiles_m * p.tiles_n), per = tiles / 8, rest = tiles % 8, xcd = blockIdx.x % 8;
   const uint32_t tile = xcd * per + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
   const uint32_t tm = static_cast<uint32_t>(p.tiles_m);
-  const int64_t m0 = static_cast<int64_t>(tile % tm) * kTile, n0 = static_cast<int64_t>(tile / tm) * kTile;
+  const int64_t m0 = static_cast<int64_t>(tile % tm) * kTileM, n0 = static_cast<int64_t>(tile / tm) * kTileN;
   const int ksteps = static_cast<int>(p.ksteps), steps_each = (ksteps + p.splits - 1) / p.splits;
   const int step0 = blockIdx.y * steps_each, step1 = step0 + steps_each < ksteps ? step0 + steps_each : ksteps;
-  const uint32_t ldsx = lds_address(&xs[0][0]), ldsc = lds_address(&cs[0][0]);
-  const int rows = p.M - m0 < kTile ? static_cast<int>(p.M - m0) : kTile, cols = p.N - n0 < kTile ? static_cast<int>(p.N - n0) : kTile;
+  const uint32_t lds0 = lds_address(lds);
+  const int rows = p.M - m0 < kTileM ? static_cast<int>(p.M - m0) : kTileM;
+  const int cols = p.N - n0 < kTileN ? static_cast<int>(p.N - n0) : kTileN;
 
   // Stage of x: a wave's load is 1 KB, 4 rows of 16 pieces; piece c of row r lies at slot c ^ (r % 16).  Offsets from the
-  // tile's first row stay below 2^32 (checked on the host).
-  constexpr int kLoads = StageBytes / 1024 / 4;
-  uint32_t xoff[kLoads], coff[2];
+  // tile's first row stay below 2^32 (checked on the host).  Rows and columns past the end re-read the last one.
+  constexpr int kXLoads = XBytes / 1024 / 8, kCodeLoads = CodeBytes / 1024 / 8;
+  uint32_t xoff[kXLoads], coff[kCodeLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int r = (wave * kLoads + i) * 4 + lane / Chunks, c = (lane % Chunks) ^ (r % Chunks);
+  for (int i = 0; i < kXLoads; ++i) {
+    const int r = (wave * kXLoads + i) * 4 + lane / Chunks, c = (lane % Chunks) ^ (r % Chunks);
     xoff[i] = static_cast<uint32_t>(r < rows ? r : rows - 1) * static_cast<uint32_t>(p.ldx * 2) + c * 16;
   }
-  // stage of codes: 64 bytes a column
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = (wave * 2 + i) * 16 + lane / 4;
+  for (int i = 0; i < kCodeLoads; ++i) {  // 64 bytes a column
+    const int r = (wave * kCodeLoads + i) * 16 + lane / 4;
     coff[i] = static_cast<uint32_t>(r < cols ? r : cols - 1) * static_cast<uint32_t>(p.pitch) + lane % 4 * 16;
   }
   const uint8_t* xbase = static_cast<const uint8_t*>(p.x) + m0 * p.ldx * 2;
   const uint8_t* cbase = p.codes + n0 * p.pitch;
-  auto fetch_x = [&](int step, int plane, int slot) {
-    const uint8_t* base = uniform(xbase + plane * p.plane + static_cast<int64_t>(step) * RowBytes);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) group_dma16(base, xoff[i], ldsx + slot * StageBytes + (wave * kLoads + i) * 1024);
-  };
-  auto fetch_codes = [&](int step, int slot) {
-    const uint8_t* base = uniform(cbase + static_cast<int64_t>(step) * 64);
-    // past the row's last block that block again (x is 0 there)
-    const int over = (step + 1) * 64 - static_cast<int>(p.pitch), back = over > 0 ? lane % 4 * 16 + over - 48 : 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      group_dma16(base, coff[i] - (back > 0 ? back : 0), ldsc + slot * CodeBytes + (wave * 2 + i) * 1024);
-  };
-  // scales of 4 blocks of 16 columns in a step (their bits; load_scale); the spans' groups are counted up
-  const int wide = p.s_dt == DIMQ_F32, group_spans = static_cast<int>(p.group / SP);
+  // Scales come as the aligned dwords that hold them, for the 64 columns of the wave.
+  const int wide = p.s_dt == DIMQ_F32;
+  const uint32_t groups = static_cast<uint32_t>(p.groups), group_spans = static_cast<uint32_t>(p.group / SP);
+  const uintptr_t sfirst = reinterpret_cast<uintptr_t>(p.scales) + ((n0 * p.groups) << (1 + wide));
+  const uint8_t* sbase = reinterpret_cast<const uint8_t*>(sfirst & ~uintptr_t(3));
+  const uint32_t sodd = static_cast<uint32_t>(sfirst >> 1) & 1;  // of a 16-bit scale
+  const auto column = [&](int n) { return static_cast<uint32_t>(n < cols ? n : cols - 1) * groups; };
+  const uint32_t sown = column(wn * 64 + lane);
   uint32_t goff[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int n = wn * 64 + c * 16 + col;
-    goff[c] = static_cast<uint32_t>(n < cols ? n : cols - 1) * static_cast<uint32_t>(p.groups);
-  }
-  const uint16_t* sbase = static_cast<const uint16_t*>(p.scales) + ((n0 * p.groups) << wide);
-  const uint32_t groups = static_cast<uint32_t>(p.groups);
-  auto raw_scale = [&](int c, uint32_t at) -> RawScale {
-    const uint32_t i = (goff[c] + at) << wide;
-    return {sbase[i], sbase[i + wide]};
-  };
-  RawScale rs[4][NS];
-  uint32_t g = static_cast<uint32_t>(step0) * NS / group_spans, phase = static_cast<uint32_t>(step0) * NS % group_spans;
-  auto fetch_scales = [&]() {
+  for (int c = 0; c < 4; ++c) goff[c] = column(wn * 64 + c * 16 + col);
+  GroupCount fetched(step0 * NS, group_spans, groups), used = fetched;
+
+  constexpr int kStageLoads = kXLoads + kCodeLoads + NS;  // a wave's
+  int fstep = step0, fplane = 0;
+  uint32_t at[NS];
+  auto fetch = [&](int slot) {
+    const uint32_t to = lds0 + slot * SlotBytes;
+    const uint8_t* xb = uniform(xbase + fplane * p.plane + static_cast<int64_t>(fstep) * RowBytes);
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
+    for (int i = 0; i < kXLoads; ++i) group_dma16(xb, xoff[i], to + (wave * kXLoads + i) * 1024);
+    const uint8_t* cb = uniform(cbase + static_cast<int64_t>(fstep) * 64);
+    // past the row's last block that block again (x is 0 there)
+    const int over = (fstep + 1) * 64 - static_cast<int>(p.pitch), back = over > 0 ? lane % 4 * 16 + over - 48 : 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) rs[c][s] = raw_scale(c, g < groups ? g : groups - 1);
-      if (++phase == static_cast<uint32_t>(group_spans)) phase = 0, ++g;
+    for (int i = 0; i < kCodeLoads; ++i)
+      group_dma16(cb, coff[i] - (back > 0 ? back : 0), to + XBytes + (wave * kCodeLoads + i) * 1024);
+    if (fplane == 0) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) at[s] = fetched.next();
     }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      group_dma4(sbase, (((sown + at[s]) << (1 + wide)) + 2 * sodd) & ~3u, to + XBytes + CodeBytes + (s * kTileN + wn * 64) * 4);
+    if (++fplane == P) fplane = 0, ++fstep;
   };
 
-  floatx4 acc[4][4];
+  // v: the span's products, added to acc times the scale when the next span begins, so that those fmas and the span's first
+  // decoding stand between its first LDS reads and their use; within a span the next step is decoded and read between the
+  // matrix instructions of this one.
+  constexpr int J = LB / 4;  // steps of 32 k in a span
+  floatx4 acc[4][4], v[4][4];
+  float scale[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[t][c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < 4; ++c) acc[t][c] = v[t][c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) scale[c] = 0.0f;
+  auto fold = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][c][i] = fmaf(scale[c], v[t][c][i], acc[t][c][i]);
+  };
 
-  if (step0 < step1) {
-    fetch_scales();
-    fetch_codes(step0, 0);
-    fetch_x(step0, 0, 0);
-  }
-  int slot = 0, cslot = 0;
-  for (int step = step0; step < step1; ++step) {
-    float sc[4][NS];
-#pragma unroll 1  // unrolled, the planes would keep their codes decoded and spill
-    for (int plane = 0; plane < P; ++plane) {
-      wait_vmcnt<0>();
-      __syncthreads();  // this stage is in the LDS, and the other one is free
-      if (plane == 0) {
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sc[c][s] = scale_of(p, rs[c][s]);
-      }
-      if (plane + 1 < P) {
-        fetch_x(step, plane + 1, slot ^ 1);
-      } else if (step + 1 < step1) {
-        fetch_scales();
-        fetch_codes(step + 1, cslot ^ 1);
-        fetch_x(step + 1, 0, slot ^ 1);
-      }
-      const uint8_t *st = xs[slot], *ct = cs[cslot] + (wn * 64 + col) * 64;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        uint32_t a[4][LB];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int r = wm * 64 + t * 16 + col, c0 = (s * SP + quarter * 2 * LB) / 8;  // piece of the row
-#pragma unroll
-          for (int i = 0; i < LB / 4; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(st + r * RowBytes + (((c0 + i) ^ (r % Chunks)) << 4));
-            a[t][4 * i] = v.x, a[t][4 * i + 1] = v.y, a[t][4 * i + 2] = v.z, a[t][4 * i + 3] = v.w;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[LB / 4], b[LB];
-          const uint8_t* q = ct + c * 1024 + s * (4 * LB) + quarter * LB;
-          if constexpr (LB == 16) {
-            const uint4 v = *reinterpret_cast<const uint4*>(q);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-          } else if constexpr (LB == 8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(q);
-            w[0] = v.x, w[1] = v.y;
-          } else {
-            w[0] = *reinterpret_cast<const uint32_t*>(q);
-          }
-          decode_span<MT, LB>(w, b);
-          floatx4 v[4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) v[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int j = 0; j < LB / 4; ++j)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) v[t] = mul_step<MT, LB>(a[t], b, j, v[t]);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][c][i] = fmaf(sc[c][s], v[t][i], acc[t][c][i]);
-        }
-      }
-      slot ^= 1;
-    }
-    cslot ^= 1;
-  }
-  // acc -= (sums of x) (s z)^T, the first of the k ranges for all of them; of the parts' products those above 2^-24
-  if (blockIdx.y == 0) {
-    const uint8_t* zbase = p.zeros ? p.zeros + n0 * p.groups : nullptr;
-    const int spans = ksteps * NS;
-    const float* sums = p.sums + m0 * spans;
+  const int stages = step1 > step0 ? (step1 - step0) * P : 0;
+  if (stages > 0) fetch(0);
+  if (stages > 1) fetch(1);
+  int slot = 0, uplane = 0;
+  for (int stage = 0; stage < stages; ++stage) {
+    // this stage is in the LDS for all waves, and the slot of the one before is free
+    if (stage + 1 < stages) wait_vmcnt<kStageLoads>();
+    else wait_vmcnt<0>();
+    lds_barrier();
+    if (stage + 2 < stages) fetch(slot == 0 ? 2 : slot - 1);
+    GroupCount span = used;
+    const uint8_t* st = lds + slot * SlotBytes;
+    const uint8_t* ct = st + XBytes + (wn * 64 + col) * 64 + quarter * LB;
+    const uint8_t* xt = st + (wm * 64 + col) * RowBytes;
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(st + XBytes + CodeBytes) + wn * 64 + col;
 #pragma unroll 1
-    for (int g0 = 0; g0 < spans; g0 += 32) {
-      const int mine = g0 + quarter * 8;
-      uint32_t a[4][3][4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int r = wm * 64 + t * 16 + col;
-        uint32_t v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = sums[static_cast<int64_t>(r < rows ? r : rows - 1) * spans + (mine + e < spans ? mine + e : spans - 1)];
-          v[e] = mine + e < spans ? __float_as_uint(f) : 0u;
-        }
-        split3(v, a[t][0], a[t][1], a[t][2]);
-      }
-      uint32_t at[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        at[e] = static_cast<uint32_t>(mine + e) / static_cast<uint32_t>(group_spans);
-        if (at[e] >= groups) at[e] = groups - 1;
-      }
+    for (int s = 0; s < NS; ++s) {
+      const uint32_t group_at = span.next();
+      uint32_t codes[4][J], a[2][4][4], b[2][4][4], raw[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t v[8], b[3][4];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float z = static_cast<float>(zbase ? zbase[goff[c] + at[e]] : 8u);
-          v[e] = __float_as_uint(-scale_of(p, raw_scale(c, at[e])) * z);
+        const uint8_t* q = ct + c * 1024 + s * (4 * LB);
+        if constexpr (LB == 16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(q);
+          codes[c][0] = w.x, codes[c][1] = w.y, codes[c][2] = w.z, codes[c][3] = w.w;
+        } else if constexpr (LB == 8) {
+          const uint2 w = *reinterpret_cast<const uint2*>(q);
+          codes[c][0] = w.x, codes[c][1] = w.y;
+        } else {
+          codes[c][0] = *reinterpret_cast<const uint32_t*>(q);
         }
-        split3(v, b[0], b[1], b[2]);
+        raw[c] = scales[s * kTileN + c * 16];
+      }
+      auto read_x = [&](int j) __attribute__((always_inline)) {
+        const int piece = ((s * SP + quarter * 2 * LB) / 8 + j) ^ col;
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
+        for (int t = 0; t < 4; ++t) {
+          const uint4 w = *reinterpret_cast<const uint4*>(xt + t * 16 * RowBytes + (piece << 4));
+          a[j & 1][t][0] = w.x, a[j & 1][t][1] = w.y, a[j & 1][t][2] = w.z, a[j & 1][t][3] = w.w;
+        }
+      };
+      auto decode = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-          for (int j = 0; i + j < 3; ++j)
+        for (int c = 0; c < 4; ++c) decode_step<MT>(codes[c][j], b[j & 1][c]);
+      };
+      read_x(0);
+      fold();
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[t][c] = mul_step<DIMQ_BF16, 4>(a[t][i], b[j], 0, acc[t][c]);
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t odd = (goff[c] + group_at + sodd) & 1;
+        const uint32_t half = odd ? raw[c] >> 16 : raw[c] & 0xffffu;
+        scale[c] = scale_of(p, wide ? RawScale{raw[c] & 0xffffu, raw[c] >> 16} : RawScale{half, half});
+      }
+      decode(0);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if (j + 1 < J) {
+          read_x(j + 1);
+          decode(j + 1);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            v[t][c] = mul_step<MT, 4>(a[j & 1][t], b[j & 1][c], 0, j == 0 ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : v[t][c]);
       }
     }
+    if (++uplane == P) uplane = 0, used = span;
+    slot = slot == 2 ? 0 : slot + 1;
   }
-  // 16 rows of the wave at a time through the LDS, so that a store is 64 neighbouring columns
+  fold();
+  // acc -= (sums of x) (s z)^T, the first of the k ranges for all of them; of the parts' products those above 2^-24
+  if (blockIdx.y == 0) {
+    const int64_t pitch = p.span_blocks * kPartBytes;
+    const uint8_t *ap[4], *bp[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int r = wm * 64 + t * 16 + col, n = wn * 64 + t * 16 + col;
+      ap[t] = p.sums + (m0 + (r < rows ? r : rows - 1)) * pitch + quarter * 16;
+      bp[t] = p.szs + (n0 + (n < cols ? n : cols - 1)) * pitch + quarter * 16;
+    }
+#pragma unroll 1
+    for (int64_t at = 0; at < pitch; at += kPartBytes) {
+      uint32_t a[3][4][4], b[3][4][4];
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint4 u = *reinterpret_cast<const uint4*>(ap[t] + at + q * 64), w = *reinterpret_cast<const uint4*>(bp[t] + at + q * 64);
+          a[q][t][0] = u.x, a[q][t][1] = u.y, a[q][t][2] = u.z, a[q][t][3] = u.w;
+          b[q][t][0] = w.x, b[q][t][1] = w.y, b[q][t][2] = w.z, b[q][t][3] = w.w;
+        }
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = 0; i + j < 3; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[t][c] = mul_step<DIMQ_BF16, 4>(a[i][t], b[j][c], 0, acc[t][c]);
+    }
+  }
+  // 16 rows of the wave at a time through the LDS, so that a lane stores 8 neighbouring columns
   __syncthreads();
-  float* mine = reinterpret_cast<float*>(&xs[0][0]) + wave * (16 * 65);
-  const int64_t n = n0 + wn * 64 + lane;
-  const float bias = p.bias && n < p.N && p.splits == 1 ? load_as_float(p.bias, p.bias_dt, n) : 0.0f;
+  float* mine = reinterpret_cast<float*>(lds) + wave * (16 * 68);
+  const int64_t n = n0 + wn * 64 + lane % 8 * 8;
+  const int left = p.N - n < 8 ? static_cast<int>(p.N - n) : 8;
+  float bias[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = p.bias && p.splits == 1 && j < left ? load_as_float(p.bias, p.bias_dt, n + j) : 0.0f;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine[(quarter * 4 + i) * 65 + c * 16 + col] = acc[t][c][i];
+      for (int i = 0; i < 4; ++i) mine[(quarter * 4 + i) * 68 + c * 16 + col] = acc[t][c][i];
     lds_barrier();
-    const int64_t first = m0 + wm * 64 + t * 16;
-    if (n < p.N) {
-#pragma unroll 4
-      for (int r = 0; r < 16; ++r) {
-        const int64_t m = first + r;
-        if (m >= p.M) break;
-        const float v = mine[r * 65 + lane] * row_scale(p, m);
-        if (p.splits > 1) {
-          p.part[(blockIdx.y * p.M + m) * p.N + n] = v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = h * 8 + lane / 8;
+      const int64_t m = m0 + wm * 64 + t * 16 + r;
+      if (m >= p.M || left <= 0) continue;
+      const float4* from = reinterpret_cast<const float4*>(mine + r * 68 + lane % 8 * 8);
+      const float4 x = from[0], y = from[1];
+      float o[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      const float by = row_scale(p, m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], by, bias[j]);
+      if (p.splits > 1) {
+        float* to = p.part + (blockIdx.y * p.M + m) * p.N + n;
+        if (left == 8) {
+          typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+          reinterpret_cast<f4*>(to)[0] = f4{o[0], o[1], o[2], o[3]};
+          reinterpret_cast<f4*>(to)[1] = f4{o[4], o[5], o[6], o[7]};
         } else {
-          const int64_t off = m * p.N + n;
-          store_from_float(p.y, p.y_dt, off, epi1(p.epi, off, v + bias));
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < left) to[j] = o[j];
         }
+      } else {
+        put8(p, m * p.N + n, left, o);
       }
     }
     lds_barrier();
@@ -602,22 +709,24 @@ constexpr int64_t kFewRows = 64;  // rows of the first kernel
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
 struct TilePlan {
-  int64_t ksteps, tm, tn, copy_bytes, sum_bytes, part_bytes;
+  int64_t ksteps, tm, tn, copy_bytes, sum_bytes, sz_bytes, part_bytes;
   int splits;
-  int64_t bytes() const { return copy_bytes + sum_bytes + part_bytes; }
+  int64_t bytes() const { return copy_bytes + sum_bytes + sz_bytes + part_bytes; }
 };
 // Tiles that leave CUs idle are cut along k, into parts of at least four steps.
 TilePlan tile_plan(int xt, int64_t M, int64_t K, int64_t N, bool in_place) {
   TilePlan t;
   t.ksteps = (K + kTileK - 1) / kTileK;
-  t.tm = (M + kTile - 1) / kTile, t.tn = (N + kTile - 1) / kTile;
+  t.tm = (M + kTileM - 1) / kTileM, t.tn = (N + kTileN - 1) / kTileN;
   const int64_t tiles = t.tm * t.tn, cus = device_cus();
   int64_t s = cus / tiles;
   if (s > t.ksteps / 4) s = t.ksteps / 4;
   t.splits = static_cast<int>(s < 1 ? 1 : s);
   t.splits = static_cast<int>((t.ksteps + (t.ksteps + t.splits - 1) / t.splits - 1) / ((t.ksteps + t.splits - 1) / t.splits));
   t.copy_bytes = in_place ? 0 : up256(M * t.ksteps * kTileK * 2) * planes_of(xt);
-  t.sum_bytes = up256(M * t.ksteps * (kTileK / 32) * 4);  // spans of 32 at the least
+  const int64_t blocks = (t.ksteps * (kTileK / 32) + 31) / 32;  // spans of 32 at the least
+  t.sum_bytes = up256(M * blocks * kPartBytes);
+  t.sz_bytes = up256(N * blocks * kPartBytes);
   t.part_bytes = t.splits > 1 ? t.splits * M * N * 4 : 0;
   return t;
 }
@@ -643,17 +752,19 @@ template <int XT, int LB>
 void launch_tile(GroupArgs p, const TilePlan& t, uint8_t* ws, hipStream_t s) {
   constexpr int ML = mul_type(XT), P = planes_of(XT);
   p.ksteps = t.ksteps, p.tiles_m = t.tm, p.tiles_n = t.tn, p.splits = t.splits;
-  float* sums = reinterpret_cast<float*>(ws + t.copy_bytes);
+  uint8_t *sums = ws + t.copy_bytes, *szs = sums + t.sum_bytes;
   p.plane = t.copy_bytes / P;
-  const int64_t blocks = (p.M * t.ksteps * (kTileK / 8) + 255) / 256;
-  hipLaunchKernelGGL((group_prep_kernel<XT, LB>), dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, p,
-                     t.copy_bytes ? ws : nullptr, sums);
+  p.span_blocks = (t.ksteps * (kTileK / (8 * LB)) + 31) / 32;
+  const int64_t blocks = (p.M * p.span_blocks * (32 * LB) + 255) / 256, most = (p.N * p.span_blocks * 4 + 255) / 256;
+  const int64_t grid_x = blocks > most ? blocks : most;
+  hipLaunchKernelGGL((group_prep_kernel<XT, LB>), dim3(static_cast<unsigned>(grid_x < 4096 ? grid_x : 4096), 2), dim3(256), 0, s,
+                     p, t.copy_bytes ? ws : nullptr, sums, szs);
   if (t.copy_bytes) {
     p.x = ws;
     p.ldx = t.ksteps * kTileK;
   }
-  p.sums = sums;
-  p.part = reinterpret_cast<float*>(ws + t.copy_bytes + t.sum_bytes);
+  p.sums = sums, p.szs = szs;
+  p.part = reinterpret_cast<float*>(szs + t.sz_bytes);
   const dim3 grid(static_cast<unsigned>(t.tm * t.tn), static_cast<unsigned>(t.splits));
   hipLaunchKernelGGL((group_tile_kernel<ML, LB, P>), grid, dim3(kTileThreads), 0, s, p);
   if (t.splits > 1) {

@@ -688,7 +688,8 @@ int dimq_distill_loss_backward(const void* student, int dtype, int64_t rows, int
 /* y = act(c[m] sum_g s[n, g] sum_{k in g} (q[n, k] - z[n, g]) x[m, k] + bias[n] +
  * residual[m, n]) for 4-bit weights with a scale per group of `group` (a
  * multiple of 32) elements of a row: codes [N, ceil(K / 32), 16], two a byte,
- * the earlier element in the low half (16-byte aligned), scales [N, G] and zeros
+ * the earlier element in the low half (16-byte aligned), scales [N, G] (read in
+ * whole aligned dwords) and zeros
  * [N, G] (0..15; nullable: 8), G = ceil(K / group).  x in a float dtype, or
  * DIMQ_E4M3 with x_scales[m] = c (else null).  Exact products, fp32 sums in a
  * fixed order, one rounding to y_dtype; bias [N] and residual [M, N] nullable,
