@@ -45,6 +45,7 @@ struct GroupArgs {
   float* part;            // [splits][M][N]
   int64_t tiles_m, tiles_n;
   int64_t span_blocks;    // blocks of 32 spans
+  uint32_t prep_first;    // work-groups of the first launch that prepare s z
   const uint8_t* sums;    // the zero points' product
   const uint8_t* szs;
 };
@@ -117,19 +118,26 @@ __device__ __forceinline__ floatx4 sum_span(const uint32_t (&a)[LB], floatx4 acc
   return mul_span<MT, LB>(a, b, acc);
 }
 
-// Scale i without a branch on its type: its first and last two bytes, which a 16-bit one has in common.
-struct RawScale {
-  uint32_t lo, hi;
+// Scales without a branch on their type: the aligned dword that holds scale i, and the scale of it.
+struct Scales {
+  const uint32_t* base;
+  uint32_t wide, odd, f16;  // odd: the first 16-bit scale is its dword's second half
+  __device__ __forceinline__ Scales(const void* scales, int dt, int64_t first) {
+    wide = dt == DIMQ_F32, f16 = dt == DIMQ_F16;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(scales) + (first << (1 + wide));
+    base = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+    odd = static_cast<uint32_t>(at >> 1) & 1;
+  }
+  template <class I>
+  __device__ __forceinline__ I index(I i) const { return wide ? i : (i + odd) >> 1; }
+  template <class I>
+  __device__ __forceinline__ uint32_t load(I i) const { return base[index(i)]; }
+  // low: the lowest bits of i
+  __device__ __forceinline__ float value(uint32_t raw, uint32_t low) const {
+    const uint32_t half = ((low + odd) & 1) ? raw >> 16 : raw & 0xffffu;
+    return f16 ? f16_bits_to_float(half) : __uint_as_float(wide ? raw : half << 16);
+  }
 };
-__device__ __forceinline__ RawScale load_scale(const GroupArgs& p, int64_t i) {
-  const uint16_t* s = static_cast<const uint16_t*>(p.scales);
-  const int wide = p.s_dt == DIMQ_F32;
-  return {s[i << wide], s[(i << wide) + wide]};
-}
-__device__ __forceinline__ float scale_of(const GroupArgs& p, const RawScale& r) {
-  const float wide = __uint_as_float(r.hi << 16 | (p.s_dt == DIMQ_F32 ? r.lo : 0u));  // fp32, and bf16's bits
-  return p.s_dt == DIMQ_F16 ? f16_bits_to_float(r.lo) : wide;
-}
 
 // Eight fp32 numbers as three planes of bf16 that add up to them (cut off, not rounded: nothing overflows).  An infinity
 // is in the first plane alone; a NaN is in the second, whatever the first plane's cut makes of it.
@@ -258,88 +266,107 @@ __device__ __forceinline__ void put8(const GroupArgs& p, int64_t off, int left, 
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
-// 16 MT rows by 16 columns a work-group; its 8 waves share out the spans, and their sums meet in the LDS.  A wave's loads
-// of U spans go out together.  Rows past M re-read the last one; they are not stored.
+// 16 MT rows by 16 NC columns a work-group; its 8 waves share out the spans, and their sums meet in the LDS.  A wave takes its
+// spans one after another: what hides their loads is the other waves of the CU (several spans' loads sent out together, or x
+// a span ahead, gained nothing at 4096 -> 4096 and lost up to a half where a wave has few spans, for their registers).
+// Lanes whose row is past M load no x: their sums are not stored.
 constexpr int kFewWaves = 8;
 
-template <int XT, int LB, int MT, int U>
+template <int XT, int LB, int MT, int NC>
 __global__ __launch_bounds__(64 * kFewWaves) void group_few_kernel(const GroupArgs p) {
   constexpr int ML = mul_type(XT), P = planes_of(XT), SP = 8 * LB;
-  __shared__ floatx4 red[kFewWaves][MT][64];
+  __shared__ floatx4 red[kFewWaves][MT * NC][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
-  const int64_t n = n0 + col < p.N ? n0 + col : p.N - 1;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NC), m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
   const int spans = static_cast<int>((p.nb * 32 + SP - 1) / SP), each = (spans + kFewWaves - 1) / kFewWaves;
   const int from = wave * each, to = from + each < spans ? from + each : spans;
-  const uint8_t* cw = p.codes + n * p.pitch;
-  const int group_spans = static_cast<int>(p.group / SP);  // a group is a whole number of spans
-  floatx4 acc[MT];
+  const uint32_t group_spans = static_cast<uint32_t>(p.group / SP);  // a group is a whole number of spans
+  const uint8_t* cw[NC];
+  int64_t gn[NC];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = from; s0 < to; s0 += U) {
-    uint32_t codes[U][LB / 4];
-    RawScale rs[U];
-    uint32_t z[U];
-    RawX<XT, LB> rx[U][MT];
+  for (int c = 0; c < NC; ++c) {
+    const int64_t n = n0 + 16 * c + col < p.N ? n0 + 16 * c + col : p.N - 1;
+    cw[c] = p.codes + n * p.pitch;
+    gn[c] = n * p.groups;
+  }
+  const Scales scales(p.scales, p.s_dt, 0);
+  const uint8_t* zeros = p.zeros ? p.zeros : p.codes;  // as long, and not used then
+  floatx4 acc[MT][NC];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int sp = s0 + u < to ? s0 + u : to - 1;
-      // a lane's codes past the row's last block read that block's (x is 0 there)
-      int64_t at = static_cast<int64_t>(sp) * (4 * LB) + quarter * LB;
-      if (at + LB > p.pitch) at = p.pitch - LB < 0 ? 0 : p.pitch - LB;
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[t][c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int sp = from; sp < to; ++sp) {
+    // a lane's codes past the row's last block read that block's (x is 0 there)
+    int64_t at = static_cast<int64_t>(sp) * (4 * LB) + quarter * LB;
+    if (at + LB > p.pitch) at = p.pitch - LB;
+    uint32_t codes[NC][LB / 4], rs[NC], z[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
       if constexpr (LB == 16) {
-        const uint4 c = *reinterpret_cast<const uint4*>(cw + at);
-        codes[u][0] = c.x, codes[u][1] = c.y, codes[u][2] = c.z, codes[u][3] = c.w;
+        const uint4 w = *reinterpret_cast<const uint4*>(cw[c] + at);
+        codes[c][0] = w.x, codes[c][1] = w.y, codes[c][2] = w.z, codes[c][3] = w.w;
       } else if constexpr (LB == 8) {
-        const uint2 c = *reinterpret_cast<const uint2*>(cw + at);
-        codes[u][0] = c.x, codes[u][1] = c.y;
+        const uint2 w = *reinterpret_cast<const uint2*>(cw[c] + at);
+        codes[c][0] = w.x, codes[c][1] = w.y;
       } else {
-        codes[u][0] = *reinterpret_cast<const uint32_t*>(cw + at);
-      }
-      const int64_t gi = n * p.groups + sp / group_spans;
-      rs[u] = load_scale(p, gi);
-      z[u] = p.zeros ? p.zeros[gi] : 8u;
-      const int64_t k0 = static_cast<int64_t>(sp) * SP + quarter * (2 * LB);
-      const bool fast = p.vec && static_cast<int64_t>(sp + 1) * SP <= p.K;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int64_t m = m0 + 16 * t + col;
-        rx[u][t].load(p, m < p.M ? m : p.M - 1, k0, fast);
+        codes[c][0] = *reinterpret_cast<const uint32_t*>(cw[c] + at);
       }
     }
+    RawX<XT, LB> rx[MT];
+    const int64_t k0 = static_cast<int64_t>(sp) * SP + quarter * (2 * LB);
+    const bool fast = p.vec && static_cast<int64_t>(sp + 1) * SP <= p.K;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s0 + u >= to) break;
-      uint32_t b[LB];
-      decode_span<ML, LB>(codes[u], b);
-      const float s = scale_of(p, rs[u]), zf = static_cast<float>(z[u]);
+    for (int t = 0; t < MT; ++t) {
+      const int64_t m = m0 + 16 * t + col;
+      if (m < p.M) rx[t].load(p, m, k0, fast);
+    }
+    const uint32_t g = static_cast<uint32_t>(sp) / group_spans;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        uint32_t a[P][LB];
-        rx[u][t].planes(a);
-        floatx4 q = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, x = q;
+    for (int c = 0; c < NC; ++c) {
+      rs[c] = scales.load(gn[c] + g);
+      z[c] = zeros[gn[c] + g];
+    }
+    uint32_t b[NC][LB];
+    float s[NC], zf[NC];
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          q = mul_span<ML, LB>(a[i], b, q);
-          x = sum_span<ML, LB>(a[i], x);
-        }
+    for (int c = 0; c < NC; ++c) {
+      decode_span<ML, LB>(codes[c], b[c]);
+      s[c] = scales.value(rs[c], static_cast<uint32_t>(gn[c]) + g);
+      zf[c] = p.zeros ? static_cast<float>(z[c]) : 8.0f;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(s, fmaf(-zf, x[i], q[i]), acc[t][i]);
+    for (int t = 0; t < MT; ++t) {
+      uint32_t a[P][LB];
+      rx[t].planes(a);
+      floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < P; ++i) x = sum_span<ML, LB>(a[i], x);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        floatx4 q = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < P; ++i) q = mul_span<ML, LB>(a[i], b[c], q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][c][i] = fmaf(s[c], fmaf(-zf[c], x[i], q[i]), acc[t][c][i]);
       }
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) red[wave][t * NC + c][lane] = acc[t][c];
   __syncthreads();
-  if (wave >= MT) return;
+  if (wave >= MT * NC) return;
+  const int64_t n = n0 + 16 * (wave % NC) + col;
   floatx4 v = red[0][wave][lane];
 #pragma unroll
   for (int w = 1; w < kFewWaves; ++w) v += red[w][wave][lane];
-  if (n0 + col >= p.N) return;
+  if (n >= p.N) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + 16 * wave + 4 * quarter + i;
-    if (m < p.M) put_output(p, m, n0 + col, v[i] * row_scale(p, m));
+    const int64_t m = m0 + 16 * (wave / NC) + 4 * quarter + i;
+    if (m < p.M) put_output(p, m, n, v[i] * row_scale(p, m));
   }
 }
 
@@ -356,52 +383,68 @@ __global__ __launch_bounds__(64 * kFewWaves) void group_few_kernel(const GroupAr
 constexpr int kTileM = 128, kTileN = 256, kTileK = 128, kTileThreads = 512;
 constexpr int kSlots = 3;
 
+// i / per, in 32 bits where they do (a 64-bit division is a hundred instructions).
+__device__ __forceinline__ int64_t quotient(int64_t i, uint32_t per) {
+  return i <= 0xffffffffll ? static_cast<int64_t>(static_cast<uint32_t>(i) / per) : i / per;
+}
+
 // Both operands of the zero points' product: [row][blocks of 32 spans][3 parts][32 spans] in bf16, zeros behind the last span.
 constexpr int kPartBytes = 3 * 32 * 2;  // of a block
+constexpr int kPrepEach = 4;            // pieces of 8 elements of x a thread
 
 // sums: x's, [M]; szs: -s z, [N]; out (nullable): x padded with zeros to whole k steps, [planes][M][ksteps 128].
 template <int XT, int LB>
 __global__ __launch_bounds__(256) void group_prep_kernel(const GroupArgs p, uint8_t* out, uint8_t* sums, uint8_t* szs) {
   constexpr int SP = 8 * LB;
   const int64_t blocks = p.span_blocks;
-  if (blockIdx.y == 1) {  // 8 spans a thread
+  if (blockIdx.x < p.prep_first) {  // 8 spans a thread
+    const Scales scales(p.scales, p.s_dt, 0);
     const uint32_t group_spans = static_cast<uint32_t>(p.group / SP), per = static_cast<uint32_t>(blocks) * 4;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < p.N * per; i += static_cast<int64_t>(gridDim.x) * 256) {
-      const int64_t n = i / per;
-      const uint32_t first = static_cast<uint32_t>(i - n * per) * 8;
-      uint32_t v[8], o[3][4];
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= p.N * per) return;
+    const int64_t n = quotient(i, per);
+    const uint32_t first = static_cast<uint32_t>(i - n * per) * 8;
+    uint32_t v[8], o[3][4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t g = (first + e) / group_spans;
-        const int64_t at = n * p.groups + (g < p.groups ? g : p.groups - 1);
-        const float sz = -scale_of(p, load_scale(p, at)) * static_cast<float>(p.zeros ? p.zeros[at] : 8u);
-        v[e] = g < p.groups ? __float_as_uint(sz) : 0u;
-      }
-      split3(v, o[0], o[1], o[2]);
-      uint8_t* to = szs + (n * blocks + first / 32) * kPartBytes + first % 32 * 2;
-#pragma unroll
-      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * 64) = make_uint4(o[q][0], o[q][1], o[q][2], o[q][3]);
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t g = (first + e) / group_spans;
+      const int64_t at = n * p.groups + (g < p.groups ? g : p.groups - 1);
+      const float sz = -scales.value(scales.load(at), static_cast<uint32_t>(at)) * static_cast<float>(p.zeros ? p.zeros[at] : 8u);
+      v[e] = g < p.groups ? __float_as_uint(sz) : 0u;
     }
+    split3(v, o[0], o[1], o[2]);
+    uint8_t* to = szs + (n * blocks + first / 32) * kPartBytes + first % 32 * 2;
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * 64) = make_uint4(o[q][0], o[q][1], o[q][2], o[q][3]);
     return;
   }
   const uint32_t per = static_cast<uint32_t>(blocks) * (32 * SP / 8);  // a multiple of 16: 16 neighbouring lanes share a row
-  const int64_t total = p.M * per, kp = p.ksteps * kTileK;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t m = i / per, k0 = (i - m * per) * 8;
-    RawX<XT, 4> r;
-    r.load(p, m, k0, p.vec && k0 + 8 <= p.K);
+  const int64_t total = p.M * per, kp = p.ksteps * kTileK, base = static_cast<int64_t>(blockIdx.x - p.prep_first) * (256 * kPrepEach);
+  RawX<XT, 4> r[kPrepEach];
+  int64_t m[kPrepEach], k0[kPrepEach];
+#pragma unroll
+  for (int e = 0; e < kPrepEach; ++e) {
+    const int64_t i = base + e * 256 + threadIdx.x;
+    m[e] = i < total ? quotient(i, per) : p.M;
+    k0[e] = i - m[e] * per;
+    k0[e] *= 8;
+    if (m[e] < p.M) r[e].load(p, m[e], k0[e], p.vec && k0[e] + 8 <= p.K);
+  }
+#pragma unroll
+  for (int e = 0; e < kPrepEach; ++e) {
+    if (m[e] >= p.M) return;  // with its 16 neighbours
     uint32_t a[planes_of(XT)][4];
-    r.planes(a);
-    if (out && k0 < kp) {
+    r[e].planes(a);
+    if (out && k0[e] < kp) {
 #pragma unroll
       for (int q = 0; q < planes_of(XT); ++q)
-        *reinterpret_cast<uint4*>(out + q * p.plane + (m * kp + k0) * 2) = make_uint4(a[q][0], a[q][1], a[q][2], a[q][3]);
+        *reinterpret_cast<uint4*>(out + q * p.plane + (m[e] * kp + k0[e]) * 2) = make_uint4(a[q][0], a[q][1], a[q][2], a[q][3]);
     }
     float s = 0.0f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      if constexpr (XT == DIMQ_F32) s += __uint_as_float(r.w[q]);
-      else if constexpr (XT == DIMQ_F16) s += f16_bits_to_float((r.w[q >> 1] >> (16 * (q & 1))) & 0xffffu);
+      if constexpr (XT == DIMQ_F32) s += __uint_as_float(r[e].w[q]);
+      else if constexpr (XT == DIMQ_F16) s += f16_bits_to_float((r[e].w[q >> 1] >> (16 * (q & 1))) & 0xffffu);
       else s += bf16_bits_to_float((a[0][q >> 1] >> (16 * (q & 1))) & 0xffffu);
     }
 #pragma unroll
@@ -410,8 +453,8 @@ __global__ __launch_bounds__(256) void group_prep_kernel(const GroupArgs p, uint
       const uint32_t v[8] = {__float_as_uint(s), 0, 0, 0, 0, 0, 0, 0};
       uint32_t o[3][4];
       split3(v, o[0], o[1], o[2]);
-      const int64_t span = k0 / SP;
-      uint8_t* to = sums + (m * blocks + span / 32) * kPartBytes + span % 32 * 2;
+      const int64_t span = k0[e] / SP;
+      uint8_t* to = sums + (m[e] * blocks + span / 32) * kPartBytes + span % 32 * 2;
 #pragma unroll
       for (int q = 0; q < 3; ++q) *reinterpret_cast<uint16_t*>(to + q * 64) = static_cast<uint16_t>(o[q][0]);
     }
@@ -486,11 +529,9 @@ __global__ __launch_bounds__(kTileThreads) void group_tile_kernel(const GroupArg
   const uint8_t* xbase = static_cast<const uint8_t*>(p.x) + m0 * p.ldx * 2;
   const uint8_t* cbase = p.codes + n0 * p.pitch;
   // Scales come as the aligned dwords that hold them, for the 64 columns of the wave.
-  const int wide = p.s_dt == DIMQ_F32;
   const uint32_t groups = static_cast<uint32_t>(p.groups), group_spans = static_cast<uint32_t>(p.group / SP);
-  const uintptr_t sfirst = reinterpret_cast<uintptr_t>(p.scales) + ((n0 * p.groups) << (1 + wide));
-  const uint8_t* sbase = reinterpret_cast<const uint8_t*>(sfirst & ~uintptr_t(3));
-  const uint32_t sodd = static_cast<uint32_t>(sfirst >> 1) & 1;  // of a 16-bit scale
+  const Scales scaled(p.scales, p.s_dt, n0 * p.groups);
+  const uint8_t* sbase = reinterpret_cast<const uint8_t*>(scaled.base);
   const auto column = [&](int n) { return static_cast<uint32_t>(n < cols ? n : cols - 1) * groups; };
   const uint32_t sown = column(wn * 64 + lane);
   uint32_t goff[4];
@@ -518,7 +559,7 @@ __global__ __launch_bounds__(kTileThreads) void group_tile_kernel(const GroupArg
     }
 #pragma unroll
     for (int s = 0; s < NS; ++s)
-      group_dma4(sbase, (((sown + at[s]) << (1 + wide)) + 2 * sodd) & ~3u, to + XBytes + CodeBytes + (s * kTileN + wn * 64) * 4);
+      group_dma4(sbase, scaled.index(sown + at[s]) * 4, to + XBytes + CodeBytes + (s * kTileN + wn * 64) * 4);
     if (++fplane == P) fplane = 0, ++fstep;
   };
 
@@ -592,9 +633,7 @@ __global__ __launch_bounds__(kTileThreads) void group_tile_kernel(const GroupArg
       fold();
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const uint32_t odd = (goff[c] + group_at + sodd) & 1;
-        const uint32_t half = odd ? raw[c] >> 16 : raw[c] & 0xffffu;
-        scale[c] = scale_of(p, wide ? RawScale{raw[c] & 0xffffu, raw[c] >> 16} : RawScale{half, half});
+        scale[c] = scaled.value(raw[c], goff[c] + group_at);
       }
       decode(0);
 #pragma unroll
@@ -690,13 +729,34 @@ __global__ __launch_bounds__(kTileThreads) void group_tile_kernel(const GroupArg
   }
 }
 
+// Adds the k ranges' sums, 8 neighbouring outputs of a row a thread (fewer at its end).
 __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs p) {
-  const int64_t total = p.M * p.N;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-    float v = p.part[i];
-    for (int s = 1; s < p.splits; ++s) v += p.part[s * total + i];
-    const int64_t m = i / p.N;
-    put_output(p, m, i - m * p.N, v);
+  const uint32_t per = static_cast<uint32_t>((p.N + 7) / 8);
+  const int64_t total = p.M * p.N, pieces = p.M * per;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t m = quotient(i, per), n = (i - m * per) * 8, off = m * p.N + n;
+    const int left = p.N - n < 8 ? static_cast<int>(p.N - n) : 8;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p.bias && j < left ? load_as_float(p.bias, p.bias_dt, n + j) : 0.0f;
+    float sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float* from = p.part + s * total + off;
+      if (left == 8) {
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+        const f4 x = reinterpret_cast<const f4*>(from)[0], y = reinterpret_cast<const f4*>(from)[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += x[j], sum[4 + j] += y[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += j < left ? from[j] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += sum[j];
+    put8(p, off, left, v);
   }
 }
 
@@ -704,7 +764,14 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs p) {
 
 int span_bytes(int64_t group) { return group % 128 == 0 ? 16 : group % 64 == 0 ? 8 : 4; }
 
-constexpr int64_t kFewRows = 64;  // rows of the first kernel
+// Products of fewer multiply-adds than this run on the first kernel, larger ones on the tiles, whose three launches cost about
+// 20 us before the first product.  At K 4096, groups of 128, bf16 (in us, first kernel / tiles): 64 x 4096 16 / 29, 128 x 4096
+// 28 / 34, 256 x 4096 52 / 37, 64 x 12288 42 / 38.
+constexpr double kFewProducts = 2.5e9;
+bool few_rows(int64_t M, int64_t K, int64_t N, int variant) {
+  if (variant == DIMQ_VARIANT_MFMA || M > int64_t{65535} * 16) return false;  // row blocks of one launch
+  return variant == DIMQ_VARIANT_SMALL_M || static_cast<double>(M) * static_cast<double>(K) * static_cast<double>(N) < kFewProducts;
+}
 
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
@@ -739,13 +806,34 @@ bool rows_in_place(const void* x, int xt, int64_t M, int64_t K, int64_t ldx) {
   return x_size(xt) == 2 && K % kTileK == 0 && rows_aligned(x, xt, M, ldx) && ldx < kMostApart;
 }
 
+// Blocks of 16 rows and of 16 columns a work-group: more columns read x less often, more rows the codes, but both leave fewer
+// work-groups.  In us, at 4096 -> 4096 / 4096 -> 12288, groups of 128, bf16 (MT x NC): 1 row 1x1 6.5 / 13.4, 1x4 15.1 / 15.5; 16
+// rows 1x1 9.7 / 21.8, 1x4 17.9 / 18.4; 32 rows 1x1 15.8 / 40.0, 1x2 12.5 / 30.0, 2x2 16.1 / 29.5; 64 rows 1x1 27.8 / 76.1, 2x2
+// 16.3 / 43.1, 4x1 20.4 / 57.8; fp32, 37 rows: 1x1 40.9 / 117, 1x4 24.8 / 64.7, 2x2 30.8 / 79.4.  Groups of 32, whose codes are
+// loaded by 4 bytes: 32 rows 1x1 31.9, 1x2 27.8, 2x1 21.4; 64 rows 2x2 31.6, 2x1 38.6, 4x1 28.0.
 template <int XT, int LB>
 void launch_few(const GroupArgs& p, hipStream_t s) {
-  const unsigned gx = static_cast<unsigned>((p.N + 15) / 16);
-  const dim3 threads(64 * kFewWaves);
-  if (p.M <= 16) hipLaunchKernelGGL((group_few_kernel<XT, LB, 1, 4>), dim3(gx), threads, 0, s, p);
-  else if (p.M <= 32) hipLaunchKernelGGL((group_few_kernel<XT, LB, 2, 2>), dim3(gx), threads, 0, s, p);
-  else hipLaunchKernelGGL((group_few_kernel<XT, LB, 4, 1>), dim3(gx, static_cast<unsigned>((p.M + 63) / 64)), threads, 0, s, p);
+  const int64_t gm = (p.M + 15) / 16, gn = (p.N + 15) / 16;
+  const auto go = [&](auto kernel, int mt, int nc) {
+    const dim3 grid(static_cast<unsigned>((gn + nc - 1) / nc), static_cast<unsigned>((gm + mt - 1) / mt));
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kFewWaves), 0, s, p);
+  };
+  const bool wide = gn >= 128, widest = gn >= 640;  // columns for half of the CUs, for all of them with 4 blocks each
+  if constexpr (XT == DIMQ_F32) {
+    if (LB == 4 && wide && gm >= 2) go(group_few_kernel<XT, LB, 2, 2>, 2, 2);
+    else if ((widest && p.M > 4) || (wide && gm >= 3)) go(group_few_kernel<XT, LB, 1, 4>, 1, 4);
+    else if (wide && gm == 2) go(group_few_kernel<XT, LB, 1, 2>, 1, 2);
+    else go(group_few_kernel<XT, LB, 1, 1>, 1, 1);
+  } else if constexpr (LB == 4) {
+    if (wide && gm >= 3) go(group_few_kernel<XT, LB, 4, 1>, 4, 1);
+    else if (wide && gm == 2) go(group_few_kernel<XT, LB, 2, 1>, 2, 1);
+    else go(group_few_kernel<XT, LB, 1, 1>, 1, 1);
+  } else {
+    if ((wide && gm >= 3) || (widest && gm == 2)) go(group_few_kernel<XT, LB, 2, 2>, 2, 2);
+    else if (wide && gm == 2) go(group_few_kernel<XT, LB, 1, 2>, 1, 2);
+    else if (widest && p.M > 4) go(group_few_kernel<XT, LB, 1, 4>, 1, 4);
+    else go(group_few_kernel<XT, LB, 1, 1>, 1, 1);
+  }
 }
 
 template <int XT, int LB>
@@ -755,10 +843,10 @@ void launch_tile(GroupArgs p, const TilePlan& t, uint8_t* ws, hipStream_t s) {
   uint8_t *sums = ws + t.copy_bytes, *szs = sums + t.sum_bytes;
   p.plane = t.copy_bytes / P;
   p.span_blocks = (t.ksteps * (kTileK / (8 * LB)) + 31) / 32;
-  const int64_t blocks = (p.M * p.span_blocks * (32 * LB) + 255) / 256, most = (p.N * p.span_blocks * 4 + 255) / 256;
-  const int64_t grid_x = blocks > most ? blocks : most;
-  hipLaunchKernelGGL((group_prep_kernel<XT, LB>), dim3(static_cast<unsigned>(grid_x < 4096 ? grid_x : 4096), 2), dim3(256), 0, s,
-                     p, t.copy_bytes ? ws : nullptr, sums, szs);
+  p.prep_first = static_cast<uint32_t>((p.N * p.span_blocks * 4 + 255) / 256);
+  const int64_t blocks = (p.M * p.span_blocks * (32 * LB) + 256 * kPrepEach - 1) / (256 * kPrepEach);
+  hipLaunchKernelGGL((group_prep_kernel<XT, LB>), dim3(static_cast<unsigned>(p.prep_first + blocks)), dim3(256), 0, s, p,
+                     t.copy_bytes ? ws : nullptr, sums, szs);
   if (t.copy_bytes) {
     p.x = ws;
     p.ldx = t.ksteps * kTileK;
@@ -768,8 +856,8 @@ void launch_tile(GroupArgs p, const TilePlan& t, uint8_t* ws, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(t.tm * t.tn), static_cast<unsigned>(t.splits));
   hipLaunchKernelGGL((group_tile_kernel<ML, LB, P>), grid, dim3(kTileThreads), 0, s, p);
   if (t.splits > 1) {
-    const int64_t blocks = (p.M * p.N + 255) / 256;
-    hipLaunchKernelGGL(group_join_kernel, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, p);
+    const int64_t pieces = (p.M * ((p.N + 7) / 8) + 255) / 256;
+    hipLaunchKernelGGL(group_join_kernel, dim3(static_cast<unsigned>(pieces < 4096 ? pieces : 4096)), dim3(256), 0, s, p);
   }
 }
 
@@ -778,8 +866,9 @@ void launch_tile(GroupArgs p, const TilePlan& t, uint8_t* ws, hipStream_t s) {
 
 using namespace dimq;
 
-extern "C" int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int64_t N) {
-  if (M <= kFewRows || K <= 0 || N <= 0) return 0;
+extern "C" int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int64_t N,
+                                                       int variant) {
+  if (M <= 0 || K <= 0 || N <= 0 || few_rows(M, K, N, variant)) return 0;
   if (x_dtype != DIMQ_F32 && x_dtype != DIMQ_F16 && x_dtype != DIMQ_BF16 && x_dtype != DIMQ_E4M3) return 0;
   const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
   return t.bytes();
@@ -788,8 +877,8 @@ extern "C" int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtyp
 extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const float* x_scales,
                                    const uint8_t* codes, const void* scales, int scales_dtype, const uint8_t* zeros,
                                    int64_t group, const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype,
-                                   const void* residual, int residual_dtype, int activation, void* workspace,
-                                   int64_t workspace_bytes, void* stream) {
+                                   const void* residual, int residual_dtype, int activation, int variant,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
   DIMQ_CHECK(x_dtype == DIMQ_F32 || x_dtype == DIMQ_F16 || x_dtype == DIMQ_BF16 || x_dtype == DIMQ_E4M3,
              "linear_grouped: input must be fp32, fp16, bf16 or e4m3");
   DIMQ_CHECK((x_dtype == DIMQ_E4M3) == (x_scales != nullptr) || M == 0, "linear_grouped: e4m3 rows, and no others, have scales");
@@ -803,6 +892,7 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
   DIMQ_CHECK(group > 0 && group % 32 == 0, "linear_grouped: the group size must be a positive multiple of 32");
   DIMQ_CHECK(M <= 1 || ldx >= K, "linear_grouped: row stride is below the row length");
   DIMQ_CHECK(activation >= DIMQ_ACT_NONE && activation <= DIMQ_ACT_GELU, "unknown activation %d", activation);
+  DIMQ_CHECK(variant >= DIMQ_VARIANT_AUTO && variant <= DIMQ_VARIANT_MFMA, "unknown variant %d", variant);
   DIMQ_CHECK(!bias || is_float_dtype(bias_dtype), "linear_grouped: bias must be a float type");
   DIMQ_CHECK(!residual || is_float_dtype(residual_dtype), "linear_grouped: residual must be a float type");
   if (M == 0) return DIMQ_OK;
@@ -829,14 +919,14 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
     case DIMQ_BF16: DIMQ_GROUP_LB(F, DIMQ_BF16, __VA_ARGS__) break;    \
     default: DIMQ_GROUP_LB(F, DIMQ_E4M3, __VA_ARGS__)                  \
   }
-  if (M <= kFewRows) {
+  if (few_rows(M, K, N, variant)) {
     DIMQ_GROUP_XT(launch_few, p, s)
   } else {
     const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
     DIMQ_CHECK(workspace_bytes >= t.bytes() && aligned(workspace, 16),
                "linear_grouped: the workspace is too small or not 16-byte aligned");
     DIMQ_CHECK(t.tm * t.tn < (int64_t)1 << 24, "linear_grouped: too many outputs for one launch");
-    DIMQ_CHECK(t.ksteps * kTileK < kMostApart, "linear_grouped: more than 64 rows must be shorter than 2^23 elements");
+    DIMQ_CHECK(t.ksteps * kTileK < kMostApart, "linear_grouped: rows of 2^23 elements or more take fewer rows");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     DIMQ_GROUP_XT(launch_tile, p, t, ws, s)
   }

@@ -860,7 +860,8 @@ TORCH_LIBRARY_FRAGMENT(dimq, m) {
         "-> (Tensor, Tensor)");
   m.def("rms_norm_e4m3(Tensor x, Tensor? weight, float eps, Tensor? residual=None) -> (Tensor, Tensor, Tensor)");
   m.def("linear_grouped(Tensor x, Tensor codes, Tensor scales, Tensor? zeros, int group_size, Tensor? bias=None, "
-        "Tensor? x_scales=None, Tensor? residual=None, int activation=0, ScalarType? out_dtype=None) -> Tensor");
+        "Tensor? x_scales=None, Tensor? residual=None, int activation=0, ScalarType? out_dtype=None, int variant=0) "
+        "-> Tensor");
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top=0) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 

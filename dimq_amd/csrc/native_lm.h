@@ -262,7 +262,7 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
 
 Tensor linear_grouped(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& zeros, int64_t group,
                       const OptTensor& bias, const OptTensor& x_scales, const OptTensor& residual, int64_t activation,
-                      std::optional<at::ScalarType> out_dtype) {
+                      std::optional<at::ScalarType> out_dtype, int64_t variant) {
   const char* op = "linear_grouped";
   TORCH_CHECK_NOT_IMPLEMENTED(x.is_cuda(), op, " expects a CUDA input");
   const bool q8 = x.scalar_type() == at::kFloat8_e4m3fn;
@@ -318,10 +318,11 @@ Tensor linear_grouped(const Tensor& x, const Tensor& codes, const Tensor& scales
   const int xdt = q8 ? static_cast<int>(DIMQ_E4M3) : dt(x);
   const Tensor y = at::empty(shape, x.options().dtype(odt));
   const On on(x);
-  const Tensor ws = workspace(dimq_linear_grouped_workspace_bytes(ptr(t), xdt, M, K, ld, N), c);
+  const Tensor ws = workspace(dimq_linear_grouped_workspace_bytes(ptr(t), xdt, M, K, ld, N, static_cast<int>(variant)), c);
   check_rc(dimq_linear_grouped(ptr(t), xdt, M, K, ld, static_cast<float*>(ptr(xs)), u8(c), ptr(s), dt(s),
                                static_cast<uint8_t*>(ptr(z)), group, b.p, b.dtype, N, ptr(y), dt(y), r.p, r.dtype,
-                               static_cast<int>(activation), ptr(ws), ws.defined() ? ws.numel() : 0, on.stream));
+                               static_cast<int>(activation), static_cast<int>(variant), ptr(ws), ws.defined() ? ws.numel() : 0,
+                               on.stream));
   return y;
 }
 
@@ -329,9 +330,9 @@ Tensor linear_grouped(const Tensor& x, const Tensor& codes, const Tensor& scales
 // it in the backward pass.
 Tensor linear_grouped_graph(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& zeros, int64_t group,
                             const OptTensor& bias, const OptTensor& x_scales, const OptTensor& residual, int64_t activation,
-                            std::optional<at::ScalarType> out_dtype) {
+                            std::optional<at::ScalarType> out_dtype, int64_t variant) {
   const Direct<&linear_grouped> direct{"linear_grouped"};
   return wants_grad(x) || wants_grad(scales) || wants_grad(bias) || wants_grad(x_scales) || wants_grad(residual)
-             ? direct.op(x, codes, scales, zeros, group, bias, x_scales, residual, activation, out_dtype)
-             : direct(x, codes, scales, zeros, group, bias, x_scales, residual, activation, out_dtype);
+             ? direct.op(x, codes, scales, zeros, group, bias, x_scales, residual, activation, out_dtype, variant)
+             : direct(x, codes, scales, zeros, group, bias, x_scales, residual, activation, out_dtype, variant);
 }

@@ -354,18 +354,19 @@ def quantize_grouped(w: torch.Tensor, group_size: int = 128, *, symmetric: bool 
 def dimq_linear_grouped(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None,
                         group_size: int, bias: torch.Tensor | None = None, *, x_scales: torch.Tensor | None = None,
                         residual: torch.Tensor | None = None, activation: str | None = None,
-                        out_dtype: torch.dtype | None = None) -> torch.Tensor:
+                        out_dtype: torch.dtype | None = None, variant: str = "auto") -> torch.Tensor:
     """``act(x W^T + bias + residual)`` with ``W[n, k] = scales[n, k // group_size] * (q[n, k] - zeros[n, k // group_size])``,
     q the 4-bit codes as :func:`quantize_grouped` packs them, zeros (uint8, at most 15) 8 where None.  x in fp32, fp16 or
     bf16, or in torch.float8_e4m3fn with ``x_scales`` (fp32, one for each row, as :func:`rms_norm_e4m3` gives), which
     multiplies the row.  Neither x nor W is rounded, sums are fp32; a row of x that holds a NaN or an infinity gives outputs that
     are not finite; the output in ``out_dtype`` (x's by default, bf16 for
-    float8).  For serving: a backward pass through it raises."""
+    float8).  ``variant``: "small_m" one launch, "mfma" tiles (a workspace and up to three launches), "auto" by size.  For
+    serving: a backward pass through it raises."""
     require_extension()
     from ._C import _native
 
     return _native.linear_grouped(x, codes, scales, zeros, int(group_size), bias, x_scales, residual,
-                                  ACTIVATIONS[activation], out_dtype)
+                                  ACTIVATIONS[activation], out_dtype, VARIANTS[variant])
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *,

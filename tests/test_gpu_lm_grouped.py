@@ -62,23 +62,28 @@ SHAPES = [(1, 32, 1), (1, 33, 15), (3, 1000, 130), (16, 128, 16), (2, 4096, 48),
           (90, 31, 3)]
 
 
+BOTH = pytest.mark.parametrize("variant", ["small_m", "mfma"])
+
+
+@BOTH
 @pytest.mark.parametrize("dt", XTYPES)
 @pytest.mark.parametrize("m,k,n", SHAPES)
-def test_exact_sums(gpu, m, k, n, dt):
-    announce(f"grouped {m} {k} {n} {dt}")
+def test_exact_sums(gpu, m, k, n, dt, variant):
+    announce(f"grouped {m} {k} {n} {dt} {variant}")
     x = _ints(m, k, dt, m + k)
     xs = _c(x, m)
     for group, zeros in ((32, True), (64, True), (96, False), (128, True), (192, True), (256, False), (32768, True)):
         layer = _layer(n, k, group, n + group, zeros, sdt=XTYPES[(group // 32) % 3])
-        y = _run(gpu, x, layer, group, xs, out_dtype=torch.float32)
+        y = _run(gpu, x, layer, group, xs, out_dtype=torch.float32, variant=variant)
         assert torch.equal(y.cpu().double(), _ref(x, layer, group, xs)), (group, zeros)
 
 
+@BOTH
 @pytest.mark.parametrize("dt", XTYPES)
 @pytest.mark.parametrize("m,k,n,group", [(1, 4096, 64, 128), (5, 64, 40, 32), (40, 1000, 70, 64), (100, 2048, 130, 128),
                                          (513, 640, 200, 128), (2, 96, 5, 96)])
-def test_real_values(gpu, m, k, n, group, dt):
-    announce(f"grouped real {m} {k} {n} {dt}")
+def test_real_values(gpu, m, k, n, group, dt, variant):
+    announce(f"grouped real {m} {k} {n} {dt} {variant}")
     g = _gen(m + k)
     x = torch.randn(m, k, generator=g) * torch.exp(torch.randn(k, generator=g) * 0.6)
     x = x.to(dt) if dt != torch.float8_e4m3fn else (x * 20).clamp(-448, 448).to(dt)
@@ -87,7 +92,7 @@ def test_real_values(gpu, m, k, n, group, dt):
     for zeros, act, sdt in ((True, None, torch.float16), (False, "relu", torch.float32), (True, "gelu", torch.bfloat16)):
         layer = _layer(n, k, group, 3, zeros, exact=False, sdt=sdt)
         r = res.bfloat16() if act == "relu" else None
-        y = _run(gpu, x, layer, group, xs, bias=bias, residual=r, activation=act)
+        y = _run(gpu, x, layer, group, xs, bias=bias, residual=r, activation=act, variant=variant)
         assert y.dtype == (torch.bfloat16 if dt == torch.float8_e4m3fn else dt)
         ref = _ref(x, layer, group, xs) + bias.double() + (0 if r is None else r.double())
         plus = (layer[0], layer[1], torch.zeros_like(layer[1], dtype=torch.uint8))
@@ -106,7 +111,8 @@ def test_real_values(gpu, m, k, n, group, dt):
         assert over <= 1, f"{over} times the tolerance"
 
 
-def test_fp32_inputs_are_not_rounded(gpu):
+@BOTH
+def test_fp32_inputs_are_not_rounded(gpu, variant):
     """24-bit numbers: the third of their parts counts.  One element a row, so the sum is one product."""
     announce("grouped fp32 bits")
     for m in (2, 80):
@@ -116,13 +122,14 @@ def test_fp32_inputs_are_not_rounded(gpu):
         x[torch.arange(m), at] = torch.where(torch.arange(m) % 2 == 0, v, -v)
         q = torch.ones(20, 256, dtype=torch.uint8)
         layer = (_pack(q), torch.ones(20, 2), torch.zeros(20, 2, dtype=torch.uint8))
-        y = _run(gpu, x, layer, 128).cpu()
+        y = _run(gpu, x, layer, 128, variant=variant).cpu()
         assert torch.equal(y, x.sum(1, keepdim=True).expand(m, 20))
 
 
+@BOTH
 @pytest.mark.parametrize("m", [4, 100])
 @pytest.mark.parametrize("dt", XTYPES)
-def test_rows_that_are_not_finite_stay_alone(gpu, dt, m):
+def test_rows_that_are_not_finite_stay_alone(gpu, dt, m, variant):
     announce(f"grouped not finite {dt} {m}")
     k = 300
     x = _ints(m, k, torch.float32, 1)
@@ -134,15 +141,16 @@ def test_rows_that_are_not_finite_stay_alone(gpu, dt, m):
     if xs is not None:
         xs[2] = torch.nan
     layer = _layer(50, k, 64, 2)
-    y = _run(gpu, x, layer, 64, xs, out_dtype=torch.float32).cpu()
+    y = _run(gpu, x, layer, 64, xs, out_dtype=torch.float32, variant=variant).cpu()
     assert not torch.isfinite(y[1:3]).any()
     keep = [i for i in range(m) if i not in (1, 2)]
     assert torch.equal(y[keep].double(), _ref(x[keep], layer, 64, None if xs is None else xs[keep]))
 
 
+@BOTH
 @pytest.mark.parametrize("dt", XTYPES)
 @pytest.mark.parametrize("rows", [6, 150])
-def test_strides_and_places(gpu, dt, rows):
+def test_strides_and_places(gpu, dt, rows, variant):
     """Rows of a larger tensor, odd starts, transposed and 3-D inputs; codes that do not start at 16 bytes."""
     from dimq_amd import ops
     announce(f"grouped strides {dt} {rows}")
@@ -156,19 +164,37 @@ def test_strides_and_places(gpu, dt, rows):
               big[4, 10:266], big[3:3, :256]):
         lead = x.shape[:-1]
         xs = torch.full(lead, 0.5, device=gpu) if dt == torch.float8_e4m3fn else None
-        y = ops.dimq_linear_grouped(x, odd[5:].view(40, 128), s, z, 64, x_scales=xs, out_dtype=torch.float32)
+        y = ops.dimq_linear_grouped(x, odd[5:].view(40, 128), s, z, 64, x_scales=xs, out_dtype=torch.float32, variant=variant)
         assert y.shape == (*lead, 40) and y.is_contiguous()
         assert torch.equal(y.cpu().double(), _ref(x.cpu(), (codes, s, z), 64, None if xs is None else xs.cpu()))
 
 
-def test_more_columns_than_tiles_and_split_sums(gpu):
-    """Few tiles with a long reduction (cut along k), and tiles beyond a multiple of the XCDs."""
-    announce("grouped splits")
-    for m, k, n in ((65, 16384, 64), (129, 8192, 300), (260, 256, 1300), (1000, 128, 1000)):
+@BOTH
+def test_more_columns_than_tiles_and_split_sums(gpu, variant):
+    """Few tiles with a long reduction (cut along k), tiles beyond a multiple of the XCDs, and every number of row and column
+    blocks that the single launch gives a work-group."""
+    announce(f"grouped splits {variant}")
+    for m, k, n in ((65, 16384, 64), (129, 8192, 300), (260, 256, 1300), (1000, 128, 1000), (3, 128, 2100), (20, 128, 2050),
+                    (40, 256, 2049), (20, 128, 10300), (16, 128, 10245), (50, 128, 10250)):
         x = _ints(m, k, torch.bfloat16, 1)
         layer = _layer(n, k, 128, 2)
-        y = _run(gpu, x, layer, 128, out_dtype=torch.float32)
+        y = _run(gpu, x, layer, 128, out_dtype=torch.float32, variant=variant)
         assert torch.equal(y.cpu().double(), _ref(x, layer, 128))
+    for dt in (torch.float32, torch.float8_e4m3fn):
+        for m, group in ((5, 32), (20, 32), (40, 32), (20, 64), (40, 64), (40, 128)):
+            x = _ints(m, 128, dt, 1)
+            layer = _layer(2050, 128, group, 2)
+            y = _run(gpu, x, layer, group, _c(x, m), out_dtype=torch.float32, variant=variant)
+            assert torch.equal(y.cpu().double(), _ref(x, layer, group, _c(x, m)))
+
+
+def test_large_products_choose_tiles(gpu):
+    announce("grouped large")
+    x, layer = _ints(700, 1024, torch.bfloat16, 1), _layer(4096, 1024, 128, 2)
+    y = _run(gpu, x, layer, 128, out_dtype=torch.float32)
+    assert torch.equal(y, _run(gpu, x, layer, 128, out_dtype=torch.float32, variant="mfma"))
+    rows = torch.randint(0, 700, (20,), generator=_gen(5))
+    assert torch.equal(y.cpu()[rows].double(), _ref(x[rows], layer, 128))
 
 
 def test_layer_of_a_linear(gpu):
@@ -226,11 +252,12 @@ def test_norm_rows_feed_the_layer(gpu):
 def test_streams_and_graphs(gpu):
     announce("grouped graph")
     from dimq_amd import ops
-    for m, dt in ((3, torch.bfloat16), (100, torch.bfloat16), (70, torch.float32), (200, torch.float8_e4m3fn)):
+    for m, dt, variant in ((3, torch.bfloat16, "small_m"), (100, torch.bfloat16, "mfma"), (70, torch.float32, "mfma"),
+                           (200, torch.float8_e4m3fn, "mfma")):
         x = _ints(m, 1000, dt, 1).to(gpu)
         xs = torch.ones(m, device=gpu) if dt == torch.float8_e4m3fn else None
         codes, s, z = (t.to(gpu) for t in _layer(96, 1000, 128, 2))
-        call = lambda: ops.dimq_linear_grouped(x, codes, s, z, 128, x_scales=xs, out_dtype=torch.float32)  # noqa: E731
+        call = lambda: ops.dimq_linear_grouped(x, codes, s, z, 128, x_scales=xs, out_dtype=torch.float32, variant=variant)  # noqa: E731,B023
         want = call()
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
