@@ -1,8 +1,13 @@
 // Rows of logits x: log probabilities of given tokens, entropy and the largest alternatives, the distillation loss of a
 // teacher's top logits, and the gradients of both.
 //
-//   m = max x, s = sum exp(x - m), u = sum exp(x - m) (x - m)            one pass, kept as a running (m, s, u)
-//   lse = m + log s,  log p = x - lse,  entropy = -sum p log p = log s - u / s
+//   m = max x,  s = sum 2^(k x - i),  u = sum 2^(k x - i) (k x - i)      one pass, kept as a running (m, s, u)
+//   k = log2 e (over the temperature),  i = k m rounded to an integer
+//   log p = (x - m) / t - l,  l = log s - (k m - i) log 2,  entropy = -sum p log p = log s - (u / s) log 2
+//
+// so that an element costs an fma, an exponential and an addition, nothing but the fma rounds an exponent, and a larger
+// maximum scales s by a power of two.  From |k m| = 2^20 on, where k m's own rounding would count (a row of masks at the type's
+// lowest number), the exponent is k (x - m) instead.
 //
 // A row that holds a NaN or +infinity, or nothing above -infinity, has no distribution: its values are NaN and its
 // alternatives' tokens -1.  -infinity in a row has p = 0 and adds nothing; the type's lowest finite number is a number.
@@ -13,6 +18,10 @@
 //
 // Bound by bytes: a row is read once (the gradients read it once more and write theirs).  A row is cut over several
 // work-groups where there are few of them; a second launch then joins their (m, s, u) and candidates.
+//
+// Measured (large reads reach 6.0 to 6.8 TB/s, copies 5.07): distillation of 2048 x 128000 bf16 103 us forward (5.1 TB/s) and
+// 209 backward (5.0 TB/s); scores of 4096 x 32768 fp16 with 32 alternatives 74 us (3.6 TB/s; 45 of them are the pass), of one
+// row of 128000 12 us, where the two launches' latencies count.
 #include "common.h"
 #include "rows.h"
 
@@ -54,20 +63,40 @@ struct LogitArgs {
   uint64_t* cand;  // [rows][splits][top]
 };
 
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// 2^d, d no larger than 1.
+__device__ __forceinline__ float exp2_of(float d) { return __builtin_amdgcn_exp2f(d); }
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// Where the exponents of a running maximum m are counted from.
+struct Origin {
+  float m, i;
+  bool far;
+  __device__ __forceinline__ Origin(float max, float k) : m(max) {
+    const float x = max * k;
+    far = !(fabsf(x) < 0x1p20f);
+    i = far ? 0.0f : __builtin_rintf(x);
+  }
+  __device__ __forceinline__ float exponent(float x, float k) const { return far ? (x - m) * k : fmaf(x, k, -i); }
+  // from this origin to another
+  __device__ __forceinline__ float to(const Origin& o, float k) const {
+    return far ? (o.far ? (m - o.m) * k : fmaf(m, k, -o.i)) : (o.far ? fmaf(-o.m, k, i) : i - o.i);
+  }
+};
+
 struct Stats {
   float m, s, u;
 };
 
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
-
-// (m, s, u) with the maximum raised to m: s and u are sums of exp(x - m) and exp(x - m) (x - m).  The difference is held
-// above -200, whose exponential is 0, so that no 0 * infinity arises.
+// (m, s, u) from its own maximum's origin to a larger one's.  Exponents are held above -300, whose power is 0, so that no
+// 0 * infinity arises.
 template <bool U>
-__device__ __forceinline__ void raise(Stats& a, float m, float scale) {
-  const float d = fmaxf(a.m - m, -200.0f / scale), e = exp_of(d * scale);
+__device__ __forceinline__ void raise(Stats& a, const Origin& from, const Origin& o, float k) {
+  const float d = fmaxf(from.to(o, k), -300.0f), e = exp2_of(d);
   if constexpr (U) a.u = e * fmaf(a.s, d, a.u);
   a.s *= e;
-  a.m = m;
+  a.m = o.m;
 }
 
 // Two sums over the work-group behind one barrier.
@@ -82,9 +111,9 @@ __device__ __forceinline__ void block_add2(float& a, float& b, float (*red)[4]) 
 
 // Every thread's to the common maximum, then plain sums.
 template <bool U>
-__device__ __forceinline__ Stats block_stats(Stats a, float scale, float (*red)[4]) {
+__device__ __forceinline__ Stats block_stats(Stats a, float k, float (*red)[4]) {
   const float m = row_reduce<kLgThreads, true>(a.m, red[0]);
-  raise<U>(a, m, scale);
+  raise<U>(a, Origin(a.m, k), Origin(m, k), k);
   block_add2(a.s, a.u, red + 1);
   return a;
 }
@@ -149,25 +178,46 @@ struct Span {
   }
 };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {  // not of fmaxf: it would quiet each operand first
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Adds N elements; NaN and +infinity make s NaN.
 template <int N, bool U>
-__device__ __forceinline__ void add_to(Stats& st, const float (&v)[N], float scale) {
-  float cm = v[0];
+__device__ __forceinline__ void add_to(Stats& st, Origin& o, const float (&v)[N], float k) {
+  float cm;
+  if constexpr (N == 8) cm = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[7]));
+  else if constexpr (N == 4) cm = max3(max3(v[0], v[1], v[2]), v[3], v[3]);
+  else cm = v[0];
+  if (cm > st.m) {
+    const Origin n(cm, k);
+    raise<U>(st, o, n, k);
+    o = n;
+  }
+  float d[N];
+  if (__builtin_expect(o.far, 0)) {
 #pragma unroll
-  for (int j = 1; j < N; ++j) cm = fmaxf(cm, v[j]);
-  if (cm > st.m) raise<U>(st, cm, scale);
+    for (int j = 0; j < N; ++j) d[j] = (v[j] - o.m) * k;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) d[j] = fmaf(v[j], k, -o.i);
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const float d = v[j] - st.m, e = exp_of(d * scale);
+    const float e = exp2_of(d[j]);
     st.s += e;
-    if constexpr (U) st.u = fmaf(e, fmaxf(d, -200.0f), st.u);
+    if constexpr (U) st.u = fmaf(e, fmaxf(d[j], -300.0f), st.u);
   }
 }
 
 // The calling thread's part of [a, b): pieces tid, tid + 256, ..., and one of the single elements.
 template <int XT, bool U>
-__device__ __forceinline__ Stats stream_stats(const void* row, const Span& sp, float scale) {
+__device__ __forceinline__ Stats stream_stats(const void* row, const Span& sp, float k) {
   constexpr int P = pack_of<XT>();
   Stats st{kLowest, 0.0f, 0.0f};
+  Origin o(kLowest, k);
   const uint4* body = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + sp.body * (16 / P));
   int64_t i = threadIdx.x;
   for (; i + 3 * kLgThreads < sp.pieces; i += 4 * kLgThreads) {
@@ -178,17 +228,17 @@ __device__ __forceinline__ Stats stream_stats(const void* row, const Span& sp, f
     for (int q = 0; q < 4; ++q) {
       float v[P];
       unpack16<XT>(t[q], v);
-      add_to<P, U>(st, v, scale);
+      add_to<P, U>(st, o, v, k);
     }
   }
   for (; i < sp.pieces; i += kLgThreads) {
     float v[P];
     unpack16<XT>(body[i], v);
-    add_to<P, U>(st, v, scale);
+    add_to<P, U>(st, o, v, k);
   }
   if (static_cast<int>(threadIdx.x) < sp.singles(P)) {
     const float v[1] = {logit<XT>(row, sp.single(threadIdx.x, P))};
-    add_to<1, U>(st, v, scale);
+    add_to<1, U>(st, o, v, k);
   }
   return st;
 }
@@ -219,12 +269,27 @@ struct TopShared {
 };
 
 // A lower bound of the top-th largest logit's order, from the largest order each thread knows of (0: none): the top-th
-// largest of these, found by counting.  Their last 8 bits give way to the thread's number, so that no two are alike and a
-// comparison is all it takes; the bound is only lower for it.
+// largest of these, found by counting.  Their last 8 bits give way to a number, so that no two are alike and a comparison is
+// all it takes; the bound is only lower for it.  Up to 48 alternatives the maxima of four threads each do: 64 of them, which
+// every wave counts by itself in a quarter of the time, for a third more candidates at the most.
+constexpr int kFewTop = 48;
+
 __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int top, TopShared& sh) {
+  if (threadIdx.x == 0) sh.count = 0, sh.nowners = 0;
+  if (top <= kFewTop) {
+    sh.maxima[threadIdx.x] = mine;
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t a = sh.maxima[lane], b = sh.maxima[lane + 64], c = sh.maxima[lane + 128], d = sh.maxima[lane + 192];
+    const uint32_t ab = a > b ? a : b, cd = c > d ? c : d, key = ((ab > cd ? ab : cd) & ~0xffu) | (63u - lane);
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) before += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), i)) > key;
+    const uint64_t at = __ballot(before == top - 1);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), __builtin_ctzll(at))) & ~0xffu;
+  }
   const uint32_t key = (mine & ~0xffu) | (255u - threadIdx.x);
   sh.maxima[threadIdx.x] = key;
-  if (threadIdx.x == 0) sh.count = 0, sh.nowners = 0;
   __syncthreads();
   int before = 0;
 #pragma unroll 16
@@ -235,6 +300,11 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int top, TopShared& 
   if (before == top - 1) sh.bound = mine & ~0xffu;
   __syncthreads();
   return sh.bound;
+}
+
+// The bound as a number to compare with: every logit but a NaN of that order or a higher one is no smaller.
+__device__ __forceinline__ float bound_value(uint32_t bound) {
+  return bound <= 0x007fffffu ? __uint_as_float(0xff800000u) : of_order(bound);
 }
 
 __device__ __forceinline__ void push(TopShared& sh, uint64_t key) {
@@ -266,16 +336,19 @@ __device__ __forceinline__ void span_top(const void* row, const Span& sp, uint32
   const int no = sh.nowners;
   const int items = no * static_cast<int>((sp.pieces + kLgThreads - 1) / kLgThreads);  // at most 2^29 + 2^8
   const uint4* body = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + sp.body * (16 / P));
+  const float least = bound_value(bound), per_owner = 1.0f / static_cast<float>(no);
   auto test = [&](float v, int64_t at) {
-    if (order_of(v) >= bound) push(sh, key_of(v, at));
+    if (!(v < least)) push(sh, key_of(v, at));  // with a NaN the row's alternatives are not used
   };
   for (int base = threadIdx.x; base < items; base += 4 * kLgThreads) {
     uint4 t[4];
     int64_t at[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
+      // turn and owner of an item; up to 2^22 items the product is off by less than the half that keeps it from the next
       const int item = base + q * kLgThreads;
-      const int64_t i = item < items ? sh.owners[item % no] + item / no * static_cast<int64_t>(kLgThreads) : sp.pieces;
+      const int turn = items < 1 << 22 ? static_cast<int>((static_cast<float>(item) + 0.5f) * per_owner) : item / no;
+      const int64_t i = item < items ? sh.owners[item - turn * no] + turn * static_cast<int64_t>(kLgThreads) : sp.pieces;
       at[q] = i < sp.pieces ? i : -1;
       t[q] = body[at[q] < 0 ? 0 : at[q]];  // there is a piece: items > 0
     }
@@ -343,18 +416,25 @@ struct TokenLogit {
   }
 };
 
+// log sum exp((x - m) / t) of complete statistics.
+__device__ __forceinline__ float log_sum(const Stats& st, float k) {
+  const Origin o(st.m, k);
+  return logf(st.s) - o.exponent(st.m, k) * kLn2;
+}
+
 __device__ __forceinline__ void finish_score(const LogitArgs& a, int64_t row, const TokenLogit& t, const Stats& st) {
   if (threadIdx.x != 0) return;
   const bool ok = proper(st);
-  const float ls = ok ? logf(st.s) : nan32();
+  const float ls = ok ? log_sum(st, kLog2e) : nan32();
   a.logp[row] = t.token < 0 ? 0.0f : ok && t.token < a.V ? (t.x - st.m) - ls : nan32();
-  a.entropy[row] = ok ? ls - st.u / st.s : nan32();
+  a.entropy[row] = ok ? logf(st.s) - st.u / st.s * kLn2 : nan32();
   if (a.norm) a.norm[2 * row] = st.m, a.norm[2 * row + 1] = ls;
 }
 
-__device__ __forceinline__ void put_top(const LogitArgs& a, int64_t row, int r, uint64_t key, const Stats& st, bool ok) {
+// ls: log_sum of the row
+__device__ __forceinline__ void put_top(const LogitArgs& a, int64_t row, int r, uint64_t key, float m, float ls, bool ok) {
   const float v = of_order(static_cast<uint32_t>(key >> 32));
-  a.top_logp[row * a.top + r] = ok ? (v - st.m) - logf(st.s) : nan32();
+  a.top_logp[row * a.top + r] = ok ? (v - m) - ls : nan32();
   a.top_ids[row * a.top + r] = ok ? static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key)) : -1;
 }
 
@@ -382,7 +462,7 @@ struct Entry {
 template <int XT>
 __device__ __forceinline__ void finish_distill(const LogitArgs& a, int64_t row, const void* xr, const Entry& first,
                                                const Stats& st, float (*red)[4]) {
-  const float ls = logf(st.s), tau = 1.0f / a.tau_inv;
+  const float ls = log_sum(st, a.tau_inv * kLog2e), tau = 1.0f / a.tau_inv;
   const float none = __uint_as_float(0xff800000u);
   float m = none;
   auto each = [&](auto f) {
@@ -424,15 +504,15 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const LogitArgs a) {
     const char* xr = static_cast<const char*>(a.x) + row * a.ldx * (XT == DIMQ_F32 ? 4 : 2);
     const int64_t from = blockIdx.x * a.chunk, to = from + a.chunk < a.V ? from + a.chunk : a.V;
     const Span sp = Span::of<XT>(xr, from, to);
-    const float scale = DISTILL ? a.tau_inv : 1.0f;
+    const float k = DISTILL ? a.tau_inv * kLog2e : kLog2e;
     TokenLogit token;
     Entry entry;
     if (a.splits == 1) {
       if constexpr (DISTILL) entry = Entry::of<XT>(a, row, xr, threadIdx.x);
       else token = TokenLogit::of<XT>(a, row, xr);
     }
-    const Stats mine = stream_stats<XT, !DISTILL>(xr, sp, scale);
-    const Stats st = block_stats<!DISTILL>(mine, scale, red);
+    const Stats mine = stream_stats<XT, !DISTILL>(xr, sp, k);
+    const Stats st = block_stats<!DISTILL>(mine, k, red);
     if (a.splits > 1) {
       if (threadIdx.x == 0) {
         float* to_stats = a.stats + (row * a.splits + blockIdx.x) * 4;
@@ -453,9 +533,10 @@ __global__ __launch_bounds__(kLgThreads) void logits_kernel(const LogitArgs a) {
         if (a.splits > 1) {
           span_top<XT>(xr, sp, m, a.top, sh, [&](int r, uint64_t key) { cand[r] = key; });
         } else if (ok) {
-          span_top<XT>(xr, sp, m, a.top, sh, [&](int r, uint64_t key) { put_top(a, row, r, key, st, true); });
+          const float ls = log_sum(st, k);
+          span_top<XT>(xr, sp, m, a.top, sh, [&](int r, uint64_t key) { put_top(a, row, r, key, st.m, ls, true); });
         } else {
-          for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, st, false);
+          for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, 0.0f, 0.0f, false);
         }
       }
     }
@@ -478,7 +559,7 @@ __global__ __launch_bounds__(kLgThreads) void logits_join_kernel(const LogitArgs
   }
   if constexpr (DISTILL) {
     const Entry entry = Entry::of<XT>(a, row, xr, threadIdx.x);
-    st = block_stats<false>(st, a.tau_inv, red);
+    st = block_stats<false>(st, a.tau_inv * kLog2e, red);
     finish_distill<XT>(a, row, xr, entry, st, red + 3);
   } else {
     const TokenLogit token = TokenLogit::of<XT>(a, row, xr);
@@ -489,11 +570,11 @@ __global__ __launch_bounds__(kLgThreads) void logits_join_kernel(const LogitArgs
       keys[i] = key;
       mine = key > mine ? key : mine;
     }
-    st = block_stats<true>(st, 1.0f, red);
+    st = block_stats<true>(st, kLog2e, red);
     finish_score(a, row, token, st);
     if (a.top == 0) return;
     if (!proper(st)) {
-      for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, st, false);
+      for (int r = threadIdx.x; r < a.top; r += kLgThreads) put_top(a, row, r, 0, 0.0f, 0.0f, false);
       return;
     }
     // as in span_top, over the splits' keys: there are at least `top` of them that are not 0
@@ -503,7 +584,8 @@ __global__ __launch_bounds__(kLgThreads) void logits_join_kernel(const LogitArgs
       if (key != 0 && static_cast<uint32_t>(key >> 32) >= bound) push(sh, key);
     }
     __syncthreads();
-    auto put = [&](int r, uint64_t key) { put_top(a, row, r, key, st, true); };
+    const float ls = log_sum(st, kLog2e);
+    auto put = [&](int r, uint64_t key) { put_top(a, row, r, key, st.m, ls, true); };
     if (sh.count <= kLgCand) rank_keys(sh.cand, sh.count, a.top, put);
     else rank_keys(keys, n, a.top, put);  // zeros rank behind all others
   }
@@ -552,9 +634,12 @@ struct GradArgs {
 //   scoring        a ([v = token] - p) - b p (log p + H)
 //   distillation   tau c (q - p_teacher), the teacher's entries subtracted after the chunk is written
 template <int XT, bool DISTILL>
-__global__ __launch_bounds__(kLgThreads) void logits_grad_kernel(const GradArgs a) {
+__global__ __launch_bounds__(kLgThreads, 8) void logits_grad_kernel(const GradArgs a) {
   constexpr int P = pack_of<XT>(), kSize = XT == DIMQ_F32 ? 4 : 2;
-  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+  for (int64_t turn = blockIdx.y; turn < a.rows; turn += gridDim.y) {
+    // The forward pass's last rows first, which may still be in the cache, and gradients stored past it: forward and backward
+    // of 2048 x 128000 bf16 take 313 us, in the rows' order 338, with cached stores as well 364.
+    const int64_t row = a.rows - 1 - turn;
     const char* xr = static_cast<const char*>(a.x) + row * a.ldx * kSize;
     char* gr = static_cast<char*>(a.gx) + row * a.V * kSize;
     const int64_t from = blockIdx.x * a.chunk, to = from + a.chunk < a.V ? from + a.chunk : a.V;
@@ -604,7 +689,8 @@ __global__ __launch_bounds__(kLgThreads) void logits_grad_kernel(const GradArgs 
           if constexpr (XT == DIMQ_F32) o[j] = __float_as_uint(v[j]);
           else o[j] = XT == DIMQ_F16 ? f16x2_rne(v[2 * j], v[2 * j + 1]) : bf16x2_rne(v[2 * j], v[2 * j + 1]);
         }
-        out[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(u4{o[0], o[1], o[2], o[3]}, reinterpret_cast<u4*>(out) + i);
       };
       int64_t i = threadIdx.x;
       for (; i + 3 * kLgThreads < sp.pieces; i += 4 * kLgThreads) {
