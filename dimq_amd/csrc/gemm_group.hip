@@ -899,6 +899,7 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
   DIMQ_CHECK(x && codes && scales && y, "linear_grouped: null pointer");
   DIMQ_CHECK(aligned(codes, 16), "linear_grouped: codes must be 16-byte aligned");
   DIMQ_CHECK(aligned(x, x_dtype == DIMQ_E4M3 ? 1 : dtype_size(x_dtype)), "linear_grouped: misaligned input");
+  if (group >= K) group = (K + 127) / 128 * 128;  // one group a row, however large: the longest spans
   GroupArgs p{};
   p.x = x, p.M = M, p.K = K, p.ldx = ldx, p.xs = x_scales, p.vec = rows_aligned(x, x_dtype, M, ldx);
   p.nb = (K + 31) / 32, p.codes = codes, p.pitch = p.nb * 16, p.scales = scales, p.s_dt = scales_dtype, p.zeros = zeros;
@@ -925,7 +926,7 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
     const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
     DIMQ_CHECK(workspace_bytes >= t.bytes() && aligned(workspace, 16),
                "linear_grouped: the workspace is too small or not 16-byte aligned");
-    DIMQ_CHECK(t.tm * t.tn < (int64_t)1 << 24, "linear_grouped: too many outputs for one launch");
+    DIMQ_CHECK(t.tm * t.tn < (int64_t)1 << 23, "linear_grouped: too many outputs for one launch");
     DIMQ_CHECK(t.ksteps * kTileK < kMostApart, "linear_grouped: rows of 2^23 elements or more take fewer rows");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     DIMQ_GROUP_XT(launch_tile, p, t, ws, s)

@@ -229,9 +229,9 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     // what the backward pass reads in one allocation: the divisor, norm [rows, 2], p [rows, k]; the rows' losses and the
     // workspace (16-byte aligned) in another
     const Tensor kept = at::empty({4 + x.n * (2 + k)}, f);
+    const On on(student);
     const int64_t bytes = dimq_logits_workspace_bytes(x.n, x.cols, 0);
     const Tensor ws = at::empty({bytes / 4 + (none ? 0 : x.n)}, f);
-    const On on(student);
     check_rc(dimq_distill_loss(ptr(x.t), dt(x.t), x.n, x.cols, x.ld, ptr(v), dt(v), ptr(id), id.scalar_type() == at::kLong, k,
                                temperature, static_cast<int>(reduction), none ? f32(loss) : f32(ws) + bytes / 4, f32(loss), f32(kept),
                                f32(kept) + 4, f32(kept) + 4 + 2 * x.n, ptr(ws), bytes, on.stream));

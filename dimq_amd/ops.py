@@ -38,6 +38,15 @@ def require_extension() -> None:
         )
 
 
+@lru_cache(maxsize=1)
+def _native():
+    """The compiled half of the operators that are called past the dispatcher."""
+    require_extension()
+    from ._C import _native as compiled
+
+    return compiled
+
+
 def pack_u4(indices: torch.Tensor) -> torch.Tensor:
     require_extension()
     return torch.ops.dimq.pack_u4(indices)
@@ -362,11 +371,8 @@ def dimq_linear_grouped(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     are not finite; the output in ``out_dtype`` (x's by default, bf16 for
     float8).  ``variant``: "small_m" one launch, "mfma" tiles (a workspace and up to three launches), "auto" by size.  For
     serving: a backward pass through it raises."""
-    require_extension()
-    from ._C import _native
-
-    return _native.linear_grouped(x, codes, scales, zeros, int(group_size), bias, x_scales, residual,
-                                  ACTIVATIONS[activation], out_dtype, VARIANTS[variant])
+    return _native().linear_grouped(x, codes, scales, zeros, int(group_size), bias, x_scales, residual,
+                                    ACTIVATIONS[activation], out_dtype, VARIANTS[variant])
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *,
@@ -374,10 +380,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
     """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, h = x; with a residual (x's shape and dtype)
     ``(y, h)``, h = x + residual rounded to their dtype.  x in fp32, fp16 or bf16, y in ``out_dtype`` (x's by default).
     Gradients reach x, the residual and the weight; they have none of their own."""
-    require_extension()
-    from ._C import _native
-
-    y, h = _native.rms_norm(x, weight, float(eps), residual, out_dtype)
+    y, h = _native().rms_norm(x, weight, float(eps), residual, out_dtype)
     return y if residual is None else (y, h)
 
 
@@ -387,10 +390,7 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor | None = None, eps: floa
     residual ``(codes, scales, h)``.  codes: torch.float8_e4m3fn of y / scale, to nearest even; scales: fp32, max|y| / 448
     of each row (at least 2^-126; 0 for a row of zeros).  A row with a y that is not finite has the scale NaN.  For serving:
     it has no gradients."""
-    require_extension()
-    from ._C import _native
-
-    codes, scales, h = _native.rms_norm_e4m3(x, weight, float(eps), residual)
+    codes, scales, h = _native().rms_norm_e4m3(x, weight, float(eps), residual)
     return (codes, scales) if residual is None else (codes, scales, h)
 
 
@@ -401,10 +401,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     token first among equals.  The values are fp32.  A row that holds a NaN or +infinity, or nothing above -infinity, has
     no distribution: its values are NaN, its alternatives' tokens -1.  Gradients reach the logits from the log
     probabilities and the entropy (zero where both of a row's are); they have none of their own."""
-    require_extension()
-    from ._C import _native
-
-    return _native.token_logprobs(logits, tokens, int(top))
+    return _native().token_logprobs(logits, tokens, int(top))
 
 
 def max_pool2d_nhwc(x: torch.Tensor, kernel_size, stride=None, padding=0) -> torch.Tensor:

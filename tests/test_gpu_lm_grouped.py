@@ -72,8 +72,9 @@ def test_exact_sums(gpu, m, k, n, dt, variant):
     announce(f"grouped {m} {k} {n} {dt} {variant}")
     x = _ints(m, k, dt, m + k)
     xs = _c(x, m)
-    for group, zeros in ((32, True), (64, True), (96, False), (128, True), (192, True), (256, False), (32768, True)):
-        layer = _layer(n, k, group, n + group, zeros, sdt=XTYPES[(group // 32) % 3])
+    for group, zeros in ((32, True), (64, True), (96, False), (128, True), (192, True), (256, False), (32768, True),
+                         (2 ** 40, False), (2 ** 39 + 32, True)):
+        layer = _layer(n, k, group, n + group % 1000, zeros, sdt=XTYPES[(group // 32) % 3])
         y = _run(gpu, x, layer, group, xs, out_dtype=torch.float32, variant=variant)
         assert torch.equal(y.cpu().double(), _ref(x, layer, group, xs)), (group, zeros)
 

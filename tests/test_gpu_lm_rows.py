@@ -203,6 +203,37 @@ def test_rms_norm_gradient_by_differences(gpu):
         assert abs(diff - g.cpu().double().view(-1)[i]) <= 1e-6 + 200 * E * (1 + abs(diff))
 
 
+def test_rms_norm_gradients_of_some_inputs(gpu):
+    """Any of the three absent or without a gradient of its own; the same tensor twice; accumulation into .grad."""
+    from dimq_amd import ops
+    announce("rms_norm some inputs")
+    leaf = lambda seed, on: _rows(4, 48, torch.float32, seed).to(gpu).requires_grad_(on)  # noqa: E731
+    gy, gh = _rows(4, 48, torch.float32, 8).to(gpu), _rows(4, 48, torch.float32, 9).to(gpu)
+    for has_w in (None, False, True):
+        for on_x, on_r in ((True, True), (True, False), (False, True), (False, False)):
+            w = None if has_w is None else (1 + 0.1 * torch.randn(48, generator=_gen(1))).to(gpu).requires_grad_(has_w)
+            x, r = leaf(2, on_x), leaf(3, on_r)
+            y, h = ops.rms_norm(x, w, 1e-5, residual=r)
+            if not (on_x or on_r or has_w):
+                assert not y.requires_grad
+                continue
+            torch.autograd.backward((y, h), (gy, gh)) if h.requires_grad else y.backward(gy)
+            ref, ref_w, terms = lm.rms_norm_grads(h, w, 1e-5, gy, gh)
+            for t, on in ((x, on_x), (r, on_r)):
+                assert (t.grad is not None) == on
+                if on:
+                    _close(t.grad, ref, 300 * E * terms + _half(ref, torch.float32))
+            if on_x and on_r:
+                assert x.grad.data_ptr() != r.grad.data_ptr()
+            if has_w:
+                _close(w.grad, ref_w, 400 * E * lm.rms_norm_grads(h.abs(), w, 1e-5, gy.abs(), None)[1] + 1e-30)
+    x = leaf(2, True)
+    y, h = ops.rms_norm(x, None, 1e-5, residual=x)
+    torch.autograd.backward((y, h), (gy, gh))
+    ref, _, terms = lm.rms_norm_grads(h, None, 1e-5, gy, gh)
+    _close(x.grad, 2 * ref, 700 * E * terms + _half(2 * ref, torch.float32))
+
+
 def test_rms_norm_no_rows(gpu):
     from dimq_amd import ops
     x, w = torch.zeros(0, 16, device=gpu, requires_grad=True), torch.ones(16, device=gpu, requires_grad=True)
