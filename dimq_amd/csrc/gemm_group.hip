@@ -769,7 +769,8 @@ int span_bytes(int64_t group) { return group % 128 == 0 ? 16 : group % 64 == 0 ?
 // 28 / 34, 256 x 4096 52 / 37, 64 x 12288 42 / 38.
 constexpr double kFewProducts = 2.5e9;
 bool few_rows(int64_t M, int64_t K, int64_t N, int variant) {
-  if (variant == DIMQ_VARIANT_MFMA || M > int64_t{65535} * 16) return false;  // row blocks of one launch
+  // row and column blocks of one launch
+  if (variant == DIMQ_VARIANT_MFMA || M > int64_t{65535} * 16 || N > (int64_t{1} << 23) * 16 - 16) return false;
   return variant == DIMQ_VARIANT_SMALL_M || static_cast<double>(M) * static_cast<double>(K) * static_cast<double>(N) < kFewProducts;
 }
 
@@ -797,6 +798,8 @@ TilePlan tile_plan(int xt, int64_t M, int64_t K, int64_t N, bool in_place) {
   t.part_bytes = t.splits > 1 ? t.splits * M * N * 4 : 0;
   return t;
 }
+
+int64_t span_blocks(const TilePlan& t, int lb) { return (t.ksteps * (kTileK / (8 * lb)) + 31) / 32; }
 
 bool rows_aligned(const void* x, int xt, int64_t M, int64_t ldx) {
   return aligned(x, 16) && (M <= 1 || ldx * x_size(xt) % 16 == 0);
@@ -842,7 +845,7 @@ void launch_tile(GroupArgs p, const TilePlan& t, uint8_t* ws, hipStream_t s) {
   p.ksteps = t.ksteps, p.tiles_m = t.tm, p.tiles_n = t.tn, p.splits = t.splits;
   uint8_t *sums = ws + t.copy_bytes, *szs = sums + t.sum_bytes;
   p.plane = t.copy_bytes / P;
-  p.span_blocks = (t.ksteps * (kTileK / (8 * LB)) + 31) / 32;
+  p.span_blocks = span_blocks(t, LB);
   p.prep_first = static_cast<uint32_t>((p.N * p.span_blocks * 4 + 255) / 256);
   const int64_t blocks = (p.M * p.span_blocks * (32 * LB) + 256 * kPrepEach - 1) / (256 * kPrepEach);
   hipLaunchKernelGGL((group_prep_kernel<XT, LB>), dim3(static_cast<unsigned>(p.prep_first + blocks)), dim3(256), 0, s, p,
@@ -898,6 +901,7 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
   if (M == 0) return DIMQ_OK;
   DIMQ_CHECK(x && codes && scales && y, "linear_grouped: null pointer");
   DIMQ_CHECK(aligned(codes, 16), "linear_grouped: codes must be 16-byte aligned");
+  DIMQ_CHECK(aligned(scales, dtype_size(scales_dtype)), "linear_grouped: misaligned scales");
   DIMQ_CHECK(aligned(x, x_dtype == DIMQ_E4M3 ? 1 : dtype_size(x_dtype)), "linear_grouped: misaligned input");
   if (group >= K) group = (K + 127) / 128 * 128;  // one group a row, however large: the longest spans
   GroupArgs p{};
@@ -926,7 +930,9 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
     const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
     DIMQ_CHECK(workspace_bytes >= t.bytes() && aligned(workspace, 16),
                "linear_grouped: the workspace is too small or not 16-byte aligned");
-    DIMQ_CHECK(t.tm * t.tn < (int64_t)1 << 23, "linear_grouped: too many outputs for one launch");
+    // a launch has less than 2^32 threads
+    const int64_t prepared = span_blocks(t, lb) * (N * 4 + M * 32 * lb / kPrepEach);
+    DIMQ_CHECK(t.tm * t.tn < (int64_t)1 << 23 && prepared < ((int64_t)1 << 32) - 4096, "linear_grouped: too many outputs for one launch");
     DIMQ_CHECK(t.ksteps * kTileK < kMostApart, "linear_grouped: rows of 2^23 elements or more take fewer rows");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     DIMQ_GROUP_XT(launch_tile, p, t, ws, s)

@@ -32,6 +32,7 @@ constexpr int kLgThreads = 256;
 constexpr int kLgCand = 1024;      // candidates a work-group holds: more fall back to one pass per alternative
 constexpr int kLgTop = 128;        // most alternatives
 constexpr int kLgSplits = 32;      // most work-groups to a row
+constexpr int64_t kMostEntries = 4096;  // of a teacher's row: the gradient looks for equal tokens by comparing all pairs
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.402823466e38f;
 
@@ -745,6 +746,7 @@ int check_logits(const char* what, const void* x, int dtype, int64_t rows, int64
   DIMQ_CHECK(V < (int64_t)1 << 31, "%s: rows of 2^31 logits or more are not supported", what);
   DIMQ_CHECK(rows <= 1 || ldx >= V, "%s: row stride is below the row length", what);
   DIMQ_CHECK(rows == 0 || x, "%s: null pointer", what);
+  DIMQ_CHECK(aligned(x, dtype_size(dtype)), "%s: misaligned logits", what);
   return DIMQ_OK;
 }
 
@@ -838,9 +840,11 @@ extern "C" int dimq_distill_loss(const void* student, int dtype, int64_t rows, i
   const int rc = check_logits("top_logits_distillation_loss", student, dtype, rows, vocab, ldx);
   if (rc != DIMQ_OK) return rc;
   DIMQ_CHECK(float_logits(values_dtype), "top_logits_distillation_loss: teacher values must be fp32, fp16 or bf16");
-  DIMQ_CHECK(k >= 0 && k < 1 << 20, "top_logits_distillation_loss: at most 2^20 teacher entries a row");
-  DIMQ_CHECK(temperature >= 1e-30 && temperature <= 1e30,
-             "top_logits_distillation_loss: the temperature must be in [1e-30, 1e30]");
+  DIMQ_CHECK(k >= 0 && k <= kMostEntries, "top_logits_distillation_loss: at most %d teacher entries a row",
+             static_cast<int>(kMostEntries));
+  // t^2 multiplies what fp32 leaves of a difference of logarithms
+  DIMQ_CHECK(temperature >= 1e-3 && temperature <= 1e3,
+             "top_logits_distillation_loss: the temperature must be in [0.001, 1000]");
   DIMQ_CHECK(reduction >= 0 && reduction <= 2, "top_logits_distillation_loss: unknown reduction");
   const hipStream_t s = as_stream(stream);
   if (rows > 0) {
@@ -871,8 +875,8 @@ extern "C" int dimq_distill_loss_backward(const void* student, int dtype, int64_
   const int rc = check_logits("top_logits_distillation_loss backward", student, dtype, rows, vocab, ldx);
   if (rc != DIMQ_OK) return rc;
   if (rows == 0) return DIMQ_OK;
-  DIMQ_CHECK(k >= 0 && k < 1 << 20 && (k == 0 || (ids && p)) && norm && grad && grad_student,
-             "top_logits_distillation_loss backward: null pointer");
+  DIMQ_CHECK(k >= 0 && k <= kMostEntries && (k == 0 || (ids && p)) && norm && grad && grad_student,
+             "top_logits_distillation_loss backward: null pointer or too many entries");
   GradArgs a{};
   a.x = student, a.ldx = ldx, a.rows = rows, a.V = vocab, a.norm = norm, a.gx = grad_student;
   a.ga = grad, a.sa = grad_stride, a.tau = static_cast<float>(temperature), a.tau_inv = static_cast<float>(1.0 / temperature);

@@ -421,11 +421,12 @@ int check_rms(const char* what, const void* x, int x_dtype, int64_t rows, int64_
               double eps) {
   DIMQ_CHECK(float_of_row(x_dtype), "%s: input must be fp32, fp16 or bf16", what);
   DIMQ_CHECK(rows >= 0 && dim > 0, "%s: dimensions must be positive", what);
-  DIMQ_CHECK(dim < (int64_t)1 << 31, "%s: rows of 2^31 elements or more are not supported", what);
+  DIMQ_CHECK(dim < (int64_t)1 << 30, "%s: rows of 2^30 elements or more are not supported", what);
   DIMQ_CHECK(rows <= 1 || ldx >= dim, "%s: row stride is below the row length", what);
   DIMQ_CHECK(!w || float_of_row(w_dtype), "%s: weight must be fp32, fp16 or bf16", what);
   DIMQ_CHECK(eps >= 0.0, "%s: eps must be non-negative", what);
   DIMQ_CHECK(rows == 0 || x, "%s: null pointer", what);
+  DIMQ_CHECK(aligned(x, dtype_size(x_dtype)), "%s: misaligned input", what);
   return DIMQ_OK;
 }
 

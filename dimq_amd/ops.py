@@ -343,6 +343,8 @@ def quantize_grouped(w: torch.Tensor, group_size: int = 128, *, symmetric: bool 
         raise RuntimeError("quantize_grouped expects a weight [out_features, in_features]")
     if group_size <= 0 or group_size % 32:
         raise RuntimeError("quantize_grouped: the group size must be a positive multiple of 32")
+    if scale_dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise RuntimeError("quantize_grouped: scales must be fp32, fp16 or bf16")
     w = w.detach().float()
     if not bool(torch.isfinite(w).all()):
         raise RuntimeError("quantize_grouped: the weight must be finite")

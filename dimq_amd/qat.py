@@ -86,8 +86,9 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 def top_logits_distillation_loss(student: Tensor, teacher_values: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
                                  reduction: str = "mean") -> Tensor:
     """``t^2 sum_j p_j (log p_j - log q[id_j])`` of each row of student logits ``[..., vocab]`` (fp32, fp16 or bf16), with
-    ``p = softmax(values / t)`` over the teacher's entries ``[..., k]`` (its logits or log probabilities, and int64 or int32
-    tokens, as ``ops.token_logprobs`` returns them) and ``q = softmax(student / t)``.  Entries with a negative token or a
+    ``p = softmax(values / t)`` over the teacher's entries ``[..., k]``, k up to 4096 (its logits or log probabilities, and
+    int64 or int32 tokens, as ``ops.token_logprobs`` returns them) and ``q = softmax(student / t)``, t in [0.001, 1000].
+    Probabilities of a token that is named more than once add up in the gradient.  Entries with a negative token or a
     value of -infinity are left out; a row without entries has loss 0 and no gradient, whatever its logits.
     ``reduction`` "mean" (over the rows with entries; 0 without any), "sum" or "none"; the loss is fp32.  A token beyond the
     vocabulary, or logits without a distribution, give NaN.  The gradient reaches the student alone and has none of its own."""

@@ -667,8 +667,9 @@ int dimq_token_logprobs_backward(const void* logits, int dtype, int64_t rows, in
                                  const float* grad_logprobs, int64_t stride_logprobs, const float* grad_entropy,
                                  int64_t stride_entropy, void* grad_logits, void* stream);
 
-/* Distillation from a teacher's k top logits a row (values, ids [rows, k]; an
- * entry with a negative id or a value of -infinity is left out):
+/* Distillation from a teacher's k top logits a row (values, ids [rows, k], k up
+ * to 4096; an entry with a negative id or a value of -infinity is left out; t in
+ * [0.001, 1000]):
  *   row_loss = t^2 sum_j p_j (log p_j - log q[id_j]),
  *   p = softmax(values / t) over the kept entries, q = softmax(student / t),
  * 0 for a row without entries.  reduction 0: row_loss alone; 1 the mean over the

@@ -234,6 +234,23 @@ def test_rms_norm_gradients_of_some_inputs(gpu):
     _close(x.grad, 2 * ref, 700 * E * terms + _half(2 * ref, torch.float32))
 
 
+def test_rms_norm_of_a_row_added_to_itself(gpu):
+    """The residual may be the input itself: its gradient is both's."""
+    from dimq_amd import ops
+    announce("norm of x + x")
+    x = torch.randn(9, 520, generator=_gen(5)).to(gpu).requires_grad_()
+    two = x.detach().clone().requires_grad_()
+    gy, gh = (torch.randn(9, 520, generator=_gen(s)).to(gpu) for s in (6, 7))
+    got, = torch.autograd.grad(ops.rms_norm(x, residual=x), x, (gy, gh))
+    ref, = torch.autograd.grad(ops.rms_norm(two, residual=x.detach()), two, (gy, gh))
+    assert torch.equal(got, 2 * ref)
+    # the sum alone, and the norm alone
+    got, = torch.autograd.grad(ops.rms_norm(x, residual=x)[1], x, gh)
+    assert torch.equal(got, 2 * gh)
+    a, b = torch.autograd.grad(ops.rms_norm(x, residual=two)[1], (x, two), gh)
+    assert torch.equal(a, gh) and torch.equal(b, gh)
+
+
 def test_rms_norm_no_rows(gpu):
     from dimq_amd import ops
     x, w = torch.zeros(0, 16, device=gpu, requires_grad=True), torch.ones(16, device=gpu, requires_grad=True)
@@ -492,6 +509,20 @@ def test_distillation(gpu, rows, vocab, k, tau, reduction, dt):
         g = torch.randn(rows, generator=_gen(8)).to(gpu) if reduction == "none" else torch.tensor(1.7, device=gpu)
         gx, = torch.autograd.grad(loss, x, g)
         _check_distill(x, v, i, tau, reduction, loss, gx, g if reduction == "none" else 1.7)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 5000), (1, 40000)])
+def test_distillation_of_most_entries(gpu, rows, vocab):
+    """As many teacher entries as there may be, tokens among them more than once."""
+    from dimq_amd import qat
+    announce(f"distillation of 4096 entries, {rows} {vocab}")
+    x = _logits(rows, vocab, torch.float32, 19).to(gpu).requires_grad_()
+    values = torch.randn(rows, 4096, generator=_gen(3)).to(gpu)
+    ids = torch.randint(0, vocab, (rows, 4096), generator=_gen(4)).to(gpu)
+    loss = qat.top_logits_distillation_loss(x, values, ids, 2.0, "none")
+    g = torch.randn(rows, generator=_gen(8)).to(gpu)
+    gx, = torch.autograd.grad(loss, x, g)
+    _check_distill(x, values, ids, 2.0, "none", loss, gx, g)
 
 
 def test_distillation_special_rows(gpu):

@@ -82,7 +82,9 @@ def test_quantize_grouped_refuses():
     w = torch.randn(4, 64)
     for bad, match in ((lambda: ops.quantize_grouped(w[0]), "expects a weight"), (lambda: ops.quantize_grouped(w, 48), "multiple of 32"),
                        (lambda: ops.quantize_grouped(w, 0), "multiple of 32"), (lambda: ops.quantize_grouped(w[:0]), "expects a weight"),
-                       (lambda: ops.quantize_grouped(w / 0), "finite")):
+                       (lambda: ops.quantize_grouped(w / 0), "finite"),
+                       (lambda: ops.quantize_grouped(w, 32, scale_dtype=torch.float64), "scales must be"),
+                       (lambda: ops.quantize_grouped(w, 32, scale_dtype=torch.int8), "scales must be")):
         with pytest.raises(RuntimeError, match=match):
             bad()
 
@@ -152,6 +154,8 @@ def test_c_abi_norm_refusals():
     _refused(call(eps=-1.0), "eps")
     _refused(call(eps=float("nan")), "eps")
     _refused(call(x=None), "null")
+    _refused(call(x=P + 2), "misaligned")
+    _refused(call(dim=1 << 30, ldx=1 << 30), "2^30")
     _refused(call(y=None), "null")
     _refused(call(yd=E4M3), "with scales")
     _refused(call(scales=P), "with scales")
@@ -200,8 +204,15 @@ def test_c_abi_score_refusals():
     _refused(call(t=0.0), "temperature")
     _refused(call(t=float("nan")), "temperature")
     _refused(call(t=-1.0), "temperature")
+    _refused(call(t=0.0009), "temperature")
+    _refused(call(t=1001.0), "temperature")
+    _refused(call(t=float("inf")), "temperature")
     _refused(call(red=3), "reduction")
     _refused(call(k=-1), "entries")
+    _refused(call(k=4097), "entries")
+    _refused(call(x=P + 2), "misaligned")
+    b = _C.lib.dimq_distill_loss_backward
+    _refused(b(P, F32, 2, 100, 100, P, 1, 4097, P, P, 1.0, P, 0, None, P, None), "entries")
     _refused(call(ids=None), "null")
     _refused(call(norm=None), "null")
     _refused(call(rows=1, vocab=128000, ldx=128000, wsb=8), "workspace")
@@ -234,6 +245,9 @@ def test_c_abi_grouped_refusals():
     _refused(call(codes=None), "null")
     _refused(call(codes=P + 8), "aligned")
     _refused(call(x=P + 2), "misaligned")
+    _refused(call(scales=P + 1), "misaligned")
+    _refused(call(N=(1 << 31) - 1, variant=1, ws=P, wsb=1 << 60), "one launch")
+    _refused(call(M=1 << 30, variant=2, ws=P, wsb=1 << 60), "one launch")
     _refused(call(K=1 << 31, ldx=1 << 31), "2^31")
     assert call(M=0) == 0
     q = _C.lib.dimq_linear_grouped_workspace_bytes
