@@ -2,8 +2,9 @@
 
 Public API mirrors ``dimq_backend/__init__.py`` of the reference
 (``dimq_cuda_backend/dimq_backend/__init__.py:3-37``), plus the weight-only,
-b-bit, per-channel codebook layers and ops, and microscaled 4-bit layers with
-8-bit activation checkpoints (``mx``).  The CPU reference functions of
+b-bit, per-channel codebook layers and ops, microscaled 4-bit layers with
+8-bit activation checkpoints (``mx``), and operators of quantized language
+models (group-scaled 4-bit layers, RMS norm, scores, distillation).  The CPU reference functions of
 the reference package (``dimq_linear_reference`` ...) are test oracles and
 live in ``oracle/``, not here.
 """
