@@ -17,6 +17,8 @@
 // LB 16 for groups of multiples of 128, 8 for other multiples of 64, 4 for other multiples of 32.
 #include "decode.h"
 
+#include <type_traits>
+
 namespace dimq {
 namespace {
 
@@ -268,7 +270,8 @@ __device__ __forceinline__ void put8(const GroupArgs& p, int64_t off, int left, 
 // ---- few rows -----------------------------------------------------------------------------------------------------
 // 16 MT rows by 16 NC columns a work-group; its 8 waves share out the spans, and their sums meet in the LDS.  A wave takes its
 // spans one after another: what hides their loads is the other waves of the CU (several spans' loads sent out together, or x
-// a span ahead, gained nothing at 4096 -> 4096 and lost up to a half where a wave has few spans, for their registers).
+// a span ahead, gained nothing at 4096 -> 4096 and lost up to a half where a wave has few spans, for their registers; 16 waves are
+// 0 to 3 % slower, in fp32 up to 60 %).  16 x 4096 -> 12288, e4m3, groups of 128: 13.7 us (27 MB, 2 TB/s).
 // Lanes whose row is past M load no x: their sums are not stored.
 constexpr int kFewWaves = 8;
 
@@ -357,16 +360,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void group_few_kernel(const GroupAr
 #pragma unroll
     for (int c = 0; c < NC; ++c) red[wave][t * NC + c][lane] = acc[t][c];
   __syncthreads();
-  if (wave >= MT * NC) return;
-  const int64_t n = n0 + 16 * (wave % NC) + col;
-  floatx4 v = red[0][wave][lane];
+  for (int tile = wave; tile < MT * NC; tile += kFewWaves) {
+    const int64_t n = n0 + 16 * (tile % NC) + col;
+    floatx4 v = red[0][tile][lane];
 #pragma unroll
-  for (int w = 1; w < kFewWaves; ++w) v += red[w][wave][lane];
-  if (n >= p.N) return;
+    for (int w = 1; w < kFewWaves; ++w) v += red[w][tile][lane];
+    if (n >= p.N) continue;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + 16 * (wave / NC) + 4 * quarter + i;
-    if (m < p.M) put_output(p, m, n, v[i] * row_scale(p, m));
+    for (int i = 0; i < 4; ++i) {
+      const int64_t m = m0 + 16 * (tile / NC) + 4 * quarter + i;
+      if (m < p.M) put_output(p, m, n, v[i] * row_scale(p, m));
+    }
   }
 }
 
@@ -767,13 +771,15 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs p) {
 int span_bytes(int64_t group) { return group % 128 == 0 ? 16 : group % 64 == 0 ? 8 : 4; }
 
 // Products of fewer multiply-adds than this run on the first kernel, larger ones on the tiles, whose three launches cost about
-// 20 us before the first product.  At K 4096, groups of 128, bf16 (in us, first kernel / tiles): 64 x 4096 16 / 29, 128 x 4096
-// 28 / 34, 256 x 4096 52 / 37, 64 x 12288 42 / 38.
-constexpr double kFewProducts = 2.5e9;
-bool few_rows(int64_t M, int64_t K, int64_t N, int variant) {
+// 20 us before the first product.  In us, bf16, groups of 128 (first kernel / tiles): K 4096, 128 x 4096 24 / 34, 256 x 4096 35 / 35,
+// 384 x 4096 66 / 41, 64 x 12288 30 / 36, 128 x 12288 58 / 40, 32 x 28000 46 / 53, 64 x 28000 69 / 56; K 1024, 384 x 8192 33 / 37,
+// 512 x 8192 43 / 37; K 2048, 1024 x 2048 38 / 36.  fp32, whose three planes cost the first kernel more: K 4096, 128 x 4096 50 / 50,
+// 192 x 4096 73 / 52, 64 x 12288 66 / 68.
+bool few_rows(int xt, int64_t M, int64_t K, int64_t N, int variant) {
   // row and column blocks of one launch
   if (variant == DIMQ_VARIANT_MFMA || M > int64_t{65535} * 16 || N > (int64_t{1} << 23) * 16 - 16) return false;
-  return variant == DIMQ_VARIANT_SMALL_M || static_cast<double>(M) * static_cast<double>(K) * static_cast<double>(N) < kFewProducts;
+  const double most = xt == DIMQ_F32 ? 2.1e9 : 4e9;
+  return variant == DIMQ_VARIANT_SMALL_M || static_cast<double>(M) * static_cast<double>(K) * static_cast<double>(N) < most;
 }
 
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -811,34 +817,43 @@ bool rows_in_place(const void* x, int xt, int64_t M, int64_t K, int64_t ldx) {
   return x_size(xt) == 2 && K % kTileK == 0 && rows_aligned(x, xt, M, ldx) && ldx < kMostApart;
 }
 
-// Blocks of 16 rows and of 16 columns a work-group: more columns read x less often, more rows the codes, but both leave fewer
-// work-groups.  In us, at 4096 -> 4096 / 4096 -> 12288, groups of 128, bf16 (MT x NC): 1 row 1x1 6.5 / 13.4, 1x4 15.1 / 15.5; 16
-// rows 1x1 9.7 / 21.8, 1x4 17.9 / 18.4; 32 rows 1x1 15.8 / 40.0, 1x2 12.5 / 30.0, 2x2 16.1 / 29.5; 64 rows 1x1 27.8 / 76.1, 2x2
-// 16.3 / 43.1, 4x1 20.4 / 57.8; fp32, 37 rows: 1x1 40.9 / 117, 1x4 24.8 / 64.7, 2x2 30.8 / 79.4.  Groups of 32, whose codes are
-// loaded by 4 bytes: 32 rows 1x1 31.9, 1x2 27.8, 2x1 21.4; 64 rows 2x2 31.6, 2x1 38.6, 4x1 28.0.
+// Blocks of 16 rows (MT) and of 16 columns (NC) a work-group.  Its time goes as the loads and conversions of a span,
+// x_cost MT + code_cost NC, whatever MT NC products they feed, and one CU's work-groups add up: the plan is the one
+// of least work-groups a CU times that.  Over 150 calls of 1 to 256 rows, K 1000 to 4096 and N 1030 to 28000, each measured on
+// all plans, the choice is 1.2 % slower than the best in the mean, 18 % at worst.  In us, bf16, K 4096, groups of 128 (MT x NC):
+// 16 x 12288 1x1 22.1, 1x2 21.9, 1x3 16.0, 1x4 19.4; 64 x 12288 1x1 77, 2x2 42, 4x3 30.5; 256 x 4096 1x1 101, 4x4 34.9; groups of
+// 32: 64 x 12288 1x1 171, 4x1 79, 4x3 52.8.
+template <int XT, int LB>
+constexpr bool few_plan(int mt, int nc) {
+  return XT != DIMQ_F32 || (mt <= 2 && (LB < 16 || mt * nc < 8));  // fp32 spans of 128 by 2 x 4 blocks: spilled registers
+}
+
 template <int XT, int LB>
 void launch_few(const GroupArgs& p, hipStream_t s) {
-  const int64_t gm = (p.M + 15) / 16, gn = (p.N + 15) / 16;
-  const auto go = [&](auto kernel, int mt, int nc) {
-    const dim3 grid(static_cast<unsigned>((gn + nc - 1) / nc), static_cast<unsigned>((gm + mt - 1) / mt));
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kFewWaves), 0, s, p);
+  constexpr int kXCost = XT == DIMQ_F32 ? 4 : 1, kCodeCost = LB == 16 ? 1 : LB == 8 ? 2 : 3;
+  const int64_t gm = (p.M + 15) / 16, gn = (p.N + 15) / 16, cus = device_cus();
+  int64_t least = INT64_MAX;
+  int plan = 0;
+  const auto each_plan = [](auto f) {
+    const auto columns = [&](auto mt) {
+      f(mt, std::integral_constant<int, 1>()), f(mt, std::integral_constant<int, 2>());
+      f(mt, std::integral_constant<int, 3>()), f(mt, std::integral_constant<int, 4>());
+    };
+    columns(std::integral_constant<int, 1>()), columns(std::integral_constant<int, 2>()), columns(std::integral_constant<int, 4>());
   };
-  const bool wide = gn >= 128, widest = gn >= 640;  // columns for half of the CUs, for all of them with 4 blocks each
-  if constexpr (XT == DIMQ_F32) {
-    if (LB == 4 && wide && gm >= 2) go(group_few_kernel<XT, LB, 2, 2>, 2, 2);
-    else if ((widest && p.M > 4) || (wide && gm >= 3)) go(group_few_kernel<XT, LB, 1, 4>, 1, 4);
-    else if (wide && gm == 2) go(group_few_kernel<XT, LB, 1, 2>, 1, 2);
-    else go(group_few_kernel<XT, LB, 1, 1>, 1, 1);
-  } else if constexpr (LB == 4) {
-    if (wide && gm >= 3) go(group_few_kernel<XT, LB, 4, 1>, 4, 1);
-    else if (wide && gm == 2) go(group_few_kernel<XT, LB, 2, 1>, 2, 1);
-    else go(group_few_kernel<XT, LB, 1, 1>, 1, 1);
-  } else {
-    if ((wide && gm >= 3) || (widest && gm == 2)) go(group_few_kernel<XT, LB, 2, 2>, 2, 2);
-    else if (wide && gm == 2) go(group_few_kernel<XT, LB, 1, 2>, 1, 2);
-    else if (widest && p.M > 4) go(group_few_kernel<XT, LB, 1, 4>, 1, 4);
-    else go(group_few_kernel<XT, LB, 1, 1>, 1, 1);
-  }
+  each_plan([&](auto mt, auto nc) {
+    if (!few_plan<XT, LB>(mt, nc)) return;
+    const int64_t groups = ((gm + mt - 1) / mt) * ((gn + nc - 1) / nc), cost = kXCost * mt + kCodeCost * nc;
+    const int64_t all = ((groups + cus - 1) / cus * cost) << 8 | cost;  // among equals the smaller work-group
+    if (all < least) least = all, plan = mt * 8 + nc;
+  });
+  each_plan([&](auto mt, auto nc) {
+    if constexpr (few_plan<XT, LB>(mt, nc)) {
+      if (plan != mt * 8 + nc) return;
+      const dim3 grid(static_cast<unsigned>((gn + nc - 1) / nc), static_cast<unsigned>((gm + mt - 1) / mt));
+      hipLaunchKernelGGL((group_few_kernel<XT, LB, mt, nc>), grid, dim3(64 * kFewWaves), 0, s, p);
+    }
+  });
 }
 
 template <int XT, int LB>
@@ -873,7 +888,7 @@ using namespace dimq;
 
 extern "C" int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int64_t N,
                                                        int variant) {
-  if (M <= 0 || K <= 0 || N <= 0 || few_rows(M, K, N, variant)) return 0;
+  if (M <= 0 || K <= 0 || N <= 0 || few_rows(x_dtype, M, K, N, variant)) return 0;
   if (x_dtype != DIMQ_F32 && x_dtype != DIMQ_F16 && x_dtype != DIMQ_BF16 && x_dtype != DIMQ_E4M3) return 0;
   const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
   return t.bytes();
@@ -926,7 +941,7 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
     case DIMQ_BF16: DIMQ_GROUP_LB(F, DIMQ_BF16, __VA_ARGS__) break;    \
     default: DIMQ_GROUP_LB(F, DIMQ_E4M3, __VA_ARGS__)                  \
   }
-  if (few_rows(M, K, N, variant)) {
+  if (few_rows(x_dtype, M, K, N, variant)) {
     DIMQ_GROUP_XT(launch_few, p, s)
   } else {
     const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));

@@ -189,6 +189,49 @@ def test_more_columns_than_tiles_and_split_sums(gpu, variant):
             assert torch.equal(y.cpu().double(), _ref(x, layer, group, _c(x, m)))
 
 
+# (rows, columns) that between them take every plan of the few-row kernel: 16, 32 or 64 rows by 16 to 64 columns a work-group
+PLANS = [(5, 1001), (5, 8100), (16, 12280), (3, 16379), (33, 4099), (47, 8190), (30, 12271), (20, 16300), (60, 4090), (63, 8189),
+         (50, 12280), (64, 16381), (130, 2050)]
+
+
+@pytest.mark.parametrize("dt", XTYPES)
+@pytest.mark.parametrize("m,n", PLANS)
+def test_plans_of_few_rows(gpu, m, n, dt):
+    announce(f"grouped plans {m} {n} {dt}")
+    k = 1300
+    x = _ints(m, k, dt, m)
+    xs = _c(x, m)
+    some = torch.cat([torch.randint(0, n, (60,), generator=_gen(4)), torch.arange(n - 20, n)])
+    bias, res = torch.randint(-9, 9, (n,), generator=_gen(5)).float(), torch.randint(-9, 9, (m, n), generator=_gen(6)).float()
+    for group in (32, 64, 128):
+        g = _gen(group)
+        codes = torch.randint(0, 256, (n, -(-k // 32) * 16), generator=g, dtype=torch.uint8)
+        scales = 2.0 ** torch.randint(-2, 2, (n, -(-k // group)), generator=g)
+        zeros = torch.randint(0, 16, scales.shape, generator=g, dtype=torch.uint8)
+        y = _run(gpu, x, (codes, scales, zeros), group, xs, bias=bias, residual=res, out_dtype=torch.float32, variant="small_m")
+        ref = _ref(x, (codes[some], scales[some], zeros[some]), group, xs) + bias[some] + res[:, some]
+        assert torch.equal(y.cpu()[:, some].double(), ref), group
+
+
+@pytest.mark.parametrize("dt", XTYPES)
+def test_products_that_auto_gives_to_each_kernel(gpu, dt):
+    """On both sides of the sizes at which the kernels change."""
+    from dimq_amd import _C
+    announce(f"grouped routes {dt}")
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 5}[dt]
+    most = 2.1e9 if dt == torch.float32 else 4e9
+    m = int(most / (1024 * 4096))
+    for rows in (m, m + 1):
+        x, layer = _ints(rows, 1024, dt, 1), _layer(4096, 1024, 128, 2)
+        xs = _c(x, rows)
+        at = x.to(gpu)
+        tiles = _C.lib.dimq_linear_grouped_workspace_bytes(at.data_ptr(), code, rows, 1024, 1024, 4096, 0) > 0
+        assert tiles == (rows > m)
+        y = _run(gpu, x, layer, 128, xs, out_dtype=torch.float32)
+        some = torch.randint(0, rows, (20,), generator=_gen(5))
+        assert torch.equal(y.cpu()[some].double(), _ref(x[some], layer, 128, None if xs is None else xs[some]))
+
+
 def test_large_products_choose_tiles(gpu):
     announce("grouped large")
     x, layer = _ints(700, 1024, torch.bfloat16, 1), _layer(4096, 1024, 128, 2)
