@@ -154,7 +154,7 @@ _SIGS = {
                                  _vp, _vp, _i64, _vp]),
     "dimq_distill_loss_backward": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp, _dbl, _vp, _i64, _vp, _vp,
                                           _vp]),
-    "dimq_linear_grouped_workspace_bytes": (_i64, [_vp, _int, _i64, _i64, _i64, _i64, _int]),
+    "dimq_linear_grouped_workspace_bytes": (_i64, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _int]),
     "dimq_linear_grouped": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _i64, _vp, _int, _i64, _vp, _int, _vp,
                                    _int, _int, _int, _vp, _i64, _vp]),
     "dimq_separation_loss": (_int, [_vp, _int, _i64, _vp, _i64, _dbl, _dbl, _vp, _vp, _vp, _i64, _vp]),

@@ -268,22 +268,49 @@ __device__ __forceinline__ void put8(const GroupArgs& p, int64_t off, int left, 
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
-// 16 MT rows by 16 NC columns a work-group; its 8 waves share out the spans, and their sums meet in the LDS.  A wave takes its
-// spans one after another: what hides their loads is the other waves of the CU (several spans' loads sent out together, or x
-// a span ahead, gained nothing at 4096 -> 4096 and lost up to a half where a wave has few spans, for their registers; 16 waves are
+// 16 MT rows by 16 NC columns a work-group; its 8 waves share out the k in turns of 128, and their sums meet in the LDS.  Codes
+// come by 16 bytes a lane whatever the spans; shorter ones are dealt out among a column's four lanes by swaps of their rows.  A
+// wave takes its turns one after another: what hides their loads is the other waves of the CU (several turns' loads sent out together, or x
+// a span ahead, gained nothing at 4096 -> 4096 and lost up to a half where a wave has few of them, for their registers; 16 waves are
 // 0 to 3 % slower, in fp32 up to 60 %).  16 x 4096 -> 12288, e4m3, groups of 128: 13.7 us (27 MB, 2 TB/s).
 // Lanes whose row is past M load no x: their sums are not stored.
 constexpr int kFewWaves = 8;
 
+// Rows of 16 lanes: (a0 b0 a2 b2), (a1 b1 a3 b3), and (a0 a1 b0 b1), (a2 a3 b2 b3).
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+// A lane's 16 bytes of a turn's 64, quarter after quarter, to the LB bytes of each of its 16 / LB spans that the lane takes.
+template <int LB>
+__device__ __forceinline__ void to_spans(uint32_t (&w)[4]) {
+  if constexpr (LB == 8) swap32(w[0], w[2]), swap32(w[1], w[3]);
+  if constexpr (LB == 4) swap16(w[0], w[1]), swap16(w[2], w[3]), swap32(w[0], w[2]), swap32(w[1], w[3]);
+}
+// What the quarters hold of a turn's spans (LB 8: of the first span in the first two) to every lane.
+template <int LB>
+__device__ __forceinline__ void to_lanes(uint32_t v, uint32_t (&o)[16 / LB]) {
+#pragma unroll
+  for (int i = 0; i < 16 / LB; ++i) o[i] = v;
+  if constexpr (LB == 8) swap32(o[0], o[1]);
+  if constexpr (LB == 4) swap16(o[0], o[1]), swap16(o[2], o[3]), swap32(o[0], o[2]), swap32(o[1], o[3]);
+}
+
 template <int XT, int LB, int MT, int NC>
 __global__ __launch_bounds__(64 * kFewWaves) void group_few_kernel(const GroupArgs p) {
-  constexpr int ML = mul_type(XT), P = planes_of(XT), SP = 8 * LB;
+  constexpr int ML = mul_type(XT), P = planes_of(XT), SP = 8 * LB, S = 16 / LB;
   __shared__ floatx4 red[kFewWaves][MT * NC][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NC), m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
-  const int spans = static_cast<int>((p.nb * 32 + SP - 1) / SP), each = (spans + kFewWaves - 1) / kFewWaves;
-  const int from = wave * each, to = from + each < spans ? from + each : spans;
-  const uint32_t group_spans = static_cast<uint32_t>(p.group / SP);  // a group is a whole number of spans
+  const int turns = static_cast<int>((p.nb + 3) / 4), each = (turns + kFewWaves - 1) / kFewWaves;
+  const int from = wave * each, to = from + each < turns ? from + each : turns;
+  const uint32_t group_spans = static_cast<uint32_t>(p.group / SP), last = static_cast<uint32_t>(p.groups - 1);
+  const int mine = LB == 4 ? quarter : LB == 8 ? quarter >> 1 : 0;  // the span whose scale the lane loads
+  const int xat = LB == 8 ? (quarter & 1) * 32 + (quarter >> 1) * 16 : quarter * (2 * LB);  // the lane's first k of a span
   const uint8_t* cw[NC];
   int64_t gn[NC];
 #pragma unroll
@@ -299,59 +326,67 @@ __global__ __launch_bounds__(64 * kFewWaves) void group_few_kernel(const GroupAr
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[t][c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int sp = from; sp < to; ++sp) {
-    // a lane's codes past the row's last block read that block's (x is 0 there)
-    int64_t at = static_cast<int64_t>(sp) * (4 * LB) + quarter * LB;
-    if (at + LB > p.pitch) at = p.pitch - LB;
-    uint32_t codes[NC][LB / 4], rs[NC], z[NC];
+  for (int turn = from; turn < to; ++turn) {
+    // a lane's codes past the row's last block are that block's (x is 0 there), scales past the last group that group's
+    int64_t at = static_cast<int64_t>(turn) * 64 + quarter * 16;
+    if (at + 16 > p.pitch) at = p.pitch - 16;
+    uint32_t codes[NC][4], rs[NC], z[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if constexpr (LB == 16) {
-        const uint4 w = *reinterpret_cast<const uint4*>(cw[c] + at);
-        codes[c][0] = w.x, codes[c][1] = w.y, codes[c][2] = w.z, codes[c][3] = w.w;
-      } else if constexpr (LB == 8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(cw[c] + at);
-        codes[c][0] = w.x, codes[c][1] = w.y;
-      } else {
-        codes[c][0] = *reinterpret_cast<const uint32_t*>(cw[c] + at);
-      }
+      const uint4 w = *reinterpret_cast<const uint4*>(cw[c] + at);
+      codes[c][0] = w.x, codes[c][1] = w.y, codes[c][2] = w.z, codes[c][3] = w.w;
     }
-    RawX<XT, LB> rx[MT];
-    const int64_t k0 = static_cast<int64_t>(sp) * SP + quarter * (2 * LB);
-    const bool fast = p.vec && static_cast<int64_t>(sp + 1) * SP <= p.K;
+    RawX<XT, LB> rx[MT][S];
+    const int64_t k0 = static_cast<int64_t>(turn) * 128 + xat;
+    const bool fast = p.vec && static_cast<int64_t>(turn + 1) * 128 <= p.K;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       const int64_t m = m0 + 16 * t + col;
-      if (m < p.M) rx[t].load(p, m, k0, fast);
+      if (m < p.M) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) rx[t][s].load(p, m, k0 + s * SP, fast);
+      }
     }
-    const uint32_t g = static_cast<uint32_t>(sp) / group_spans;
+    uint32_t g = (static_cast<uint32_t>(turn) * S + mine) / group_spans;
+    g = g < last ? g : last;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       rs[c] = scales.load(gn[c] + g);
       z[c] = zeros[gn[c] + g];
     }
-    uint32_t b[NC][LB];
-    float s[NC], zf[NC];
+    uint32_t sv[NC][S], zv[NC][S];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      decode_span<ML, LB>(codes[c], b[c]);
-      s[c] = scales.value(rs[c], static_cast<uint32_t>(gn[c]) + g);
-      zf[c] = p.zeros ? static_cast<float>(z[c]) : 8.0f;
+      to_spans<LB>(codes[c]);
+      to_lanes<LB>(__float_as_uint(scales.value(rs[c], static_cast<uint32_t>(gn[c]) + g)), sv[c]);
+      to_lanes<LB>(__float_as_uint(p.zeros ? static_cast<float>(z[c]) : 8.0f), zv[c]);
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      uint32_t a[P][LB];
-      rx[t].planes(a);
-      floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < P; ++i) x = sum_span<ML, LB>(a[i], x);
+    for (int s = 0; s < S; ++s) {
+      uint32_t b[NC][LB];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        floatx4 q = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t part[LB / 4];
 #pragma unroll
-        for (int i = 0; i < P; ++i) q = mul_span<ML, LB>(a[i], b[c], q);
+        for (int i = 0; i < LB / 4; ++i) part[i] = codes[c][s * (LB / 4) + i];
+        decode_span<ML, LB>(part, b[c]);
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][c][i] = fmaf(s[c], fmaf(-zf[c], x[i], q[i]), acc[t][c][i]);
+      for (int t = 0; t < MT; ++t) {
+        uint32_t a[P][LB];
+        rx[t][s].planes(a);
+        floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < P; ++i) x = sum_span<ML, LB>(a[i], x);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          floatx4 q = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < P; ++i) q = mul_span<ML, LB>(a[i], b[c], q);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[t][c][i] = fmaf(__uint_as_float(sv[c][s]), fmaf(-__uint_as_float(zv[c][s]), x[i], q[i]), acc[t][c][i]);
+        }
       }
     }
   }
@@ -775,12 +810,17 @@ int span_bytes(int64_t group) { return group % 128 == 0 ? 16 : group % 64 == 0 ?
 // 384 x 4096 66 / 41, 64 x 12288 30 / 36, 128 x 12288 58 / 40, 32 x 28000 46 / 53, 64 x 28000 69 / 56; K 1024, 384 x 8192 33 / 37,
 // 512 x 8192 43 / 37; K 2048, 1024 x 2048 38 / 36.  fp32, whose three planes cost the first kernel more: K 4096, 128 x 4096 50 / 50,
 // 192 x 4096 73 / 52, 64 x 12288 66 / 68.
-bool few_rows(int xt, int64_t M, int64_t K, int64_t N, int variant) {
+// With groups that are no multiple of 64 the tiles decode and scale in spans of 32 and are slower: 256 x 4096 35 / 58,
+// 192 x 12288 85 / 98, 256 x 12288 102 / 99, in fp32 192 x 4096 81 / 86, 256 x 4096 106 / 88.
+bool few_rows(int xt, int64_t M, int64_t K, int64_t N, int64_t group, int variant) {
   // row and column blocks of one launch
   if (variant == DIMQ_VARIANT_MFMA || M > int64_t{65535} * 16 || N > (int64_t{1} << 23) * 16 - 16) return false;
-  const double most = xt == DIMQ_F32 ? 2.1e9 : 4e9;
+  const bool fp32 = xt == DIMQ_F32, shorter = span_bytes(group) == 4;
+  const double most = fp32 ? (shorter ? 3.5e9 : 2.1e9) : (shorter ? 8e9 : 4e9);
   return variant == DIMQ_VARIANT_SMALL_M || static_cast<double>(M) * static_cast<double>(K) * static_cast<double>(N) < most;
 }
+// One group a row, however large: the longest spans.
+int64_t group_of(int64_t group, int64_t K) { return group >= K ? (K + 127) / 128 * 128 : group; }
 
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
@@ -817,20 +857,20 @@ bool rows_in_place(const void* x, int xt, int64_t M, int64_t K, int64_t ldx) {
   return x_size(xt) == 2 && K % kTileK == 0 && rows_aligned(x, xt, M, ldx) && ldx < kMostApart;
 }
 
-// Blocks of 16 rows (MT) and of 16 columns (NC) a work-group.  Its time goes as the loads and conversions of a span,
-// x_cost MT + code_cost NC, whatever MT NC products they feed, and one CU's work-groups add up: the plan is the one
-// of least work-groups a CU times that.  Over 150 calls of 1 to 256 rows, K 1000 to 4096 and N 1030 to 28000, each measured on
-// all plans, the choice is 1.2 % slower than the best in the mean, 18 % at worst.  In us, bf16, K 4096, groups of 128 (MT x NC):
-// 16 x 12288 1x1 22.1, 1x2 21.9, 1x3 16.0, 1x4 19.4; 64 x 12288 1x1 77, 2x2 42, 4x3 30.5; 256 x 4096 1x1 101, 4x4 34.9; groups of
-// 32: 64 x 12288 1x1 171, 4x1 79, 4x3 52.8.
+// Blocks of 16 rows (MT) and of 16 columns (NC) a work-group.  Its time goes as the loads and conversions of a turn, MT + NC (fp32,
+// with three planes of x, 4 MT + NC), whatever MT NC products they feed, and one CU's work-groups add up: the plan is the one of
+// least work-groups a CU times that.  Over 150 calls of 1 to 256 rows, K 1000 to 4096, N 1030 to 28000 and groups of 32, 64 and 128,
+// each measured on all plans, the choice is 0.4 % slower than the best in the mean, 6 % at worst.  In us, bf16, K 4096, groups of
+// 128 (MT x NC): 16 x 12288 1x1 22.1, 1x2 21.9, 1x3 16.0, 1x4 19.4; 64 x 12288 1x1 77, 2x2 42, 4x3 30.5; 256 x 4096 1x1 101, 4x4
+// 34.9; groups of 32: 1 x 4096 1x1 7.6, 64 x 12288 1x1 81, 4x3 30.3 (with codes loaded by 4 bytes 14.5 and 52.8).
 template <int XT, int LB>
 constexpr bool few_plan(int mt, int nc) {
-  return XT != DIMQ_F32 || (mt <= 2 && (LB < 16 || mt * nc < 8));  // fp32 spans of 128 by 2 x 4 blocks: spilled registers
+  return XT != DIMQ_F32 || (mt <= 2 && mt * nc < (LB == 4 ? 6 : 8));  // more would spill registers
 }
 
 template <int XT, int LB>
 void launch_few(const GroupArgs& p, hipStream_t s) {
-  constexpr int kXCost = XT == DIMQ_F32 ? 4 : 1, kCodeCost = LB == 16 ? 1 : LB == 8 ? 2 : 3;
+  constexpr int kXCost = XT == DIMQ_F32 ? 4 : 1;
   const int64_t gm = (p.M + 15) / 16, gn = (p.N + 15) / 16, cus = device_cus();
   int64_t least = INT64_MAX;
   int plan = 0;
@@ -843,7 +883,7 @@ void launch_few(const GroupArgs& p, hipStream_t s) {
   };
   each_plan([&](auto mt, auto nc) {
     if (!few_plan<XT, LB>(mt, nc)) return;
-    const int64_t groups = ((gm + mt - 1) / mt) * ((gn + nc - 1) / nc), cost = kXCost * mt + kCodeCost * nc;
+    const int64_t groups = ((gm + mt - 1) / mt) * ((gn + nc - 1) / nc), cost = kXCost * mt + nc;
     const int64_t all = ((groups + cus - 1) / cus * cost) << 8 | cost;  // among equals the smaller work-group
     if (all < least) least = all, plan = mt * 8 + nc;
   });
@@ -886,9 +926,9 @@ void launch_tile(GroupArgs p, const TilePlan& t, uint8_t* ws, hipStream_t s) {
 
 using namespace dimq;
 
-extern "C" int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int64_t N,
-                                                       int variant) {
-  if (M <= 0 || K <= 0 || N <= 0 || few_rows(x_dtype, M, K, N, variant)) return 0;
+extern "C" int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,
+                                                       int64_t group, int64_t N, int variant) {
+  if (M <= 0 || K <= 0 || N <= 0 || few_rows(x_dtype, M, K, N, group_of(group, K), variant)) return 0;
   if (x_dtype != DIMQ_F32 && x_dtype != DIMQ_F16 && x_dtype != DIMQ_BF16 && x_dtype != DIMQ_E4M3) return 0;
   const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));
   return t.bytes();
@@ -920,7 +960,7 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
   DIMQ_CHECK(aligned(codes, 16), "linear_grouped: codes must be 16-byte aligned");
   DIMQ_CHECK(aligned(scales, dtype_size(scales_dtype)), "linear_grouped: misaligned scales");
   DIMQ_CHECK(aligned(x, x_dtype == DIMQ_E4M3 ? 1 : dtype_size(x_dtype)), "linear_grouped: misaligned input");
-  if (group >= K) group = (K + 127) / 128 * 128;  // one group a row, however large: the longest spans
+  group = group_of(group, K);
   GroupArgs p{};
   p.x = x, p.M = M, p.K = K, p.ldx = ldx, p.xs = x_scales, p.vec = rows_aligned(x, x_dtype, M, ldx);
   p.nb = (K + 31) / 32, p.codes = codes, p.pitch = p.nb * 16, p.scales = scales, p.s_dt = scales_dtype, p.zeros = zeros;
@@ -941,7 +981,7 @@ extern "C" int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_
     case DIMQ_BF16: DIMQ_GROUP_LB(F, DIMQ_BF16, __VA_ARGS__) break;    \
     default: DIMQ_GROUP_LB(F, DIMQ_E4M3, __VA_ARGS__)                  \
   }
-  if (few_rows(x_dtype, M, K, N, variant)) {
+  if (few_rows(x_dtype, M, K, N, group, variant)) {
     DIMQ_GROUP_XT(launch_few, p, s)
   } else {
     const TilePlan t = tile_plan(x_dtype, M, K, N, rows_in_place(x, x_dtype, M, K, ldx));

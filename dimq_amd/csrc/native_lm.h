@@ -318,7 +318,7 @@ Tensor linear_grouped(const Tensor& x, const Tensor& codes, const Tensor& scales
   const int xdt = q8 ? static_cast<int>(DIMQ_E4M3) : dt(x);
   const Tensor y = at::empty(shape, x.options().dtype(odt));
   const On on(x);
-  const Tensor ws = workspace(dimq_linear_grouped_workspace_bytes(ptr(t), xdt, M, K, ld, N, static_cast<int>(variant)), c);
+  const Tensor ws = workspace(dimq_linear_grouped_workspace_bytes(ptr(t), xdt, M, K, ld, group, N, static_cast<int>(variant)), c);
   check_rc(dimq_linear_grouped(ptr(t), xdt, M, K, ld, static_cast<float*>(ptr(xs)), u8(c), ptr(s), dt(s),
                                static_cast<uint8_t*>(ptr(z)), group, b.p, b.dtype, N, ptr(y), dt(y), r.p, r.dtype,
                                static_cast<int>(activation), static_cast<int>(variant), ptr(ws), ws.defined() ? ws.numel() : 0,

@@ -696,8 +696,8 @@ int dimq_distill_loss_backward(const void* student, int dtype, int64_t rows, int
  * fixed order, one rounding to y_dtype; bias [N] and residual [M, N] nullable,
  * any float dtype.  variant: DIMQ_VARIANT_SMALL_M one launch for few outputs,
  * DIMQ_VARIANT_MFMA tiles, DIMQ_VARIANT_AUTO by size. */
-int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int64_t N,
-                                            int variant);
+int64_t dimq_linear_grouped_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int64_t group,
+                                            int64_t N, int variant);
 int dimq_linear_grouped(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const float* x_scales,
                         const uint8_t* codes, const void* scales, int scales_dtype, const uint8_t* zeros, int64_t group,
                         const void* bias, int bias_dtype, int64_t N, void* y, int y_dtype, const void* residual,

@@ -213,23 +213,23 @@ def test_plans_of_few_rows(gpu, m, n, dt):
         assert torch.equal(y.cpu()[:, some].double(), ref), group
 
 
+@pytest.mark.parametrize("group,most32,most16", [(128, 2.1e9, 4e9), (64, 2.1e9, 4e9), (96, 3.5e9, 8e9)])
 @pytest.mark.parametrize("dt", XTYPES)
-def test_products_that_auto_gives_to_each_kernel(gpu, dt):
+def test_products_that_auto_gives_to_each_kernel(gpu, dt, group, most32, most16):
     """On both sides of the sizes at which the kernels change."""
     from dimq_amd import _C
-    announce(f"grouped routes {dt}")
+    announce(f"grouped routes {dt} {group}")
     code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 5}[dt]
-    most = 2.1e9 if dt == torch.float32 else 4e9
-    m = int(most / (1024 * 4096))
+    m = int((most32 if dt == torch.float32 else most16) / (1024 * 4096))
     for rows in (m, m + 1):
-        x, layer = _ints(rows, 1024, dt, 1), _layer(4096, 1024, 128, 2)
+        x, layer = _ints(rows, 1024, dt, 1), _layer(4096, 1024, group, 2)
         xs = _c(x, rows)
         at = x.to(gpu)
-        tiles = _C.lib.dimq_linear_grouped_workspace_bytes(at.data_ptr(), code, rows, 1024, 1024, 4096, 0) > 0
+        tiles = _C.lib.dimq_linear_grouped_workspace_bytes(at.data_ptr(), code, rows, 1024, 1024, group, 4096, 0) > 0
         assert tiles == (rows > m)
-        y = _run(gpu, x, layer, 128, xs, out_dtype=torch.float32)
+        y = _run(gpu, x, layer, group, xs, out_dtype=torch.float32)
         some = torch.randint(0, rows, (20,), generator=_gen(5))
-        assert torch.equal(y.cpu()[some].double(), _ref(x[some], layer, 128, None if xs is None else xs[some]))
+        assert torch.equal(y.cpu()[some].double(), _ref(x[some], layer, group, None if xs is None else xs[some]))
 
 
 def test_large_products_choose_tiles(gpu):

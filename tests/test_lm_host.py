@@ -251,12 +251,12 @@ def test_c_abi_grouped_refusals():
     _refused(call(K=1 << 31, ldx=1 << 31), "2^31")
     assert call(M=0) == 0
     q = _C.lib.dimq_linear_grouped_workspace_bytes
-    assert q(P, F32, 2, 64, 64, 4, 0) == 0 and q(P, F32, 2, 64, 64, 4, 1) == 0 and q(P, F32, 2, 64, 64, 4, 2) > 0
-    assert q(P, F16, 2048, 4096, 4096, 4096, 0) > 0 and q(P, 3, 2048, 4096, 4096, 4096, 0) == 0
+    assert q(P, F32, 2, 64, 64, 32, 4, 0) == 0 and q(P, F32, 2, 64, 64, 32, 4, 1) == 0 and q(P, F32, 2, 64, 64, 32, 4, 2) > 0
+    assert q(P, F16, 2048, 4096, 4096, 32, 4096, 0) > 0 and q(P, 3, 2048, 4096, 4096, 32, 4096, 0) == 0
     _refused(call(variant=2), "workspace")
-    need = q(P, F32, 2, 64, 64, 4, 2)
+    need = q(P, F32, 2, 64, 64, 32, 4, 2)
     _refused(call(variant=2, ws=P, wsb=need - 1), "workspace")
     _refused(call(variant=2, ws=P + 8, wsb=need), "workspace")
     # copies are made of rows that cannot be read in place
-    assert q(P, F16, 4096, 4096, 4096, 4096, 2) < q(P + 2, F16, 4096, 4096, 4096, 4096, 2)
-    assert q(P, F16, 4096, 4096, 4096, 4096, 2) < q(P, F16, 4096, 4096, 4097, 4096, 2)
+    assert q(P, F16, 4096, 4096, 4096, 32, 4096, 2) < q(P + 2, F16, 4096, 4096, 4096, 32, 4096, 2)
+    assert q(P, F16, 4096, 4096, 4096, 32, 4096, 2) < q(P, F16, 4096, 4096, 4097, 32, 4096, 2)
