@@ -13,7 +13,7 @@
 // largest: against 64 bits, sums of 32 products were up to 4,700 2^-24 of their terms' magnitudes off, in bf16 0.1.
 //
 // Which 32 k of an instruction's share a lane holds is free as long as both operands agree: lane l (column or row l % 16,
-// quarter l / 16) takes 2 LB consecutive k of a "span" of 8 LB, its codes one load of LB bytes.  A span lies in one group:
+// quarter l / 16) takes 2 LB consecutive k of a "span" of 8 LB, whose codes are LB bytes.  A span lies in one group:
 // LB 16 for groups of multiples of 128, 8 for other multiples of 64, 4 for other multiples of 32.
 #include "decode.h"
 
@@ -269,10 +269,10 @@ __device__ __forceinline__ void put8(const GroupArgs& p, int64_t off, int left, 
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
 // 16 MT rows by 16 NC columns a work-group; its 8 waves share out the k in turns of 128, and their sums meet in the LDS.  Codes
-// come by 16 bytes a lane whatever the spans; shorter ones are dealt out among a column's four lanes by swaps of their rows.  A
-// wave takes its turns one after another: what hides their loads is the other waves of the CU (several turns' loads sent out together, or x
-// a span ahead, gained nothing at 4096 -> 4096 and lost up to a half where a wave has few of them, for their registers; 16 waves are
-// 0 to 3 % slower, in fp32 up to 60 %).  16 x 4096 -> 12288, e4m3, groups of 128: 13.7 us (27 MB, 2 TB/s).
+// come by 16 bytes a lane whatever the spans; shorter ones are dealt out among a column's four lanes by swaps of their rows.
+// A wave takes its turns one after another: what hides their loads is the other waves of the CU (two turns' loads sent out
+// together gained nothing at 4096 -> 4096, the next turn loaded ahead lost 2 to 30 %, for its registers; 16 waves are 0 to 3 %
+// slower, in fp32 up to 60 %).  16 x 4096 -> 12288, e4m3, groups of 128: 13.7 us (27 MB, 2 TB/s).
 // Lanes whose row is past M load no x: their sums are not stored.
 constexpr int kFewWaves = 8;
 
